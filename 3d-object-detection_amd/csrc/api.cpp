@@ -64,7 +64,7 @@ bool allow_dynamic_lds(const void *fn, size_t bytes)
 
 extern "C" {
 
-int fpn_abi_version(void) { return 18; }
+int fpn_abi_version(void) { return 19; }
 
 const char *fpn_last_error_string(void) { return fpn::error_buffer(); }
 

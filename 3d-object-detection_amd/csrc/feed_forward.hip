@@ -1,0 +1,484 @@
+// The feed-forward operators' entry points: dense (act(x W + b) + r) and gated (act(x Wg + bg) * (x Wu + bu)),
+// forward and backward, and the element-wise half of the backward pass.  The products are in feed_forward.h.
+#include "feed_forward.h"
+
+namespace fpn {
+namespace ff {
+namespace {
+
+// ---- dpre and the bias gradients --------------------------------------------------------------------------------
+//
+// dense: d = dy act'(pre); gated: dg = dh u act'(g), du = dh act(g).  One pass: every input is read once, d written
+// once, and the column sums (the bias gradients) are taken from the unrounded fp32 values on the way: a thread owns
+// eight columns and every eighth row of its workgroup's rows, the eight row sums meet in LDS in a fixed order and the
+// workgroups' sums in column_join_kernel - no atomics, so a step's gradients repeat bit for bit.
+// Bound by memory.
+struct GradArgs {
+    long rows;
+    int n;
+    const void *dy;
+    long lddy;
+    const void *pre[2];      // null where the activation is the identity
+    long ldp;
+    int act;
+    void *d[2];              // (rows, n) dense, or null: column sums only
+    float *sums;             // (gridDim.y, 1 or 2, n), or null
+    long rows_per_block;
+};
+
+template <class T, bool GATED> __global__ __launch_bounds__(kThreads) void grad_kernel(const GradArgs p)
+{
+    constexpr bool EXACT = sizeof(T) == 4;
+    __shared__ float part[8][32][8];
+    const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
+    const int n = (int)blockIdx.x * 256 + c * 8;
+    const long left = p.n - n;
+    const long m0 = (long)blockIdx.y * p.rows_per_block, m1 = min(m0 + p.rows_per_block, p.rows);
+    float sum[2][8] = {};
+    if (left > 0) {
+        for_activation(p.act, [&](auto tag) {
+            constexpr int ACT = decltype(tag)::value;
+            for (long m = m0 + r; m < m1; m += 8) {
+                float d[8], g[8], u[8], du[8];
+                load8(reinterpret_cast<const T *>(p.dy) + m * p.lddy + n, left, d);
+                if (GATED || ACT != FPN_ACT_NONE) load8(reinterpret_cast<const T *>(p.pre[0]) + m * p.ldp + n, left, g);
+                if (GATED) load8(reinterpret_cast<const T *>(p.pre[1]) + m * p.ldp + n, left, u);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float value = 0.f;
+                    const float slope = ACT == FPN_ACT_NONE && !GATED ? 1.f : activate_grad<ACT, EXACT>(g[i], value);
+                    if (GATED) {
+                        du[i] = d[i] * value;
+                        d[i] = d[i] * u[i] * slope;
+                        sum[1][i] += du[i];
+                    } else {
+                        d[i] *= slope;
+                    }
+                    sum[0][i] += d[i];
+                }
+                if (p.d[0]) {
+                    store8(reinterpret_cast<T *>(p.d[0]) + m * p.n + n, left, d);
+                    if (GATED) store8(reinterpret_cast<T *>(p.d[1]) + m * p.n + n, left, du);
+                }
+            }
+        });
+    }
+    if (!p.sums) return;                                       // (uniform)
+#pragma unroll
+    for (int g = 0; g < (GATED ? 2 : 1); ++g) {
+        if (g) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) part[r][c][i] = sum[g][i];
+        __syncthreads();
+        if (r == 0 && left > 0) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                v[i] = part[0][c][i];
+                for (int s = 1; s < 8; ++s) v[i] += part[s][c][i];
+            }
+            store8(p.sums + ((long)blockIdx.y * (GATED ? 2 : 1) + g) * p.n + n, left, v);
+        }
+    }
+}
+
+// out[j][n] = sum over the workgroups of sums[.][j][n]
+template <class T> __global__ __launch_bounds__(kThreads) void column_join_kernel(int n, int blocks, int planes, const float *sums, T *out0, T *out1)
+{
+    __shared__ float part[8][32];
+    const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
+    const int col = (int)blockIdx.x * 32 + c, j = blockIdx.y;
+    float v = 0.f;
+    if (col < n)
+        for (int s = r; s < blocks; s += 8) v += sums[((long)s * planes + j) * n + col];
+    part[r][c] = v;
+    __syncthreads();
+    if (r || col >= n) return;
+    for (int s = 1; s < 8; ++s) v += part[s][c];
+    (j ? out1 : out0)[col] = (T)v;
+}
+
+int grad_rows_grid(long rows, int n)
+{
+    // 2048 workgroups fill the chip eight deep; a workgroup takes at least 16 rows, and the second pass reads one
+    // fp32 row per workgroup row, so that there are at most 512 of those
+    const long cols = (n + 255) / 256;
+    return (int)std::max(1l, std::min({(rows + 15) / 16, (2048 + cols - 1) / cols, 512l}));
+}
+
+template <class T>
+int launch_grad(GradArgs p, bool gated, void *const (&sums_out)[2], hipStream_t stream)
+{
+    const int gy = grad_rows_grid(p.rows, p.n), gx = (p.n + 255) / 256;
+    p.rows_per_block = (p.rows + gy - 1) / gy;
+    if (gated) hipLaunchKernelGGL((grad_kernel<T, true>), dim3(gx, gy), dim3(kThreads), 0, stream, p);
+    else hipLaunchKernelGGL((grad_kernel<T, false>), dim3(gx, gy), dim3(kThreads), 0, stream, p);
+    int rc = check_launch("feed-forward gradient");
+    if (rc != FPN_OK || !p.sums) return rc;
+    hipLaunchKernelGGL((column_join_kernel<T>), dim3((p.n + 31) / 32, gated ? 2 : 1), dim3(kThreads), 0, stream, p.n, gy, gated ? 2 : 1,
+                       p.sums, reinterpret_cast<T *>(sums_out[0]), reinterpret_cast<T *>(sums_out[1]));
+    return check_launch("bias gradient");
+}
+
+// ---- host side --------------------------------------------------------------------------------------------------
+
+int element_size(int dtype) { return dtype == FPN_F32 ? 4 : 2; }
+
+size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+int run_product(int dtype, const Args &p, int order_a, int order_b, bool gated, float *partial, size_t partial_bytes, hipStream_t stream)
+{
+    const Plan plan = plan_product(dtype, p.m, p.n, p.k, p.segs, p.batch, gated);
+    if (plan.partial_bytes > partial_bytes)
+        return fail(FPN_E_INVALID_ARG, "workspace: %zu bytes of partial sums needed, %zu there", plan.partial_bytes, partial_bytes);
+    if (dtype == FPN_F32) return launch_product<float>(p, order_a, order_b, gated, plan, partial, stream);
+    if (dtype == FPN_BF16) return launch_product<__bf16>(p, order_a, order_b, gated, plan, partial, stream);
+    return launch_product<_Float16>(p, order_a, order_b, gated, plan, partial, stream);
+}
+
+constexpr long kMostLd = (1l << 21) - 1;      // a tile's byte offsets inside an operand are 32 bits
+
+int check_common(int dtype, long rows, int cin, int cout, int activation)
+{
+    FPN_REQUIRE(dtype == FPN_F32 || dtype == FPN_BF16 || dtype == FPN_F16, "dtype %d is none of FPN_F32, FPN_BF16, FPN_F16", dtype);
+    FPN_REQUIRE(rows >= 0 && cin >= 1 && cout >= 1, "rows %ld, cin %d, cout %d: rows >= 0 and widths >= 1 are needed", rows, cin, cout);
+    FPN_REQUIRE(activation >= FPN_ACT_NONE && activation <= FPN_ACT_GELU_TANH, "unknown activation %d", activation);
+    if (cin > kMostLd || cout > kMostLd) return fail(FPN_E_UNSUPPORTED, "widths up to %ld are supported, got %d and %d", kMostLd, cin, cout);
+    return FPN_OK;
+}
+
+// a matrix argument: present, its rows apart by at least `width` (0: any stride, one row repeated) and addressable
+int check_matrix(const char *name, const void *p, long ld, long width, int dtype, bool broadcast = false)
+{
+    FPN_REQUIRE(p, "%s is null", name);
+    FPN_REQUIRE(reinterpret_cast<uintptr_t>(p) % element_size(dtype) == 0, "%s is not aligned to its elements", name);
+    FPN_REQUIRE(ld >= width || (broadcast && ld == 0), "%s: row stride %ld is less than its %ld columns", name, ld, width);
+    if (ld > kMostLd) return fail(FPN_E_UNSUPPORTED, "%s: row stride %ld is over %ld elements", name, ld, kMostLd);
+    return FPN_OK;
+}
+
+int check_vector(const char *name, const void *p, int dtype)
+{
+    FPN_REQUIRE(!p || reinterpret_cast<uintptr_t>(p) % element_size(dtype) == 0, "%s is not aligned to its elements", name);
+    return FPN_OK;
+}
+
+int check_workspace(const void *ws, size_t have, size_t need)
+{
+    FPN_REQUIRE(need == 0 || (ws && have >= need), "workspace of %zu bytes needed, got %zu", need, ws ? have : 0);
+    FPN_REQUIRE(reinterpret_cast<uintptr_t>(ws) % 16 == 0, "workspace must be 16-byte aligned");
+    return FPN_OK;
+}
+
+#define FPN_FF_TRY(call)                \
+    do {                                \
+        const int rc_ = (call);         \
+        if (rc_ != FPN_OK) return rc_;  \
+    } while (0)
+
+// The parts of a backward pass' workspace: dpre (one matrix, or two where gated), the workgroups' column sums, and
+// the partial sums of dx and dw, which run one after the other
+struct GradSpace {
+    size_t d, sums, partial, total;
+};
+GradSpace grad_space(int dtype, long rows, int cin, int n, bool gated, bool with_d)
+{
+    GradSpace s;
+    const int planes = gated ? 2 : 1;
+    s.d = with_d ? align256((size_t)rows * n * element_size(dtype)) * planes : 0;
+    s.sums = align256((size_t)grad_rows_grid(rows, n) * planes * n * sizeof(float));
+    const Plan dx = plan_product(dtype, rows, cin, n, planes, 1, false);
+    const Plan dw = plan_product(dtype, cin, n, rows, 1, planes, false), dwt = plan_product(dtype, n, cin, rows, 1, planes, false);
+    s.partial = align256(std::max({dx.partial_bytes, dw.partial_bytes, dwt.partial_bytes}));
+    s.total = s.d + s.sums + s.partial;
+    return s;
+}
+
+Args product(long m, int n, long k)
+{
+    Args p = {};
+    p.m = m;
+    p.n = n;
+    p.k = k;
+    p.segs = 1;
+    p.batch = 1;
+    p.act = FPN_ACT_NONE;
+    return p;
+}
+
+// dw = x^T d for one or two d, in the weights' own storage order
+int weight_gradients(int dtype, long rows, int cin, int n, const void *x, long ldx, const void *const (&d)[2], long ldd, int members,
+                     void *const (&dw)[2], long lddw, int transposed, float *partial, size_t partial_bytes, hipStream_t stream)
+{
+    if (!transposed) {
+        Args p = product(cin, n, rows);
+        p.a[0] = x;
+        p.lda[0] = ldx;
+        p.batch = members;
+        for (int i = 0; i < members; ++i) { p.b[i] = d[i]; p.ldb[i] = ldd; p.c[i] = dw[i]; }
+        p.ldc = lddw;
+        return run_product(dtype, p, kOuter, kOuter, false, partial, partial_bytes, stream);
+    }
+    // held (out,in): the operands change places (one product each, x is the b side of both)
+    for (int i = 0; i < members; ++i) {
+        Args p = product(n, cin, rows);
+        p.a[0] = d[i];
+        p.lda[0] = ldd;
+        p.b[0] = x;
+        p.ldb[0] = ldx;
+        p.c[0] = dw[i];
+        p.ldc = lddw;
+        FPN_FF_TRY(run_product(dtype, p, kOuter, kOuter, false, partial, partial_bytes, stream));
+    }
+    return FPN_OK;
+}
+
+int run_grad(int dtype, const GradArgs &p, bool gated, void *const (&sums_out)[2], hipStream_t stream)
+{
+    if (dtype == FPN_F32) return launch_grad<float>(p, gated, sums_out, stream);
+    if (dtype == FPN_BF16) return launch_grad<__bf16>(p, gated, sums_out, stream);
+    return launch_grad<_Float16>(p, gated, sums_out, stream);
+}
+
+}  // namespace
+
+Plan plan_product(int dtype, long m, int n, long k, int segs, int batch, bool gated)
+{
+    Plan p;
+    const int bk = kTileBytes / element_size(dtype);
+    const long kt = (k + bk - 1) / bk * segs;
+    auto tiles = [&](int bm, int bn) { return (m + bm - 1) / bm * ((n + (gated ? bn / 2 : bn) - 1) / (gated ? bn / 2 : bn)) * batch; };
+    p.bm = m > 64 && tiles(128, 128) >= 256 ? 128 : 64;
+    p.bn = 128;
+    const long t = std::max(1l, tiles(p.bm, p.bn));
+    // too few tiles for the chip: k is split so that about 512 workgroups run, each with at least four k tiles
+    long splits = t >= 256 ? 1 : std::max(1l, std::min({512 / t, kt / 4, 256l}));
+    p.tiles_per_split = std::max(1l, (kt + splits - 1) / splits);
+    splits = std::max(1l, (kt + p.tiles_per_split - 1) / p.tiles_per_split);
+    p.splits = (int)splits;
+    p.partial_bytes = splits > 1 ? (size_t)splits * batch * (gated ? 2 : 1) * m * n * sizeof(float) : 0;
+    return p;
+}
+
+}  // namespace ff
+}  // namespace fpn
+
+using namespace fpn;
+using namespace fpn::ff;
+
+extern "C" {
+
+size_t fpn_dense_workspace_bytes(int dtype, long rows, int cin, int cout)
+{
+    if (check_common(dtype, rows, cin, cout, FPN_ACT_NONE) != FPN_OK) return 0;
+    return plan_product(dtype, rows, cout, cin, 1, 1, false).partial_bytes;
+}
+
+int fpn_dense(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w, long ldw, int w_transposed,
+              const void *bias, int activation, const void *residual, long ldr, void *y, long ldy, void *pre, long ldp,
+              void *workspace, size_t workspace_bytes, void *stream)
+{
+    FPN_FF_TRY(check_common(dtype, rows, cin, cout, activation));
+    if (rows == 0) return FPN_OK;
+    FPN_FF_TRY(check_matrix("x", x, ldx, cin, dtype, true));
+    FPN_FF_TRY(check_matrix("w", w, ldw, w_transposed ? cin : cout, dtype));
+    FPN_FF_TRY(check_matrix("y", y, ldy, cout, dtype));
+    FPN_FF_TRY(check_vector("bias", bias, dtype));
+    if (residual) FPN_FF_TRY(check_matrix("residual", residual, ldr, cout, dtype, true));
+    if (pre) FPN_FF_TRY(check_matrix("pre", pre, ldp, cout, dtype));
+    FPN_FF_TRY(check_workspace(workspace, workspace_bytes, fpn_dense_workspace_bytes(dtype, rows, cin, cout)));
+    Args p = product(rows, cout, cin);
+    p.a[0] = x;
+    p.lda[0] = ldx;
+    p.b[0] = w;
+    p.ldb[0] = ldw;
+    p.bias[0] = bias;
+    p.act = activation;
+    p.residual = residual;
+    p.ldr = ldr;
+    p.c[0] = y;
+    p.ldc = ldy;
+    p.pre[0] = pre;
+    p.ldp = ldp;
+    return run_product(dtype, p, kInner, w_transposed ? kInner : kOuter, false, reinterpret_cast<float *>(workspace), workspace_bytes,
+                       as_stream(stream));
+}
+
+size_t fpn_dense_grad_workspace_bytes(int dtype, long rows, int cin, int cout, int activation)
+{
+    if (check_common(dtype, rows, cin, cout, activation) != FPN_OK) return 0;
+    return grad_space(dtype, rows, cin, cout, false, activation != FPN_ACT_NONE).total;
+}
+
+int fpn_dense_grad(int dtype, long rows, int cin, int cout, const void *dy, long lddy, const void *x, long ldx, const void *w,
+                   long ldw, int w_transposed, const void *pre, long ldp, int activation, void *dx, long lddx, void *dw, long lddw,
+                   void *dbias, void *workspace, size_t workspace_bytes, void *stream)
+{
+    FPN_FF_TRY(check_common(dtype, rows, cin, cout, activation));
+    const bool act = activation != FPN_ACT_NONE;
+    if (rows > 0) {
+        FPN_FF_TRY(check_matrix("dy", dy, lddy, cout, dtype));
+        if (act) FPN_FF_TRY(check_matrix("pre", pre, ldp, cout, dtype));
+        if (dw) FPN_FF_TRY(check_matrix("x", x, ldx, cin, dtype, true));
+        if (dx) FPN_FF_TRY(check_matrix("w", w, ldw, w_transposed ? cin : cout, dtype));
+        if (dx) FPN_FF_TRY(check_matrix("dx", dx, lddx, cin, dtype));
+    }
+    if (dw) FPN_FF_TRY(check_matrix("dw", dw, lddw, w_transposed ? cin : cout, dtype));
+    FPN_FF_TRY(check_vector("dbias", dbias, dtype));
+    const GradSpace space = grad_space(dtype, rows, cin, cout, false, act);
+    FPN_FF_TRY(check_workspace(workspace, workspace_bytes, space.total));
+    char *ws = reinterpret_cast<char *>(workspace);
+    float *partial = reinterpret_cast<float *>(ws + space.d + space.sums);
+    const hipStream_t st = as_stream(stream);
+
+    const void *d[2] = {dy, nullptr};
+    long ldd = lddy;
+    if (act || dbias) {
+        GradArgs g = {};
+        g.rows = rows;
+        g.n = cout;
+        g.dy = dy;
+        g.lddy = lddy;
+        g.pre[0] = pre;
+        g.ldp = ldp;
+        g.act = activation;
+        if (act) {
+            g.d[0] = ws;
+            d[0] = ws;
+            ldd = cout;
+        }
+        g.sums = dbias ? reinterpret_cast<float *>(ws + space.d) : nullptr;
+        void *const out[2] = {dbias, nullptr};
+        FPN_FF_TRY(run_grad(dtype, g, false, out, st));
+    }
+    if (dx && rows > 0) {
+        Args p = product(rows, cin, cout);
+        p.a[0] = d[0];
+        p.lda[0] = ldd;
+        p.b[0] = w;
+        p.ldb[0] = ldw;
+        p.c[0] = dx;
+        p.ldc = lddx;
+        FPN_FF_TRY(run_product(dtype, p, kInner, w_transposed ? kOuter : kInner, false, partial, space.partial, st));
+    }
+    if (dw) {
+        void *const out[2] = {dw, nullptr};
+        FPN_FF_TRY(weight_gradients(dtype, rows, cin, cout, x, ldx, d, ldd, 1, out, lddw, w_transposed, partial, space.partial, st));
+    }
+    return FPN_OK;
+}
+
+size_t fpn_gated_workspace_bytes(int dtype, long rows, int cin, int cout)
+{
+    if (check_common(dtype, rows, cin, cout, FPN_ACT_NONE) != FPN_OK) return 0;
+    return plan_product(dtype, rows, cout, cin, 1, 1, true).partial_bytes;
+}
+
+int fpn_gated(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w_gate, long ldg, const void *w_up, long ldu,
+              int w_transposed, const void *bias_gate, const void *bias_up, int activation, void *h, long ldh, void *gate, void *up,
+              long ldp, void *workspace, size_t workspace_bytes, void *stream)
+{
+    FPN_FF_TRY(check_common(dtype, rows, cin, cout, activation));
+    FPN_REQUIRE(!gate == !up, "gate and up are kept together or not at all");
+    if (rows == 0) return FPN_OK;
+    FPN_FF_TRY(check_matrix("x", x, ldx, cin, dtype, true));
+    FPN_FF_TRY(check_matrix("w_gate", w_gate, ldg, w_transposed ? cin : cout, dtype));
+    FPN_FF_TRY(check_matrix("w_up", w_up, ldu, w_transposed ? cin : cout, dtype));
+    FPN_FF_TRY(check_matrix("h", h, ldh, cout, dtype));
+    FPN_FF_TRY(check_vector("bias_gate", bias_gate, dtype));
+    FPN_FF_TRY(check_vector("bias_up", bias_up, dtype));
+    if (gate) FPN_FF_TRY(check_matrix("gate", gate, ldp, cout, dtype));
+    if (up) FPN_FF_TRY(check_matrix("up", up, ldp, cout, dtype));
+    FPN_FF_TRY(check_workspace(workspace, workspace_bytes, fpn_gated_workspace_bytes(dtype, rows, cin, cout)));
+    Args p = product(rows, cout, cin);
+    p.a[0] = x;
+    p.lda[0] = ldx;
+    p.b[0] = w_gate;
+    p.b[1] = w_up;
+    p.ldb[0] = ldg;
+    p.ldb[1] = ldu;
+    p.bias[0] = bias_gate;
+    p.bias[1] = bias_up;
+    p.act = activation;
+    p.c[0] = h;
+    p.ldc = ldh;
+    p.pre[0] = gate;
+    p.pre[1] = up;
+    p.ldp = ldp;
+    return run_product(dtype, p, kInner, w_transposed ? kInner : kOuter, true, reinterpret_cast<float *>(workspace), workspace_bytes,
+                       as_stream(stream));
+}
+
+size_t fpn_gated_grad_workspace_bytes(int dtype, long rows, int cin, int cout)
+{
+    if (check_common(dtype, rows, cin, cout, FPN_ACT_NONE) != FPN_OK) return 0;
+    return grad_space(dtype, rows, cin, cout, true, true).total;
+}
+
+int fpn_gated_grad(int dtype, long rows, int cin, int cout, const void *dh, long lddh, const void *x, long ldx, const void *w_gate,
+                   long ldg, const void *w_up, long ldu, int w_transposed, const void *gate, const void *up, long ldp, int activation,
+                   void *dx, long lddx, void *dw_gate, void *dw_up, long lddw, void *dbias_gate, void *dbias_up, void *workspace,
+                   size_t workspace_bytes, void *stream)
+{
+    FPN_FF_TRY(check_common(dtype, rows, cin, cout, activation));
+    FPN_REQUIRE(!dw_gate == !dw_up && !dbias_gate == !dbias_up, "the gradients of gate and up are wanted together or not at all");
+    if (rows > 0) {
+        FPN_FF_TRY(check_matrix("dh", dh, lddh, cout, dtype));
+        FPN_FF_TRY(check_matrix("gate", gate, ldp, cout, dtype));
+        FPN_FF_TRY(check_matrix("up", up, ldp, cout, dtype));
+        if (dw_gate) FPN_FF_TRY(check_matrix("x", x, ldx, cin, dtype, true));
+        if (dx) {
+            FPN_FF_TRY(check_matrix("w_gate", w_gate, ldg, w_transposed ? cin : cout, dtype));
+            FPN_FF_TRY(check_matrix("w_up", w_up, ldu, w_transposed ? cin : cout, dtype));
+            FPN_FF_TRY(check_matrix("dx", dx, lddx, cin, dtype));
+        }
+    }
+    if (dw_gate) {
+        FPN_FF_TRY(check_matrix("dw_gate", dw_gate, lddw, w_transposed ? cin : cout, dtype));
+        FPN_FF_TRY(check_matrix("dw_up", dw_up, lddw, w_transposed ? cin : cout, dtype));
+    }
+    FPN_FF_TRY(check_vector("dbias_gate", dbias_gate, dtype));
+    FPN_FF_TRY(check_vector("dbias_up", dbias_up, dtype));
+    const GradSpace space = grad_space(dtype, rows, cin, cout, true, true);
+    FPN_FF_TRY(check_workspace(workspace, workspace_bytes, space.total));
+    char *ws = reinterpret_cast<char *>(workspace);
+    float *partial = reinterpret_cast<float *>(ws + space.d + space.sums);
+    const hipStream_t st = as_stream(stream);
+
+    GradArgs g = {};
+    g.rows = rows;
+    g.n = cout;
+    g.dy = dh;
+    g.lddy = lddh;
+    g.pre[0] = gate;
+    g.pre[1] = up;
+    g.ldp = ldp;
+    g.act = activation;
+    g.d[0] = ws;
+    g.d[1] = ws + space.d / 2;
+    g.sums = dbias_gate ? reinterpret_cast<float *>(ws + space.d) : nullptr;
+    void *const sums_out[2] = {dbias_gate, dbias_up};
+    FPN_FF_TRY(run_grad(dtype, g, true, sums_out, st));
+    if (dx && rows > 0) {                         // dg Wg^T + du Wu^T: one sum over both
+        Args p = product(rows, cin, cout);
+        p.segs = 2;
+        p.a[0] = g.d[0];
+        p.a[1] = g.d[1];
+        p.lda[0] = p.lda[1] = cout;
+        p.b[0] = w_gate;
+        p.b[1] = w_up;
+        p.ldb[0] = ldg;
+        p.ldb[1] = ldu;
+        p.c[0] = dx;
+        p.ldc = lddx;
+        FPN_FF_TRY(run_product(dtype, p, kInner, w_transposed ? kOuter : kInner, false, partial, space.partial, st));
+    }
+    if (dw_gate) {
+        const void *const d[2] = {g.d[0], g.d[1]};
+        void *const out[2] = {dw_gate, dw_up};
+        FPN_FF_TRY(weight_gradients(dtype, rows, cin, cout, x, ldx, d, cout, 2, out, lddw, w_transposed, partial, space.partial, st));
+    }
+    return FPN_OK;
+}
+
+}  // extern "C"

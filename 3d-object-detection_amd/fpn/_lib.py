@@ -16,7 +16,7 @@ LIB_PATH = os.path.abspath(os.environ["FPN_LIB_PATH"]) if os.environ.get("FPN_LI
 
 FPN_OK = 0
 STATIC_SCRATCH_BYTES = 8 << 20   # FPN_STATIC_SCRATCH_BYTES of include/fpn.h
-ABI_VERSION = 18
+ABI_VERSION = 19
 
 
 class FpnError(RuntimeError):
@@ -88,7 +88,21 @@ SIGNATURES = {
     "fpn_box3d_intersection_f64": [_l, _vp, _l, _vp, _l, _vp, _vp, _vp],
     "fpn_box3d_best_overlap_f64": [_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
     "fpn_detection_records": [_i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "fpn_dense": [_i, _l, _i, _i, _vp, _l, _vp, _l, _i, _vp, _i, _vp, _l, _vp, _l, _vp, _l, _vp, _sz, _vp],
+    "fpn_dense_grad": [_i, _l, _i, _i, _vp, _l, _vp, _l, _vp, _l, _i, _vp, _l, _i, _vp, _l, _vp, _l, _vp, _vp, _sz, _vp],
+    "fpn_gated": [_i, _l, _i, _i, _vp, _l, _vp, _l, _vp, _l, _i, _vp, _vp, _i, _vp, _l, _vp, _vp, _l, _vp, _sz, _vp],
+    "fpn_gated_grad": [_i, _l, _i, _i, _vp, _l, _vp, _l, _vp, _l, _vp, _l, _i, _vp, _vp, _l, _i, _vp, _l, _vp, _vp, _l, _vp, _vp,
+                       _vp, _sz, _vp],
     "fpn_mask_gather": [_i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+}
+
+# functions that return a size
+SIZES = {
+    "fpn_shared_mlp_workspace_bytes": [_l, _i, _i],
+    "fpn_dense_workspace_bytes": [_i, _l, _i, _i],
+    "fpn_dense_grad_workspace_bytes": [_i, _l, _i, _i, _i],
+    "fpn_gated_workspace_bytes": [_i, _l, _i, _i],
+    "fpn_gated_grad_workspace_bytes": [_i, _l, _i, _i],
 }
 
 _lib = None
@@ -107,8 +121,10 @@ def load():
     lib = ctypes.CDLL(LIB_PATH)
     lib.fpn_abi_version.restype = _i
     lib.fpn_last_error_string.restype = ctypes.c_char_p
-    lib.fpn_shared_mlp_workspace_bytes.restype = _sz
-    lib.fpn_shared_mlp_workspace_bytes.argtypes = [_l, _i, _i]
+    for name, argtypes in SIZES.items():
+        fn = getattr(lib, name)
+        fn.restype = _sz
+        fn.argtypes = argtypes
     lib.fpn_ball_threshold.restype = _f
     lib.fpn_ball_threshold.argtypes = [_f]
     for name, argtypes in SIGNATURES.items():

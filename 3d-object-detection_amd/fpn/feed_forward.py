@@ -1,0 +1,346 @@
+"""Feed-forward operators: products with bias, activation and residual in the epilogue, and gated blocks, forward and
+backward, through libfpn_hip.so (fpn_dense, fpn_dense_grad, fpn_gated, fpn_gated_grad; include/fpn.h).
+
+    dense               y = act(x w + bias) + residual
+    gated               h = act(x w_gate + bias_gate) * (x w_up + bias_up)
+    gated_feed_forward  y = gated(x) w_down + bias_down + residual
+
+They stand beside `ops.shared_mlp` (fp32, scale / shift / ReLU, pooling): every tensor of a call is float32, bfloat16
+or float16, sums are fp32, weights are (in, out) - or the `.t()` view of weights held (out, in) -, rows may lie apart
+(column slices of wider buffers).  Work is enqueued on the current stream of the tensors' device; nothing synchronises.
+
+Gradients, either way:
+  * tensors that require gradients: the calls are recorded by autograd;
+  * `keep=True` returns what the backward pass needs beside the result, and `dense_grad` / `gated_grad` are that pass.
+    This is the form for HIP graphs: recording through autograd while a graph is being captured is refused, since
+    autograd would join streams that the capture does not know.
+"""
+import torch
+
+from . import _lib
+
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "sigmoid": 3, "gelu": 4, "gelu_tanh": 5}
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _activation(name):
+    try:
+        return ACTIVATIONS[name]
+    except (KeyError, TypeError):
+        raise ValueError("activation must be one of %s, got %r" % (", ".join(repr(a) for a in ACTIVATIONS), name)) from None
+
+
+def _tensor(name, t, like, shape):
+    """The checks that every argument gets: a tensor of the call's type, on its device, of this shape."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a torch.Tensor, got %s" % (name, type(t).__name__))
+    if not t.is_cuda:
+        raise ValueError("%s must live on a ROCm device (got %s); this package has no CPU path" % (name, t.device))
+    if like is not None:
+        if t.dtype != like.dtype:
+            raise ValueError("%s must be %s like x, got %s" % (name, like.dtype, t.dtype))
+        if t.device != like.device:
+            raise ValueError("all tensors must be on the same device (%s is on %s, x on %s)" % (name, t.device, like.device))
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError("%s has shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
+
+
+def _first(name, x):
+    if not isinstance(x, torch.Tensor):
+        raise TypeError("%s must be a torch.Tensor, got %s" % (name, type(x).__name__))
+    if x.dim() != 2:
+        raise ValueError("%s must have rank 2, got shape %s" % (name, tuple(x.shape)))
+    if x.dtype not in _DTYPES:
+        raise ValueError("%s must be float32, bfloat16 or float16, got %s" % (name, x.dtype))
+    _tensor(name, x, None, x.shape)
+    return _DTYPES[x.dtype]
+
+
+def _rows(name, t, broadcast=False):
+    """The row stride of a matrix whose rows are dense (broadcast: one row may stand for all)."""
+    rows, cols = t.shape
+    if cols > 1 and t.stride(1) != 1:
+        raise ValueError("%s must have unit column stride, got strides %s" % (name, t.stride()))
+    if rows <= 1:
+        return cols
+    ld = t.stride(0)
+    if ld < cols and not (broadcast and ld == 0):
+        raise ValueError("%s: rows %d elements apart overlap (%d columns)" % (name, ld, cols))
+    return ld
+
+
+def _orders(w):
+    """The storage orders a weight matrix can be read in: {transposed: row stride}."""
+    cin, cout = w.shape
+    found = {}
+    if (cout == 1 or w.stride(1) == 1) and (cin == 1 or w.stride(0) >= cout):
+        found[0] = w.stride(0) if cin > 1 else cout
+    if (cin == 1 or w.stride(0) == 1) and (cout == 1 or w.stride(1) >= cin):
+        found[1] = w.stride(1) if cout > 1 else cin
+    return found
+
+
+def _weights(names, ws):
+    """(transposed, row strides) of weights that are all (in, out) matrices or all transposed views of (out, in)."""
+    orders = [_orders(w) for w in ws]
+    for order in (0, 1):
+        if all(order in o for o in orders):
+            return order, [o[order] for o in orders]
+    raise ValueError("%s must be dense (in, out) matrices or transposed views of dense (out, in) ones%s, got strides %s"
+                     % (" and ".join(names), ", both the same" if len(ws) > 1 else "", ", ".join(str(w.stride()) for w in ws)))
+
+
+def _vector(name, t, like, n):
+    if t is None:
+        return
+    _tensor(name, t, like, (n,))
+    if not t.is_contiguous():
+        raise ValueError("%s must be contiguous" % name)
+
+
+def _overlap(a, b):
+    """Whether two row matrices share an element (column slices of one buffer do not)."""
+    if not a.numel() or not b.numel():
+        return False
+    size = a.element_size()
+    first = [t.data_ptr() for t in (a, b)]
+    end = [p + ((t.shape[0] - 1) * t.stride(0) + (t.shape[1] - 1) * t.stride(1) + 1) * size for p, t in zip(first, (a, b))]
+    if end[0] <= first[1] or end[1] <= first[0]:
+        return False
+    if a.shape[0] > 1 and b.shape[0] > 1 and a.stride() == b.stride() and a.stride(1) == 1:
+        ld = a.stride(0)
+        apart, odd = divmod(first[1] - first[0], size)
+        at = apart % ld
+        if not odd and at >= a.shape[1] and at + b.shape[1] <= ld:
+            return False
+    return True
+
+
+def _output(out, x, rows, cols, inputs, may_be=None):
+    """`out` or a new tensor, and its row stride."""
+    if out is None:
+        return torch.empty((rows, cols), dtype=x.dtype, device=x.device), cols
+    _tensor("out", out, x, (rows, cols))
+    ld = _rows("out", out)
+    for name, t in inputs:
+        t2 = t if t is None or t.dim() == 2 else t.unsqueeze(0)
+        if t2 is not None and _overlap(out, t2):
+            raise ValueError("out shares memory with %s" % name)
+    if may_be is not None and not (out.data_ptr() == may_be.data_ptr() and out.stride() == may_be.stride()) and _overlap(out, may_be):
+        raise ValueError("out shares memory with residual without being it")
+    return out, ld
+
+
+def _workspace(size, x):
+    """A call's own scratch memory, from torch's allocator on the current stream: calls on other streams and in captured
+    graphs have theirs."""
+    return (None, 0) if not size else (torch.empty(size, dtype=torch.uint8, device=x.device), size)
+
+
+def _call(x, name, *args):
+    lib = _lib.load()
+    if torch.cuda.current_device() == x.device.index:
+        _lib.check(getattr(lib, name)(*args, _lib.stream_of(x)))
+    else:
+        with torch.cuda.device(x.device):
+            _lib.check(getattr(lib, name)(*args, _lib.stream_of(x)))
+
+
+def _recorded(*tensors):
+    """Whether autograd has to see the call."""
+    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
+        return False
+    _no_capture()
+    return True
+
+
+def _no_capture():
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("a call on tensors that require gradients cannot be captured into a graph: use keep=True and "
+                           "dense_grad / gated_grad (or torch.no_grad())")
+
+
+# ---- dense ---------------------------------------------------------------------------------------------------------
+
+def dense(x, w, bias=None, activation=None, residual=None, out=None, keep=False):
+    """y = act(x w + bias) + residual: x (rows, cin), w (cin, cout), bias (cout,), residual and y (rows, cout).
+
+    activation: None, "relu", "silu", "sigmoid", "gelu" (exact) or "gelu_tanh".  `out` receives y (it may be the
+    residual itself, but share memory with no other argument).  keep=True returns (y, pre) for `dense_grad`, pre
+    being x w + bias in x's type, or None where there is no activation."""
+    dtype = _first("x", x)
+    act = _activation(activation)
+    rows, cin = x.shape
+    if not isinstance(w, torch.Tensor) or w.dim() != 2:
+        raise ValueError("w must be a (cin, cout) tensor")
+    cout = w.shape[1]
+    _tensor("w", w, x, (cin, cout))
+    _vector("bias", bias, x, cout)
+    if residual is not None:
+        _tensor("residual", residual, x, (rows, cout))
+    if not keep and _recorded(x, w, bias, residual):
+        if out is not None:
+            raise ValueError("out cannot be given for tensors that require gradients")
+        return _Dense.apply(x, w, bias, activation, residual)
+    ldx = _rows("x", x, broadcast=True)
+    transposed, (ldw,) = _weights(("w",), (w,))
+    ldr = _rows("residual", residual, broadcast=True) if residual is not None else 0
+    y, ldy = _output(out, x, rows, cout, (("x", x), ("w", w), ("bias", bias)), residual)
+    pre = torch.empty((rows, cout), dtype=x.dtype, device=x.device) if keep and act else None
+    ws, size = _workspace(_lib.load().fpn_dense_workspace_bytes(dtype, rows, cin, cout), x)
+    p = _lib.ptr
+    _call(x, "fpn_dense", dtype, rows, cin, cout, p(x), ldx, p(w), ldw, transposed, p(bias), act, p(residual), ldr, p(y), ldy,
+          p(pre), cout, p(ws), size)
+    return (y, pre) if keep else y
+
+
+def dense_grad(dy, x, w, pre=None, activation=None, bias=False, need_x=True, need_w=True):
+    """The gradients of `dense`: (dx, dw, dbias), each None where it is not asked for (bias=True asks for dbias); dw is
+    stored as w is.  `pre` is what keep=True returned.  The residual's gradient is dy."""
+    dtype = _first("x", x)
+    act = _activation(activation)
+    rows, cin = x.shape
+    if not isinstance(w, torch.Tensor) or w.dim() != 2:
+        raise ValueError("w must be a (cin, cout) tensor")
+    cout = w.shape[1]
+    _tensor("w", w, x, (cin, cout))
+    _tensor("dy", dy, x, (rows, cout))
+    lddy, ldx = _rows("dy", dy), _rows("x", x, broadcast=True)
+    transposed, (ldw,) = _weights(("w",), (w,))
+    ldp = cout
+    if act:
+        if pre is None:
+            raise ValueError("pre (from dense(..., keep=True)) is needed where there is an activation")
+        _tensor("pre", pre, x, (rows, cout))
+        ldp = _rows("pre", pre)
+    with torch.no_grad():
+        dx = torch.empty((rows, cin), dtype=x.dtype, device=x.device) if need_x else None
+        dw = _like_weights(w, transposed) if need_w else None
+        db = torch.empty(cout, dtype=x.dtype, device=x.device) if bias else None
+    ws, size = _workspace(_lib.load().fpn_dense_grad_workspace_bytes(dtype, rows, cin, cout, act), x)
+    p = _lib.ptr
+    _call(x, "fpn_dense_grad", dtype, rows, cin, cout, p(dy), lddy, p(x), ldx, p(w), ldw, transposed, p(pre) if act else None, ldp,
+          act, p(dx), cin, p(dw), cin if transposed else cout, p(db), p(ws), size)
+    return dx, dw, db
+
+
+def _like_weights(w, transposed):
+    cin, cout = w.shape
+    if transposed:
+        return torch.empty((cout, cin), dtype=w.dtype, device=w.device).t()
+    return torch.empty((cin, cout), dtype=w.dtype, device=w.device)
+
+
+def _dense_rows(t):
+    """A gradient as autograd hands it over (it may be an expanded or transposed view), with dense rows."""
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        return t.contiguous()
+    return t
+
+
+class _Dense(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, activation, residual):
+        y, pre = dense(x, w, bias, activation, residual, keep=True)
+        ctx.save_for_backward(x, w, pre)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        _no_capture()
+        x, w, pre = ctx.saved_tensors
+        need_x, need_w, need_b, _, need_r = ctx.needs_input_grad
+        dx = dw = db = None
+        if need_x or need_w or need_b:
+            dx, dw, db = dense_grad(_dense_rows(dy), x, w, pre, ctx.activation, need_b, need_x, need_w)
+        return dx, dw, db, None, dy if need_r else None
+
+
+# ---- gated ---------------------------------------------------------------------------------------------------------
+
+def _check_gated(x, w_gate, w_up):
+    dtype = _first("x", x)
+    for name, w in (("w_gate", w_gate), ("w_up", w_up)):
+        if not isinstance(w, torch.Tensor) or w.dim() != 2:
+            raise ValueError("%s must be a (cin, cout) tensor" % name)
+        _tensor(name, w, x, (x.shape[1], w_gate.shape[1]))
+    return dtype, x.shape[0], x.shape[1], w_gate.shape[1]
+
+
+def gated(x, w_gate, w_up, bias_gate=None, bias_up=None, activation="silu", out=None, keep=False):
+    """h = act(x w_gate + bias_gate) * (x w_up + bias_up) in one kernel: x (rows, cin), weights (cin, cout) - both the
+    same way round, columns of one matrix will do -, biases (cout,), h (rows, cout).
+
+    `out` receives h (it may share memory with no argument).  keep=True returns (h, gate, up) for `gated_grad`, the two
+    sums in x's type."""
+    dtype, rows, cin, cout = _check_gated(x, w_gate, w_up)
+    act = _activation(activation)
+    _vector("bias_gate", bias_gate, x, cout)
+    _vector("bias_up", bias_up, x, cout)
+    if not keep and _recorded(x, w_gate, w_up, bias_gate, bias_up):
+        if out is not None:
+            raise ValueError("out cannot be given for tensors that require gradients")
+        return _Gated.apply(x, w_gate, w_up, bias_gate, bias_up, activation)
+    ldx = _rows("x", x, broadcast=True)
+    transposed, (ldg, ldu) = _weights(("w_gate", "w_up"), (w_gate, w_up))
+    h, ldh = _output(out, x, rows, cout, (("x", x), ("w_gate", w_gate), ("w_up", w_up), ("bias_gate", bias_gate), ("bias_up", bias_up)))
+    gate = up = None
+    if keep:
+        gate, up = (torch.empty((rows, cout), dtype=x.dtype, device=x.device) for _ in range(2))
+    ws, size = _workspace(_lib.load().fpn_gated_workspace_bytes(dtype, rows, cin, cout), x)
+    p = _lib.ptr
+    _call(x, "fpn_gated", dtype, rows, cin, cout, p(x), ldx, p(w_gate), ldg, p(w_up), ldu, transposed, p(bias_gate), p(bias_up), act,
+          p(h), ldh, p(gate), p(up), cout, p(ws), size)
+    return (h, gate, up) if keep else h
+
+
+def gated_grad(dh, x, w_gate, w_up, gate, up, activation="silu", bias=False, need_x=True, need_w=True):
+    """The gradients of `gated`: (dx, dw_gate, dw_up, dbias_gate, dbias_up), each None where it is not asked for
+    (bias=True asks for the last two).  `gate` and `up` are what keep=True returned."""
+    dtype, rows, cin, cout = _check_gated(x, w_gate, w_up)
+    act = _activation(activation)
+    for name, t in (("dh", dh), ("gate", gate), ("up", up)):
+        _tensor(name, t, x, (rows, cout))
+    lddh, ldx, ldp = _rows("dh", dh), _rows("x", x, broadcast=True), _rows("gate", gate)
+    if _rows("up", up) != ldp:
+        raise ValueError("gate and up must have the same row stride")
+    transposed, (ldg, ldu) = _weights(("w_gate", "w_up"), (w_gate, w_up))
+    with torch.no_grad():
+        dx = torch.empty((rows, cin), dtype=x.dtype, device=x.device) if need_x else None
+        dwg, dwu = (_like_weights(w_gate, transposed) for _ in range(2)) if need_w else (None, None)
+        dbg, dbu = (torch.empty(cout, dtype=x.dtype, device=x.device) for _ in range(2)) if bias else (None, None)
+    ws, size = _workspace(_lib.load().fpn_gated_grad_workspace_bytes(dtype, rows, cin, cout), x)
+    p = _lib.ptr
+    _call(x, "fpn_gated_grad", dtype, rows, cin, cout, p(dh), lddh, p(x), ldx, p(w_gate), ldg, p(w_up), ldu, transposed, p(gate), p(up),
+          ldp, act, p(dx), cin, p(dwg), p(dwu), cin if transposed else cout, p(dbg), p(dbu), p(ws), size)
+    return dx, dwg, dwu, dbg, dbu
+
+
+class _Gated(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, bias_gate, bias_up, activation):
+        h, gate, up = gated(x, w_gate, w_up, bias_gate, bias_up, activation, keep=True)
+        ctx.save_for_backward(x, w_gate, w_up, gate, up)
+        ctx.activation = activation
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh):
+        _no_capture()
+        x, w_gate, w_up, gate, up = ctx.saved_tensors
+        need_x, need_g, need_u, need_bg, need_bu, _ = ctx.needs_input_grad
+        dx, dwg, dwu, dbg, dbu = gated_grad(_dense_rows(dh), x, w_gate, w_up, gate, up, ctx.activation, need_bg or need_bu, need_x,
+                                            need_g or need_u)
+        return dx, dwg if need_g else None, dwu if need_u else None, dbg if need_bg else None, dbu if need_bu else None, None
+
+
+# ---- the block -----------------------------------------------------------------------------------------------------
+
+def gated_feed_forward(x, w_gate, w_up, w_down, bias_gate=None, bias_up=None, bias_down=None, activation="silu", residual=None,
+                       out=None):
+    """y = gated(x) w_down + bias_down + residual: `gated` and then `dense` with the residual in its epilogue."""
+    h = gated(x, w_gate, w_up, bias_gate, bias_up, activation)
+    return dense(h, w_down, bias_down, None, residual, out)

@@ -12,9 +12,10 @@
  *     (a hipStream_t passed as void*, NULL = the default stream);
  *   - return value: FPN_OK, or a negative FPN_E_* code; fpn_last_error_string()
  *     then describes the failure (thread-local);
- *   - inference only: no gradient entry points (the reference registers
- *     gradients for GatherPoint/GroupPoint/ThreeInterpolate; they are training
- *     code and not part of this path).
+ *   - the point-set and network entry points are inference only: no gradients (the
+ *     reference registers gradients for GatherPoint/GroupPoint/ThreeInterpolate;
+ *     they are training code and not part of this path); the feed-forward
+ *     operators at the end of this header have theirs.
  *
  * Each declaration cites the reference interface it replaces (paths relative to
  * the reference repository root).
@@ -32,6 +33,20 @@ extern "C" {
 #define FPN_E_INVALID_ARG (-1)   /* bad size, null pointer, unsupported shape  */
 #define FPN_E_LAUNCH (-2)        /* the HIP runtime rejected a launch          */
 #define FPN_E_UNSUPPORTED (-3)   /* valid request outside the implemented range */
+
+/* Element types of the feed-forward operators (fpn_dense, fpn_gated). */
+#define FPN_F32 0
+#define FPN_BF16 1
+#define FPN_F16 2
+
+/* Their activations: identity, max(v,0), v/(1+exp(-v)) and 1/(1+exp(-v)), v Phi(v) with the normal distribution's
+ * Phi, and its form by tanh: v (1 + tanh(sqrt(2/pi) (v + 0.044715 v^3))) / 2. */
+#define FPN_ACT_NONE 0
+#define FPN_ACT_RELU 1
+#define FPN_ACT_SILU 2
+#define FPN_ACT_SIGMOID 3
+#define FPN_ACT_GELU 4
+#define FPN_ACT_GELU_TANH 5
 
 /* ABI version of this header (bumped on any signature change). */
 int fpn_abi_version(void);
@@ -735,6 +750,63 @@ int fpn_mc_statistics(int s, int b, const float *box_output, const float *stage1
 int fpn_detection_records(int b, int n, const float *mask_logits, const float *box_output,
                           const float *stage1_center, const float *rot_angle, double *records,
                           unsigned *seg_bits, void *stream);
+
+/*
+ * Feed-forward operators: products with bias, activation and residual in the epilogue, and the gated block's both
+ * projections, activation and product in one kernel, each with its backward pass.  They stand beside the shared
+ * MLP layer (fpn_shared_mlp_f32: fp32, scale / shift / ReLU, pooling) and have what it lacks: bf16 and fp16 storage,
+ * residuals, smooth activations, gates and gradients.  No counterpart in the reference.
+ *
+ *   - every matrix of a call has the call's element type (FPN_F32, FPN_BF16, FPN_F16); sums are fp32;
+ *   - "ld" arguments are row strides in elements, at least the matrix' width (x and residual: or 0, one row for all)
+ *     and below 2^21; widths below 2^21; any alignment of an element;
+ *   - w_transposed 0: weights (cin,cout); 1: held (cout,cin), row stride >= cin;
+ *   - rows 0 is a valid call: forward writes nothing, weight and bias gradients become 0;
+ *   - outputs may not share memory with inputs, except y with residual (same address and stride);
+ *   - the workspace (16-byte aligned, at least what the _workspace_bytes function of the same arguments says) belongs
+ *     to the call until its work is done: calls that may run at the same time need one each;
+ *   - results do not depend on anything but the arguments: no atomics, a fixed order of every sum.
+ */
+
+/*
+ * y = act(x w + bias) + residual.   x (rows,cin), w (cin,cout), bias (cout) or NULL, residual (rows,cout) or NULL,
+ * y (rows,cout); pre (rows,cout) or NULL receives x w + bias for fpn_dense_grad.
+ */
+size_t fpn_dense_workspace_bytes(int dtype, long rows, int cin, int cout);
+int fpn_dense(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w, long ldw, int w_transposed,
+              const void *bias, int activation, const void *residual, long ldr, void *y, long ldy, void *pre, long ldp,
+              void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Its gradients, d = dy act'(pre):  dx = d w^T, dw = x^T d (in w's storage order, row stride lddw), dbias = column
+ * sums of d; the residual's gradient is dy itself.  dx, dw, dbias may each be NULL; pre is not read where the
+ * activation is FPN_ACT_NONE, x only for dw, w only for dx.
+ */
+size_t fpn_dense_grad_workspace_bytes(int dtype, long rows, int cin, int cout, int activation);
+int fpn_dense_grad(int dtype, long rows, int cin, int cout, const void *dy, long lddy, const void *x, long ldx, const void *w,
+                   long ldw, int w_transposed, const void *pre, long ldp, int activation, void *dx, long lddx, void *dw, long lddw,
+                   void *dbias, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * h = act(x w_gate + bias_gate) * (x w_up + bias_up).   Both weights (cin,cout) or both (cout,cin), each with its own
+ * row stride (halves of one matrix will do); gate and up (rows,cout), row stride ldp, receive the two sums for
+ * fpn_gated_grad, or are both NULL.
+ */
+size_t fpn_gated_workspace_bytes(int dtype, long rows, int cin, int cout);
+int fpn_gated(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w_gate, long ldg, const void *w_up,
+              long ldu, int w_transposed, const void *bias_gate, const void *bias_up, int activation, void *h, long ldh, void *gate,
+              void *up, long ldp, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Its gradients, dg = dh up act'(gate), du = dh act(gate):  dx = dg w_gate^T + du w_up^T, dw_gate = x^T dg,
+ * dw_up = x^T du (both in the weights' storage order, row stride lddw), and the column sums of dg and du.
+ * dx, the pair of dw and the pair of dbias may each be NULL.
+ */
+size_t fpn_gated_grad_workspace_bytes(int dtype, long rows, int cin, int cout);
+int fpn_gated_grad(int dtype, long rows, int cin, int cout, const void *dh, long lddh, const void *x, long ldx, const void *w_gate,
+                   long ldg, const void *w_up, long ldu, int w_transposed, const void *gate, const void *up, long ldp, int activation,
+                   void *dx, long lddx, void *dw_gate, void *dw_up, long lddw, void *dbias_gate, void *dbias_up, void *workspace,
+                   size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }
