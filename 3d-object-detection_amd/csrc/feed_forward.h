@@ -689,12 +689,22 @@ template <class T, bool GATED> __global__ __launch_bounds__(kThreads) void join_
 
 // How a product is cut: tile, splits of k, and the bytes of partial sums that takes
 struct Plan {
+    bool wide;              // the 256 x 256 kernel (feed_forward_wide.h)
     int bm, bn;
     int splits;
     long tiles_per_split;
     size_t partial_bytes;
 };
-Plan plan_product(int dtype, long m, int n, long k, int segs, int batch, bool gated);
+// (aligned: every operand consists of whole 16-byte chunks at 16-byte addresses)
+Plan plan_product(int dtype, long m, int n, long k, int segs, int batch, bool gated, bool aligned);
+
+// whether an operand consists of whole 16-byte chunks
+inline bool whole_chunks(const void *p, long ld, int order, long extent, int element)
+{
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * element % 16 == 0 && (order == kInner || extent * element % 16 == 0);
+}
+
+template <class T> int launch_wide(const Args &p, int order_a, int order_b, bool gated, long blocks, hipStream_t stream);
 
 // Launches a planned product (p.partial and the plan's fields are filled in here)
 template <class T> int launch_product(Args p, int order_a, int order_b, bool gated, const Plan &plan, float *partial, hipStream_t stream);
@@ -703,6 +713,8 @@ template <class T> int launch_product(Args p, int order_a, int order_b, bool gat
 extern template int launch_product<float>(Args, int, int, bool, const Plan &, float *, hipStream_t);
 extern template int launch_product<__bf16>(Args, int, int, bool, const Plan &, float *, hipStream_t);
 extern template int launch_product<_Float16>(Args, int, int, bool, const Plan &, float *, hipStream_t);
+extern template int launch_wide<__bf16>(const Args &, int, int, bool, long, hipStream_t);
+extern template int launch_wide<_Float16>(const Args &, int, int, bool, long, hipStream_t);
 #endif
 
 #define FPN_FF_LAUNCH(A, B, BM_, BN_, WM_, WN_, G)                                                                            \
@@ -741,7 +753,10 @@ template <class T> int launch_product(Args p, int order_a, int order_b, bool gat
     const long blocks = p.mt * p.nt * p.splits * p.batch;
     if (blocks > 0x7fffffffl) return fail(FPN_E_UNSUPPORTED, "a product of %ld workgroups", blocks);
     int rc;
-    if (plan.bm == 128) rc = launch_tiles<T, 128, 128, 2, 2>(p, order_a, order_b, gated, blocks, stream);
+    if (plan.wide) {
+        if constexpr (sizeof(T) == 2) rc = launch_wide<T>(p, order_a, order_b, gated, blocks, stream);
+        else return fail(FPN_E_UNSUPPORTED, "no wide kernel for this type");
+    } else if (plan.bm == 128) rc = launch_tiles<T, 128, 128, 2, 2>(p, order_a, order_b, gated, blocks, stream);
     else rc = launch_tiles<T, 64, 128, 2, 2>(p, order_a, order_b, gated, blocks, stream);
     if (rc != FPN_OK || !p.partial) return rc;
     const long runs8 = p.m * ((p.n + 7) / 8);

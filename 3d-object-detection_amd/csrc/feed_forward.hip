@@ -1,5 +1,6 @@
 // The feed-forward operators' entry points: dense (act(x W + b) + r) and gated (act(x Wg + bg) * (x Wu + bu)),
 // forward and backward, and the element-wise half of the backward pass.  The products are in feed_forward.h.
+#include <cstdlib>
 #include "feed_forward.h"
 
 namespace fpn {
@@ -124,11 +125,22 @@ int launch_grad(GradArgs p, bool gated, void *const (&sums_out)[2], hipStream_t 
 
 int element_size(int dtype) { return dtype == FPN_F32 ? 4 : 2; }
 
+// the larger of the partial sums of a product's two plans
+size_t partial_bytes(int dtype, long m, int n, long k, int segs, int batch, bool gated)
+{
+    return std::max(plan_product(dtype, m, n, k, segs, batch, gated, false).partial_bytes,
+                    plan_product(dtype, m, n, k, segs, batch, gated, true).partial_bytes);
+}
+
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 int run_product(int dtype, const Args &p, int order_a, int order_b, bool gated, float *partial, size_t partial_bytes, hipStream_t stream)
 {
-    const Plan plan = plan_product(dtype, p.m, p.n, p.k, p.segs, p.batch, gated);
+    bool aligned = true;
+    for (int i = 0; i < p.segs; ++i) aligned = aligned && whole_chunks(p.a[i], p.lda[i], order_a, p.m, element_size(dtype));
+    for (int i = 0; i < std::max({p.segs, p.batch, gated ? 2 : 1}); ++i)
+        aligned = aligned && whole_chunks(p.b[i], p.ldb[i], order_b, p.n, element_size(dtype));
+    const Plan plan = plan_product(dtype, p.m, p.n, p.k, p.segs, p.batch, gated, aligned);
     if (plan.partial_bytes > partial_bytes)
         return fail(FPN_E_INVALID_ARG, "workspace: %zu bytes of partial sums needed, %zu there", plan.partial_bytes, partial_bytes);
     if (dtype == FPN_F32) return launch_product<float>(p, order_a, order_b, gated, plan, partial, stream);
@@ -187,9 +199,8 @@ GradSpace grad_space(int dtype, long rows, int cin, int n, bool gated, bool with
     const int planes = gated ? 2 : 1;
     s.d = with_d ? align256((size_t)rows * n * element_size(dtype)) * planes : 0;
     s.sums = align256((size_t)grad_rows_grid(rows, n) * planes * n * sizeof(float));
-    const Plan dx = plan_product(dtype, rows, cin, n, planes, 1, false);
-    const Plan dw = plan_product(dtype, cin, n, rows, 1, planes, false), dwt = plan_product(dtype, n, cin, rows, 1, planes, false);
-    s.partial = align256(std::max({dx.partial_bytes, dw.partial_bytes, dwt.partial_bytes}));
+    s.partial = align256(std::max({partial_bytes(dtype, rows, cin, n, planes, 1, false), partial_bytes(dtype, cin, n, rows, 1, planes, false),
+                                   partial_bytes(dtype, n, cin, rows, 1, 1, false)}));
     s.total = s.d + s.sums + s.partial;
     return s;
 }
@@ -242,14 +253,23 @@ int run_grad(int dtype, const GradArgs &p, bool gated, void *const (&sums_out)[2
 
 }  // namespace
 
-Plan plan_product(int dtype, long m, int n, long k, int segs, int batch, bool gated)
+Plan plan_product(int dtype, long m, int n, long k, int segs, int batch, bool gated, bool aligned)
 {
     Plan p;
+    p.wide = false;
     const int bk = kTileBytes / element_size(dtype);
     const long kt = (k + bk - 1) / bk * segs;
     auto tiles = [&](int bm, int bn) { return (m + bm - 1) / bm * ((n + (gated ? bn / 2 : bn) - 1) / (gated ? bn / 2 : bn)) * batch; };
     p.bm = m > 64 && tiles(128, 128) >= 256 ? 128 : 64;
     p.bn = 128;
+    if (dtype != FPN_F32 && aligned && m > 128 && tiles(256, 256) >= (getenv("FF_WIDE") ? atoi(getenv("FF_WIDE")) : 128)) {
+        p.wide = true;
+        p.bm = p.bn = 256;
+        p.splits = 1;
+        p.tiles_per_split = k / 32 * segs;
+        p.partial_bytes = 0;
+        return p;
+    }
     const long t = std::max(1l, tiles(p.bm, p.bn));
     // too few tiles for the chip: k is split so that about 512 workgroups run, each with at least four k tiles
     long splits = t >= 256 ? 1 : std::max(1l, std::min({512 / t, kt / 4, 256l}));
@@ -271,7 +291,7 @@ extern "C" {
 size_t fpn_dense_workspace_bytes(int dtype, long rows, int cin, int cout)
 {
     if (check_common(dtype, rows, cin, cout, FPN_ACT_NONE) != FPN_OK) return 0;
-    return plan_product(dtype, rows, cout, cin, 1, 1, false).partial_bytes;
+    return partial_bytes(dtype, rows, cout, cin, 1, 1, false);
 }
 
 int fpn_dense(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w, long ldw, int w_transposed,
@@ -371,7 +391,7 @@ int fpn_dense_grad(int dtype, long rows, int cin, int cout, const void *dy, long
 size_t fpn_gated_workspace_bytes(int dtype, long rows, int cin, int cout)
 {
     if (check_common(dtype, rows, cin, cout, FPN_ACT_NONE) != FPN_OK) return 0;
-    return plan_product(dtype, rows, cout, cin, 1, 1, true).partial_bytes;
+    return partial_bytes(dtype, rows, cout, cin, 1, 1, true);
 }
 
 int fpn_gated(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w_gate, long ldg, const void *w_up, long ldu,

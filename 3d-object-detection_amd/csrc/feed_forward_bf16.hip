@@ -1,10 +1,11 @@
 // The feed-forward products' kernels for bf16 operands (feed_forward.h).
 #define FPN_FF_INSTANTIATE
-#include "feed_forward.h"
+#include "feed_forward_wide.h"
 
 namespace fpn {
 namespace ff {
 
+template int launch_wide<__bf16>(const Args &, int, int, bool, long, hipStream_t);
 template int launch_product<__bf16>(Args, int, int, bool, const Plan &, float *, hipStream_t);
 
 }  // namespace ff
