@@ -5,7 +5,7 @@
 // Per 16 of k a wave reads 8 KB of operands from LDS for 512 cycles of MFMA (half of what the LDS delivers); with 128 x 128
 // tiles and 64 x 64 quadrants it is as much for 256 cycles, and the LDS, not the matrix unit, sets the pace.
 //
-// LDS holds four stages of 32 k (32 KB each).  A wave requests its eighth of stage t + 4 as soon as everyone has read
+// LDS holds four stages of 32 k (32 KB each).  A wave requests its quarter of stage t + 4 as soon as everyone has read
 // stage t, so a request has three stages' time (3072 cycles of MFMA) to arrive, and reads the next 16 of k
 // while it multiplies the present ones: one barrier per 32 MFMAs, nothing else waits.
 //
@@ -24,10 +24,11 @@ constexpr int kWideStage = 512 * kWideK * 2;                // bytes: 256 rows o
 
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"             // (m0 is reserved: nothing here indexes registers through it)
-// 16 bytes per lane from base + off to LDS at lds + 16 lane
-__device__ inline void request(unsigned lds, unsigned off, const void *base)
+// 16 bytes per lane from base + off to LDS at lds + AT + 16 lane
+template <int AT> __device__ inline void request(unsigned lds, unsigned off, const void *base)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(off), "s"(base) : "m0");
+    asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 : : "s"(lds), "v"(off), "s"(base), "i"(AT) : "m0", "scc");
 }
 #pragma clang diagnostic pop
 
@@ -36,7 +37,7 @@ __device__ inline void request(unsigned lds, unsigned off, const void *base)
 template <int LEFT> __device__ inline void arrive()
 {
     if (LEFT == 16) asm volatile("s_waitcnt vmcnt(16) lgkmcnt(0)\n\ts_barrier" : : : "memory");
-    else if (LEFT == 8) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" : : : "memory");
+    else if (LEFT == 20) asm volatile("s_waitcnt vmcnt(20) lgkmcnt(0)\n\ts_barrier" : : : "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
 }
 
@@ -52,6 +53,7 @@ template <class T, int ORDER, int R> struct Stream {
     static constexpr int kPer = R * 64 / 1024 / 4;          // requests per wave
     static constexpr int kRowBytes = R * 2;                 // kOuter
     const char *base;                                       // uniform: k = 0 of the segment
+    const char *next;                                       // the stage to be requested next
     long step;                                              // bytes between stages
     unsigned off[kPer];
 
@@ -84,12 +86,8 @@ template <class T, int ORDER, int R> struct Stream {
         }
     }
 
-    __device__ void issue(unsigned lds, long kt, int wave) const
-    {
-        const char *at = base + kt * step;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) request(lds + (wave * kPer + i) * 1024, off[i], at);
-    }
+    // request I of kPer; lds: the stage's piece for this operand and wave
+    template <int I> __device__ void issue(unsigned lds) const { request<I * 1024>(lds, off[I], next); }
 
     // the last, partial stage of a segment, through registers, zeros behind the last k
     __device__ void put_tail(char *lds, long kt, int left_k, int wave, int lane) const
@@ -156,37 +154,91 @@ constexpr int kEpilogueBytes = 32 * kEpilogueRow;
 template <class T, bool GATED>
 __device__ inline void store_quadrant(const Args &p, const floatx16 (&acc)[4][4], char *lds, int member, int split, long m0, int n0, int lane)
 {
+    constexpr bool EXACT = sizeof(T) == 4;
     const int l31 = lane & 31, h = lane >> 5;
-    constexpr int kRuns = GATED ? 8 : 16;                  // runs of eight columns per row
+    constexpr int kRuns = GATED ? 8 : 16, kRowsAtOnce = 64 / kRuns, kBatch = 4;     // runs of eight columns per row
     const int run = lane % kRuns, row0 = lane / kRuns;
     const int n = n0 + run * 8;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    const long left = p.n - n;
+    auto put = [&](const floatx16 (&c)[4]) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 floatx4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e];
+                for (int e = 0; e < 4; ++e) v[e] = c[j][4 * q + e];
                 *reinterpret_cast<floatx4 *>(lds + l31 * kEpilogueRow + (32 * j + 8 * q + 4 * h) * 4) = v;
             }
-        if (n < p.n) {
+    };
+    float bias[8] = {}, bias2[8] = {};
+    if (left > 0 && p.bias[GATED ? 0 : member]) load8(reinterpret_cast<const T *>(p.bias[GATED ? 0 : member]) + n, left, bias);
+    if (GATED && left > 0 && p.bias[1]) load8(reinterpret_cast<const T *>(p.bias[1]) + n, left, bias2);
 #pragma unroll 1
-            for (int r = row0; r < 32; r += 64 / kRuns) {
-                const long m = m0 + 32 * i + r;
-                if (m >= p.m) break;
-                float v[8], v2[8];
-                const float *from = reinterpret_cast<const float *>(lds + r * kEpilogueRow) + run * 8;
+    for (int i = 0; i < 4; ++i) {
+        if (i == 0) put(acc[0]);
+        else if (i == 1) put(acc[1]);
+        else if (i == 2) put(acc[2]);
+        else put(acc[3]);
+        if (left <= 0) continue;
+        // four rows' loads at a time, then their arithmetic, then their stores: with one wave per SIMD nothing else
+        // would cover the latency
+#pragma unroll 1
+        for (int r = row0; r < 32; r += kRowsAtOnce * kBatch) {
+            const long m = m0 + 32 * i + r;
+            float v[kBatch][8], v2[GATED ? kBatch : 1][8], res[kBatch][8];
+            if (p.residual)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) { v[e] = from[e]; v2[e] = GATED ? from[64 + e] : 0.f; }
-                if (p.partial) {
-                    float *to = p.partial + ((((long)member * p.splits + split) * (GATED ? 2 : 1)) * p.m + m) * p.n + n;
-                    store8(to, p.n - n, v);
-                    if (GATED) store8(to + p.m * p.n, p.n - n, v2);
-                } else {
-                    finish8<T, GATED>(p, member, m, n, v, v2);
+                for (int b = 0; b < kBatch; ++b)
+                    load8(reinterpret_cast<const T *>(p.residual) + min(m + b * kRowsAtOnce, p.m - 1) * p.ldr + n, left, res[b]);
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                const float *from = reinterpret_cast<const float *>(lds + (r + b * kRowsAtOnce) * kEpilogueRow) + run * 8;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    v[b][e] = from[e];
+                    if (GATED) v2[b][e] = from[64 + e];
                 }
+            }
+            if (p.partial) {
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b)
+                    if (m + b * kRowsAtOnce < p.m) {
+                        float *to = p.partial + ((((long)member * p.splits + split) * (GATED ? 2 : 1)) * p.m + m + b * kRowsAtOnce) * p.n + n;
+                        store8(to, left, v[b]);
+                        if (GATED) store8(to + p.m * p.n, left, v2[b]);
+                    }
+                continue;
+            }
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    v[b][e] += bias[e];
+                    if (GATED) v2[b][e] += bias2[e];
+                }
+            if (p.pre[0])
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b)
+                    if (m + b * kRowsAtOnce < p.m) {
+                        store8(reinterpret_cast<T *>(p.pre[0]) + (m + b * kRowsAtOnce) * p.ldp + n, left, v[b]);
+                        if (GATED) store8(reinterpret_cast<T *>(p.pre[1]) + (m + b * kRowsAtOnce) * p.ldp + n, left, v2[b]);
+                    }
+            if (p.act != FPN_ACT_NONE)
+                for_activation(p.act, [&](auto tag) {
+#pragma unroll
+                    for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[b][e] = activate<decltype(tag)::value, EXACT>(v[b][e]);
+                });
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (GATED) v[b][e] *= v2[b][e];
+                    if (p.residual) v[b][e] += res[b][e];
+                }
+                if (m + b * kRowsAtOnce < p.m) store8(reinterpret_cast<T *>(p.c[member]) + (m + b * kRowsAtOnce) * p.ldc + n, left, v[b]);
             }
         }
     }
@@ -237,24 +289,51 @@ __global__ __launch_bounds__(kThreads) void wide_product_kernel(const Args p)
             sb[0].init(p.b[s + at.member], p.ldb[s + at.member], n0, p.n - n0, wave, lane);
         }
     };
-    auto issue = [&](long kt, int stage) {
-        const unsigned to = lds0 + stage * kWideStage;
-        sa.issue(to, kt, wave);
-        sb[0].issue(to + kABytes, kt, wave);
-        if (GATED) sb[kHalves - 1].issue(to + kABytes + kCols * kWideK * 2, kt, wave);
+    // request Q of a wave's eight of a stage
+    constexpr int kPerB = Stream<T, ORDER_B, kCols>::kPer;
+    const unsigned lds_a = lds0 + wave * 4096, lds_b = lds0 + kABytes + wave * (kPerB * 1024);
+    auto issue = [&](auto q, int stage) {
+        constexpr int Q = decltype(q)::value;
+        if constexpr (Q < 4) sa.template issue<Q>(lds_a + stage * kWideStage);
+        else if constexpr (Q < 4 + kPerB) sb[0].template issue<Q - 4>(lds_b + stage * kWideStage);
+        else sb[kHalves - 1].template issue<(Q - 4) % kPerB>(lds_b + kCols * kWideK * 2 + stage * kWideStage);
     };
-    auto read = [&](uintx4 (&fa)[4], uintx4 (&fb)[4], const char *stage, int s) {
+    long asked = 0, most = 0;                               // stages whose requests are complete, and the last to ask for
+    auto advance = [&] {
+        const bool on = asked < most;
+        ++asked;
+        sa.next += on ? sa.step : 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) fa[i] = ra.frag(stage, am[i], i, s);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            fb[j] = rb.frag(stage + kABytes + (GATED && j >= 2 ? kCols * kWideK * 2 : 0), bn[j], j, s);
+        for (int g = 0; g < kHalves; ++g) sb[g].next += on ? sb[g].step : 0;
     };
-    auto multiply_all = [&](const uintx4 (&fa)[4], const uintx4 (&fb)[4]) {
+    auto read_a = [&](const char *stage, int i, int s) { return ra.frag(stage, am[i], i, s); };
+    auto read_b = [&](const char *stage, int j, int s) {
+        return rb.frag(stage + kABytes + (GATED && j >= 2 ? kCols * kWideK * 2 : 0), bn[j], j, s);
+    };
+    // 16 of k: multiplies ca, cb while na, nb come from `stage`, and issues requests Q .. Q + 3 to stage `to`.  A wave
+    // issues in order: an MFMA occupies its unit for 32 cycles, in which seven other instructions can go out, so the
+    // reads and requests are dealt out among the MFMAs one by one (all in front of a group of four MFMAs cost 12 %);
+    // no read is left for the last quarter, which covers their latency.
+    auto step = [&](const uintx4 (&ca)[4], const uintx4 (&cb)[4], uintx4 (&na)[4], uintx4 (&nb)[4], const char *stage, int s,
+                    auto q, int to) {
+        constexpr int Q = decltype(q)::value;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i][j] = multiply<T>(fb[j], fa[i], acc[i][j]);
+        for (int i = 0; i < 16; ++i) {
+            acc[i & 3][i >> 2] = multiply<T>(cb[i >> 2], ca[i & 3], acc[i & 3][i >> 2]);
+            if (i == 0) na[0] = read_a(stage, 0, s);
+            if (i == 1) na[1] = read_a(stage, 1, s);
+            if (i == 2) issue(ActTag<Q>(), to);
+            if (i == 3) na[2] = read_a(stage, 2, s);
+            if (i == 4) na[3] = read_a(stage, 3, s);
+            if (i == 5) nb[0] = read_b(stage, 0, s);
+            if (i == 6) issue(ActTag<Q + 1>(), to);
+            if (i == 7) nb[1] = read_b(stage, 1, s);
+            if (i == 8) nb[2] = read_b(stage, 2, s);
+            if (i == 9) nb[3] = read_b(stage, 3, s);
+            if (i == 10) issue(ActTag<Q + 2>(), to);
+            if (i == 12) issue(ActTag<Q + 3>(), to);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
     uintx4 fa[2][4], fb[2][4];
 
@@ -264,33 +343,40 @@ __global__ __launch_bounds__(kThreads) void wide_product_kernel(const Args p)
         segment(s);
         if (t0 < t1) {
             const long n = t1 - t0;
-            for (int i = 0; i < kStages; ++i)
-                if (i < n) issue(t0 + i, i);
-            arrive<0>();
-            read(fa[0], fb[0], lds, 0);
+            // Stage t + 4 is requested in two halves: behind the barrier of t, and in the first half of t + 1 (behind the
+            // segment's end its last stage again, which nobody reads: a loop without branches, and counts that hold).
+            // In flight at a barrier are the three stages ahead; the one read next must be there.
+            most = n - 1;
+            asked = 0;
+            sa.next = sa.base + t0 * sa.step;
+#pragma unroll
+            for (int g = 0; g < kHalves; ++g) sb[g].next = sb[g].base + t0 * sb[g].step;
+#pragma unroll
+            for (int i = 0; i < kStages; ++i) {
+                issue(ActTag<0>(), i);
+                issue(ActTag<1>(), i);
+                issue(ActTag<2>(), i);
+                issue(ActTag<3>(), i);
+                if (i == kStages - 1) break;
+                issue(ActTag<4>(), i);
+                issue(ActTag<5>(), i);
+                issue(ActTag<6>(), i);
+                issue(ActTag<7>(), i);
+                advance();
+            }
+            arrive<20>();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { fa[0][i] = read_a(lds, i, 0); fb[0][i] = read_b(lds, i, 0); }
             int stage = 0;
-            long t = 0;
-            // (in flight at a barrier: the three stages ahead; the one read next must be there)
-            for (; t + kStages < n; ++t) {
-                const char *cur = lds + stage * kWideStage;
-                read(fa[1], fb[1], cur, 1);
-                multiply_all(fa[0], fb[0]);
+            for (long t = 0; t < n; ++t) {
+                step(fa[0], fb[0], fa[1], fb[1], lds + stage * kWideStage, 1, ActTag<4>(), (stage + 3) & 3);
+                advance();
                 arrive<16>();
-                const int next = (stage + 1) & (kStages - 1);
-                read(fa[0], fb[0], lds + next * kWideStage, 0);
-                issue(t0 + t + kStages, stage);
-                multiply_all(fa[1], fb[1]);
-                stage = next;
+                const int freed = stage;
+                stage = (stage + 1) & 3;
+                step(fa[1], fb[1], fa[0], fb[0], lds + stage * kWideStage, 0, ActTag<0>(), freed);
             }
-            for (; t < n; ++t) {
-                const char *cur = lds + stage * kWideStage;
-                read(fa[1], fb[1], cur, 1);
-                multiply_all(fa[0], fb[0]);
-                arrive<0>();
-                stage = (stage + 1) & (kStages - 1);
-                read(fa[0], fb[0], lds + stage * kWideStage, 0);      // (behind the last stage: read, not used)
-                multiply_all(fa[1], fb[1]);
-            }
+            arrive<0>();
         }
         // what is left of k, with the last split
         const int left = (int)(p.k - full * kWideK);
@@ -302,8 +388,12 @@ __global__ __launch_bounds__(kThreads) void wide_product_kernel(const Args p)
             __syncthreads();
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                read(fa[0], fb[0], lds, q);
-                multiply_all(fa[0], fb[0]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { fa[0][i] = read_a(lds, i, q); fb[0][i] = read_b(lds, i, q); }
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[i][j] = multiply<T>(fb[0][j], fa[0][i], acc[i][j]);
             }
         }
         __syncthreads();
