@@ -704,7 +704,7 @@ inline bool whole_chunks(const void *p, long ld, int order, long extent, int ele
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * element % 16 == 0 && (order == kInner || extent * element % 16 == 0);
 }
 
-template <class T> int launch_wide(const Args &p, int order_a, int order_b, bool gated, long blocks, hipStream_t stream);
+template <class T> int launch_wide(const Args &p, int order_a, int order_b, bool gated, int bm, int bn, long blocks, hipStream_t stream);
 
 // Launches a planned product (p.partial and the plan's fields are filled in here)
 template <class T> int launch_product(Args p, int order_a, int order_b, bool gated, const Plan &plan, float *partial, hipStream_t stream);
@@ -713,8 +713,8 @@ template <class T> int launch_product(Args p, int order_a, int order_b, bool gat
 extern template int launch_product<float>(Args, int, int, bool, const Plan &, float *, hipStream_t);
 extern template int launch_product<__bf16>(Args, int, int, bool, const Plan &, float *, hipStream_t);
 extern template int launch_product<_Float16>(Args, int, int, bool, const Plan &, float *, hipStream_t);
-extern template int launch_wide<__bf16>(const Args &, int, int, bool, long, hipStream_t);
-extern template int launch_wide<_Float16>(const Args &, int, int, bool, long, hipStream_t);
+extern template int launch_wide<__bf16>(const Args &, int, int, bool, int, int, long, hipStream_t);
+extern template int launch_wide<_Float16>(const Args &, int, int, bool, int, int, long, hipStream_t);
 #endif
 
 #define FPN_FF_LAUNCH(A, B, BM_, BN_, WM_, WN_, G)                                                                            \
@@ -754,7 +754,7 @@ template <class T> int launch_product(Args p, int order_a, int order_b, bool gat
     if (blocks > 0x7fffffffl) return fail(FPN_E_UNSUPPORTED, "a product of %ld workgroups", blocks);
     int rc;
     if (plan.wide) {
-        if constexpr (sizeof(T) == 2) rc = launch_wide<T>(p, order_a, order_b, gated, blocks, stream);
+        if constexpr (sizeof(T) == 2) rc = launch_wide<T>(p, order_a, order_b, gated, plan.bm, plan.bn, blocks, stream);
         else return fail(FPN_E_UNSUPPORTED, "no wide kernel for this type");
     } else if (plan.bm == 128) rc = launch_tiles<T, 128, 128, 2, 2>(p, order_a, order_b, gated, blocks, stream);
     else rc = launch_tiles<T, 64, 128, 2, 2>(p, order_a, order_b, gated, blocks, stream);

@@ -1,6 +1,5 @@
 // The feed-forward operators' entry points: dense (act(x W + b) + r) and gated (act(x Wg + bg) * (x Wu + bu)),
 // forward and backward, and the element-wise half of the backward pass.  The products are in feed_forward.h.
-#include <cstdlib>
 #include "feed_forward.h"
 
 namespace fpn {
@@ -253,30 +252,67 @@ int run_grad(int dtype, const GradArgs &p, bool gated, void *const (&sums_out)[2
 
 }  // namespace
 
+namespace {
+
+// The time of a launch of `tiles` workgroups of one shape, in us, from what these took on a 256-CU chip at 8192 x 4096 x 4096,
+// 4096 x 2048 x 2048, 2048 x 2048 x 2048 and 1024 x 4096 x 4096 (bf16): a stage of 32 k with the shape's number of workgroups on
+// every CU, one with half as many, and what a round of workgroups costs besides (first loads, epilogue).
+struct Pace { int bm, bn, per_cu; double stage, half, round; };
+constexpr Pace kWide[] = {
+    {256, 256, 1, 0.88, 0.88, 8.0},        // 235 us at 8192 x 4096 x 4096 (medium 270, small 306)
+    {256, 128, 2, 1.00, 0.58, 6.0},        // 43 us at 4096 x 2048 x 2048 (large 52, small 44)
+    {128, 128, 2, 0.64, 0.34, 4.0},        // 26 us at 2048 x 2048 x 2048 (large 46, medium 35)
+};
+
+double launch_time(const Pace &p, long tiles, double stages, int cus)
+{
+    const long at_once = (long)cus * p.per_cu, rounds = tiles / at_once, rest = tiles - rounds * at_once;
+    double us = rounds * (p.stage * stages + p.round);
+    if (rest) us += (rest > cus ? p.stage : p.half) * stages + p.round;
+    return us;
+}
+
+// writing and reading the partial sums of a split (3 GB/ms as a join reaches it), and the join's launch
+double join_time(double bytes) { return bytes > 0 ? 4.0 + bytes / 1.5e6 : 0.0; }
+
+}  // namespace
+
 Plan plan_product(int dtype, long m, int n, long k, int segs, int batch, bool gated, bool aligned)
 {
-    Plan p;
-    p.wide = false;
-    const int bk = kTileBytes / element_size(dtype);
-    const long kt = (k + bk - 1) / bk * segs;
+    Plan p = {};
+    const int cus = current_device_cus() > 0 ? current_device_cus() : 256;
     auto tiles = [&](int bm, int bn) { return (m + bm - 1) / bm * ((n + (gated ? bn / 2 : bn) - 1) / (gated ? bn / 2 : bn)) * batch; };
-    p.bm = m > 64 && tiles(128, 128) >= 256 ? 128 : 64;
-    p.bn = 128;
-    if (dtype != FPN_F32 && aligned && m > 128 && tiles(256, 256) >= (getenv("FF_WIDE") ? atoi(getenv("FF_WIDE")) : 128)) {
-        p.wide = true;
-        p.bm = p.bn = 256;
-        p.splits = 1;
-        p.tiles_per_split = k / 32 * segs;
-        p.partial_bytes = 0;
-        return p;
+    const double plane = (double)batch * (gated ? 2 : 1) * m * n * sizeof(float);
+    constexpr double kMostPartial = 128 << 20;
+    if (dtype != FPN_F32 && aligned && m > 0) {
+        const long full = k / 32 * segs;
+        double best = 0;
+        for (const Pace &s : kWide)
+            for (long splits = 1; splits <= 256; splits *= 2) {
+                const long each = std::max(1l, (full + splits - 1) / splits);
+                if (splits > 1 && (each < 8 || plane * splits > kMostPartial)) break;
+                const double us = launch_time(s, tiles(s.bm, s.bn) * splits, (double)each, cus) + (splits > 1 ? join_time(plane * splits) : 0);
+                if (!p.wide || us < best) {
+                    best = us;
+                    p.wide = true;
+                    p.bm = s.bm;
+                    p.bn = s.bn;
+                    p.tiles_per_split = each;
+                    p.splits = (int)std::max(1l, (full + each - 1) / each);
+                }
+            }
+    } else {
+        const int bk = kTileBytes / element_size(dtype);
+        const long kt = (k + bk - 1) / bk * segs;
+        p.bm = m > 64 && tiles(128, 128) >= 256 ? 128 : 64;
+        p.bn = 128;
+        const long t = std::max(1l, tiles(p.bm, p.bn));
+        // too few tiles for the chip: k is split so that about 512 workgroups run, each with at least four k tiles
+        long splits = t >= 256 ? 1 : std::max(1l, std::min({512 / t, kt / 4, 256l, (long)(kMostPartial / std::max(plane, 1.0))}));
+        p.tiles_per_split = std::max(1l, (kt + splits - 1) / splits);
+        p.splits = (int)std::max(1l, (kt + p.tiles_per_split - 1) / p.tiles_per_split);
     }
-    const long t = std::max(1l, tiles(p.bm, p.bn));
-    // too few tiles for the chip: k is split so that about 512 workgroups run, each with at least four k tiles
-    long splits = t >= 256 ? 1 : std::max(1l, std::min({512 / t, kt / 4, 256l}));
-    p.tiles_per_split = std::max(1l, (kt + splits - 1) / splits);
-    splits = std::max(1l, (kt + p.tiles_per_split - 1) / p.tiles_per_split);
-    p.splits = (int)splits;
-    p.partial_bytes = splits > 1 ? (size_t)splits * batch * (gated ? 2 : 1) * m * n * sizeof(float) : 0;
+    p.partial_bytes = p.splits > 1 ? (size_t)(plane * p.splits) : 0;
     return p;
 }
 

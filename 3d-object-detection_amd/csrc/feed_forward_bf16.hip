@@ -5,7 +5,7 @@
 namespace fpn {
 namespace ff {
 
-template int launch_wide<__bf16>(const Args &, int, int, bool, long, hipStream_t);
+template int launch_wide<__bf16>(const Args &, int, int, bool, int, int, long, hipStream_t);
 template int launch_product<__bf16>(Args, int, int, bool, const Plan &, float *, hipStream_t);
 
 }  // namespace ff

@@ -1,13 +1,13 @@
 // The feed-forward products' kernel for large products of 16-bit operands: 256 x 256 output tiles, operands brought
 // into LDS by loads that write it directly.
 //
-// Four waves, each a 128 x 128 quadrant: 16 MFMA tiles of 32 x 32, 256 accumulator registers, one wave per SIMD.
-// Per 16 of k a wave reads 8 KB of operands from LDS for 512 cycles of MFMA (half of what the LDS delivers); with 128 x 128
-// tiles and 64 x 64 quadrants it is as much for 256 cycles, and the LDS, not the matrix unit, sets the pace.
+// Eight waves, each 128 x 64 of the tile: 8 MFMA tiles of 32 x 32, 128 accumulator registers, two waves per SIMD, so that
+// one wave's MFMAs run while the other's requests wait to be taken (four waves of 128 x 128 read less from LDS,
+// but every request that waited stopped the SIMD: 247 us against XXX at 8192 x 4096 x 4096).
 //
-// LDS holds four stages of 32 k (32 KB each).  A wave requests its quarter of stage t + 4 as soon as everyone has read
+// LDS holds four stages of 32 k (32 KB each).  A wave requests its eighth of stage t + 4 as soon as everyone has read
 // stage t, so a request has three stages' time (3072 cycles of MFMA) to arrive, and reads the next 16 of k
-// while it multiplies the present ones: one barrier per 32 MFMAs, nothing else waits.
+// while it multiplies the present ones: one barrier per 32 of k, nothing else waits.
 //
 // The requests are written in assembly because the compiler, which cannot tell the stages apart, would wait for all of
 // them before every LDS read.  They have no result registers; the counts in `arrive` are theirs alone, since the loop
@@ -19,8 +19,19 @@ namespace fpn {
 namespace ff {
 
 constexpr int kWideK = 32;                                  // k per stage
-constexpr int kStages = 4;
-constexpr int kWideStage = 512 * kWideK * 2;                // bytes: 256 rows of a, 256 of b
+// A shape of workgroup: BM x BN tile, WM x WN waves of TM x TN MFMA tiles, stages of 32 k in LDS, workgroups per CU.
+template <int BM_, int BN_, int WM_, int WN_, int STAGES, int PER_CU> struct Shape {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, kStages = STAGES;
+    static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves, TM = BM / WM / 32, TN = BN / WN / 32;
+    static constexpr int kStage = (BM + BN) * kWideK * 2;            // bytes: BM rows of a, BN of b
+    static constexpr int kPerSimd = kWaves * PER_CU / 4;
+    // the epilogue's piece of LDS of a wave: 32 rows of its columns, as floats
+    static constexpr int kEpilogueRow = 32 * TN * 4 + 16, kEpilogueBytes = 32 * kEpilogueRow;
+    static constexpr int kBytes = std::max(kStages * kStage, kWaves * kEpilogueBytes);
+};
+using Large = Shape<256, 256, 2, 4, 4, 1>;
+using Medium = Shape<256, 128, 2, 2, 3, 2>;
+using Small = Shape<128, 128, 4, 2, 4, 2>;
 
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"             // (m0 is reserved: nothing here indexes registers through it)
@@ -36,8 +47,13 @@ template <int AT> __device__ inline void request(unsigned lds, unsigned off, con
 // everyone's.
 template <int LEFT> __device__ inline void arrive()
 {
-    if (LEFT == 16) asm volatile("s_waitcnt vmcnt(16) lgkmcnt(0)\n\ts_barrier" : : : "memory");
-    else if (LEFT == 20) asm volatile("s_waitcnt vmcnt(20) lgkmcnt(0)\n\ts_barrier" : : : "memory");
+    static_assert(LEFT == 0 || LEFT == 4 || LEFT == 5 || LEFT == 6 || LEFT == 8 || LEFT == 9 || LEFT == 10, "a count written out below");
+    if (LEFT == 4) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" : : : "memory");
+    else if (LEFT == 5) asm volatile("s_waitcnt vmcnt(5) lgkmcnt(0)\n\ts_barrier" : : : "memory");
+    else if (LEFT == 6) asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)\n\ts_barrier" : : : "memory");
+    else if (LEFT == 8) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" : : : "memory");
+    else if (LEFT == 9) asm volatile("s_waitcnt vmcnt(9) lgkmcnt(0)\n\ts_barrier" : : : "memory");
+    else if (LEFT == 10) asm volatile("s_waitcnt vmcnt(10) lgkmcnt(0)\n\ts_barrier" : : : "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
 }
 
@@ -49,8 +65,8 @@ __device__ inline unsigned lds_address(const char *p)
 // One operand's R rows (m or n) x 32 k of a stage.  A request fills 1 KB: kInner 16 rows of 64 bytes, the four 16-byte
 // chunks of row r permuted by r >> 2 & 3; kOuter 2 or 4 rows (k) of R elements, permuted as in Tile.  The permutation is on
 // the source side: the lane that fills a slot fetches the chunk that belongs there.
-template <class T, int ORDER, int R> struct Stream {
-    static constexpr int kPer = R * 64 / 1024 / 4;          // requests per wave
+template <class T, int ORDER, int R, int WAVES> struct Stream {
+    static constexpr int kPer = R * 64 / 1024 / WAVES; // requests per wave
     static constexpr int kRowBytes = R * 2;                 // kOuter
     const char *base;                                       // uniform: k = 0 of the segment
     const char *next;                                       // the stage to be requested next
@@ -67,7 +83,7 @@ template <class T, int ORDER, int R> struct Stream {
         } else {
             constexpr int kLanes = kRowBytes / 16;
             row = q * (64 / kLanes) + lane / kLanes;
-            const int g = ((row & 1) << 1) ^ ((row >> 1 & 1) * 5);
+            const int g = (((row & 1) << 1) ^ ((row >> 1 & 1) * 5)) & (R / 16 - 1);
             first = ((lane % kLanes >> 1) ^ g) * 16 + (lane & 1) * 8;
         }
     }
@@ -113,12 +129,12 @@ template <class T, int ORDER, int R> struct Stream {
     }
 };
 
-// A lane's operands of four 32-row groups, 16 of k at a time
-template <class T, int ORDER, int R> struct StreamReader {
+// A lane's operands of TILES 32-row groups, 16 of k at a time
+template <class T, int ORDER, int R, int TILES> struct StreamReader {
     static constexpr int kRowBytes = R * 2;
-    unsigned at[ORDER == kInner ? 2 : 4];
+    unsigned at[ORDER == kInner ? 2 : TILES];
 
-    __device__ void init(const int (&first)[4], int lane)
+    __device__ void init(const int (&first)[TILES], int lane)
     {
         const int l31 = lane & 31, h = lane >> 5;
         if (ORDER == kInner) {
@@ -126,7 +142,7 @@ template <class T, int ORDER, int R> struct StreamReader {
             for (int s = 0; s < 2; ++s) at[s] = l31 * 64 + (((2 * s + h) ^ (l31 >> 2 & 3)) << 4);
         } else {
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+            for (int t = 0; t < TILES; ++t)
                 at[t] = Tile<T, kOuter, R>::outer_at(8 * h + (lane >> 2 & 3), first[t] + (lane & 16) + 4 * (lane & 3));
         }
     }
@@ -148,21 +164,19 @@ template <class T, int ORDER, int R> struct StreamReader {
 // consecutive columns of one row), read back as runs of eight columns of consecutive rows - whole lines for the
 // loads and stores, one copy of the epilogue's arithmetic, bias loaded once.  `lds` is the wave's:
 // kEpilogueBytes; nobody else uses it.
-constexpr int kEpilogueRow = 128 * 4 + 16;
-constexpr int kEpilogueBytes = 32 * kEpilogueRow;
-
-template <class T, bool GATED>
-__device__ inline void store_quadrant(const Args &p, const floatx16 (&acc)[4][4], char *lds, int member, int split, long m0, int n0, int lane)
+template <class T, bool GATED, class S>
+__device__ inline void store_piece(const Args &p, const floatx16 (&acc)[S::TM][S::TN], char *lds, int member, int split, long m0, int n0, int lane)
 {
     constexpr bool EXACT = sizeof(T) == 4;
+    constexpr int kTN = S::TN, kEpilogueRow = S::kEpilogueRow;
     const int l31 = lane & 31, h = lane >> 5;
-    constexpr int kRuns = GATED ? 8 : 16, kRowsAtOnce = 64 / kRuns, kBatch = 4;     // runs of eight columns per row
+    constexpr int kRuns = GATED ? 2 * kTN : 4 * kTN, kRowsAtOnce = 64 / kRuns, kBatch = 2;     // runs of eight columns per row
     const int run = lane % kRuns, row0 = lane / kRuns;
     const int n = n0 + run * 8;
     const long left = p.n - n;
-    auto put = [&](const floatx16 (&c)[4]) {
+    auto put = [&](const floatx16 (&c)[kTN]) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < kTN; ++j)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 floatx4 v;
@@ -175,13 +189,13 @@ __device__ inline void store_quadrant(const Args &p, const floatx16 (&acc)[4][4]
     if (left > 0 && p.bias[GATED ? 0 : member]) load8(reinterpret_cast<const T *>(p.bias[GATED ? 0 : member]) + n, left, bias);
     if (GATED && left > 0 && p.bias[1]) load8(reinterpret_cast<const T *>(p.bias[1]) + n, left, bias2);
 #pragma unroll 1
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < S::TM; ++i) {
         if (i == 0) put(acc[0]);
-        else if (i == 1) put(acc[1]);
-        else if (i == 2) put(acc[2]);
-        else put(acc[3]);
+        else if (S::TM == 2 || i == 1) put(acc[S::TM > 1 ? 1 : 0]);
+        else if (i == 2) put(acc[S::TM > 2 ? 2 : 0]);
+        else put(acc[S::TM > 2 ? 3 : 0]);
         if (left <= 0) continue;
-        // four rows' loads at a time, then their arithmetic, then their stores: with one wave per SIMD nothing else
+        // two rows' loads at a time, then their arithmetic, then their stores: with one wave per SIMD nothing else
         // would cover the latency
 #pragma unroll 1
         for (int r = row0; r < 32; r += kRowsAtOnce * kBatch) {
@@ -197,7 +211,7 @@ __device__ inline void store_quadrant(const Args &p, const floatx16 (&acc)[4][4]
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     v[b][e] = from[e];
-                    if (GATED) v2[b][e] = from[64 + e];
+                    if (GATED) v2[b][e] = from[16 * kTN + e];
                 }
             }
             if (p.partial) {
@@ -244,33 +258,38 @@ __device__ inline void store_quadrant(const Args &p, const floatx16 (&acc)[4][4]
     }
 }
 
-template <class T, int ORDER_A, int ORDER_B, bool GATED>
-__global__ __launch_bounds__(kThreads) void wide_product_kernel(const Args p)
+template <class T, int ORDER_A, int ORDER_B, bool GATED, class S>
+__global__ __launch_bounds__(S::kThreads, S::kPerSimd) void wide_product_kernel(const Args p)
 {
     extern __shared__ char lds[];
-    constexpr int kHalves = GATED ? 2 : 1, kCols = 256 / kHalves, kABytes = 256 * kWideK * 2;
+    constexpr int kWaves = S::kWaves, kStages = S::kStages, kStage = S::kStage, kTM = S::TM, kTN = S::TN, BM = S::BM;
+    constexpr int kHalves = GATED ? 2 : 1, kCols = S::BN / kHalves, kABytes = BM * kWideK * 2, kHalfBytes = kCols * kWideK * 2;
+    // (where a half of b is less than a request per wave, half of the waves request each)
+    constexpr bool kDealt = GATED && kHalfBytes / 1024 < kWaves;
+    constexpr int kStreams = kDealt ? 1 : kHalves, kWavesB = kDealt ? kWaves / 2 : kWaves;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = wave & 1, wn = wave >> 1;
+    const int wm = wave % S::WM, wn = wave / S::WM;
+    const int wave_b = wave % kWavesB, dealt = wave / kWavesB;
     const Place at = place(p, blockIdx.x, gridDim.x);
-    const long m0 = at.mt * 256;
+    const long m0 = at.mt * BM;
     const int n0 = at.nt * kCols;
 
-    int am[4], bn[4];
+    int am[kTM], bn[kTN];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) am[i] = wm * 128 + i * 32;
-    // GATED: two column groups of the gate half, then the same columns of the up half
+    for (int i = 0; i < kTM; ++i) am[i] = (wm * kTM + i) * 32;
+    // GATED: the first half of a wave's column tiles are of the gate half, the second the same columns of the up half
 #pragma unroll
-    for (int j = 0; j < 4; ++j) bn[j] = GATED ? wn * 64 + j % 2 * 32 : wn * 128 + j * 32;
-    StreamReader<T, ORDER_A, 256> ra;
-    StreamReader<T, ORDER_B, kCols> rb;
+    for (int j = 0; j < kTN; ++j) bn[j] = GATED ? (wn * (kTN / 2) + j % (kTN / 2)) * 32 : (wn * kTN + j) * 32;
+    StreamReader<T, ORDER_A, BM, kTM> ra;
+    StreamReader<T, ORDER_B, kCols, kTN> rb;
     ra.init(am, lane);
     rb.init(bn, lane);
 
-    floatx16 acc[4][4];
+    floatx16 acc[kTM][kTN];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < kTM; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < kTN; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
@@ -278,25 +297,28 @@ __global__ __launch_bounds__(kThreads) void wide_product_kernel(const Args p)
     const long first = at.split * p.tiles_per_split, last = min(first + p.tiles_per_split, full * p.segs);
     const unsigned lds0 = lds_address(lds);
 
-    Stream<T, ORDER_A, 256> sa;
-    Stream<T, ORDER_B, kCols> sb[kHalves];
+    Stream<T, ORDER_A, BM, kWaves> sa;
+    Stream<T, ORDER_B, kCols, kWavesB> sb[kStreams];
     auto segment = [&](int s) {
         sa.init(p.a[s], p.lda[s], m0, p.m - m0, wave, lane);
-        if (GATED) {
+        if (kDealt) {
+            sb[0].init(dealt ? p.b[1] : p.b[0], dealt ? p.ldb[1] : p.ldb[0], n0, p.n - n0, wave_b, lane);
+        } else if (GATED) {
             sb[0].init(p.b[0], p.ldb[0], n0, p.n - n0, wave, lane);
-            sb[kHalves - 1].init(p.b[1], p.ldb[1], n0, p.n - n0, wave, lane);
+            sb[kStreams - 1].init(p.b[1], p.ldb[1], n0, p.n - n0, wave, lane);
         } else {
             sb[0].init(p.b[s + at.member], p.ldb[s + at.member], n0, p.n - n0, wave, lane);
         }
     };
-    // request Q of a wave's eight of a stage
-    constexpr int kPerB = Stream<T, ORDER_B, kCols>::kPer;
-    const unsigned lds_a = lds0 + wave * 4096, lds_b = lds0 + kABytes + wave * (kPerB * 1024);
+    // request Q of a wave's kPer of a stage
+    constexpr int kPerA = decltype(sa)::kPer, kPerB = Stream<T, ORDER_B, kCols, kWavesB>::kPer, kPer = kPerA + kStreams * kPerB;
+    static_assert(kPer % 2 == 0 && kPerA > 0 && kPerB > 0, "half a stage's requests per step");
+    const unsigned lds_a = lds0 + wave * (kPerA * 1024), lds_b = lds0 + kABytes + (kDealt ? dealt * kHalfBytes : 0) + wave_b * (kPerB * 1024);
     auto issue = [&](auto q, int stage) {
         constexpr int Q = decltype(q)::value;
-        if constexpr (Q < 4) sa.template issue<Q>(lds_a + stage * kWideStage);
-        else if constexpr (Q < 4 + kPerB) sb[0].template issue<Q - 4>(lds_b + stage * kWideStage);
-        else sb[kHalves - 1].template issue<(Q - 4) % kPerB>(lds_b + kCols * kWideK * 2 + stage * kWideStage);
+        constexpr int G = (Q - kPerA) / kPerB * (Q >= kPerA);
+        if constexpr (Q < kPerA) sa.template issue<Q>(lds_a + stage * kStage);
+        else sb[G].template issue<(Q - kPerA) % kPerB>(lds_b + G * kHalfBytes + stage * kStage);
     };
     long asked = 0, most = 0;                               // stages whose requests are complete, and the last to ask for
     auto advance = [&] {
@@ -304,38 +326,43 @@ __global__ __launch_bounds__(kThreads) void wide_product_kernel(const Args p)
         ++asked;
         sa.next += on ? sa.step : 0;
 #pragma unroll
-        for (int g = 0; g < kHalves; ++g) sb[g].next += on ? sb[g].step : 0;
+        for (int g = 0; g < kStreams; ++g) sb[g].next += on ? sb[g].step : 0;
     };
     auto read_a = [&](const char *stage, int i, int s) { return ra.frag(stage, am[i], i, s); };
     auto read_b = [&](const char *stage, int j, int s) {
-        return rb.frag(stage + kABytes + (GATED && j >= 2 ? kCols * kWideK * 2 : 0), bn[j], j, s);
+        return rb.frag(stage + kABytes + (GATED && j >= kTN / 2 ? kHalfBytes : 0), bn[j], j, s);
     };
-    // 16 of k: multiplies ca, cb while na, nb come from `stage`, and issues requests Q .. Q + 3 to stage `to`.  A wave
+    // 16 of k: multiplies ca, cb while na, nb come from `stage`, and issues half a stage's requests from Q on to stage `to`.  A wave
     // issues in order: an MFMA occupies its unit for 32 cycles, in which seven other instructions can go out, so the
     // reads and requests are dealt out among the MFMAs one by one (all in front of a group of four MFMAs cost 12 %);
-    // no read is left for the last quarter, which covers their latency.
-    auto step = [&](const uintx4 (&ca)[4], const uintx4 (&cb)[4], uintx4 (&na)[4], uintx4 (&nb)[4], const char *stage, int s,
+    // no read is left for the last two, which cover their latency.
+    auto step = [&](const uintx4 (&ca)[kTM], const uintx4 (&cb)[kTN], uintx4 (&na)[kTM], uintx4 (&nb)[kTN], const char *stage, int s,
                     auto q, int to) {
         constexpr int Q = decltype(q)::value;
+        constexpr int kAll = kTM * kTN, kHalf = kPer / 2;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            acc[i & 3][i >> 2] = multiply<T>(cb[i >> 2], ca[i & 3], acc[i & 3][i >> 2]);
-            if (i == 0) na[0] = read_a(stage, 0, s);
-            if (i == 1) na[1] = read_a(stage, 1, s);
-            if (i == 2) issue(ActTag<Q>(), to);
-            if (i == 3) na[2] = read_a(stage, 2, s);
-            if (i == 4) na[3] = read_a(stage, 3, s);
-            if (i == 5) nb[0] = read_b(stage, 0, s);
-            if (i == 6) issue(ActTag<Q + 1>(), to);
-            if (i == 7) nb[1] = read_b(stage, 1, s);
-            if (i == 8) nb[2] = read_b(stage, 2, s);
-            if (i == 9) nb[3] = read_b(stage, 3, s);
-            if (i == 10) issue(ActTag<Q + 2>(), to);
-            if (i == 12) issue(ActTag<Q + 3>(), to);
+        for (int i = 0; i < kAll; ++i) {
+            acc[i % kTM][i / kTM] = multiply<T>(cb[i / kTM], ca[i % kTM], acc[i % kTM][i / kTM]);
+#pragma unroll
+            for (int r = 0; r < kTM + kTN; ++r)
+                if (r * kAll / (kTM + kTN + 2) == i) {
+                    if (r < kTM) na[r] = read_a(stage, r, s);
+                    else nb[r - kTM] = read_b(stage, r - kTM, s);
+                }
+            if (kAll / (2 * kHalf) == i) issue(ActTag<Q>(), to);
+            if (kHalf > 1 && 3 * kAll / (2 * kHalf) == i) issue(ActTag<Q + (kHalf > 1)>(), to);
+            if (kHalf > 2 && 5 * kAll / (2 * kHalf) == i) issue(ActTag<Q + 2 * (kHalf > 2)>(), to);
+            static_assert(kHalf <= 3, "a request written out above");
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    uintx4 fa[2][4], fb[2][4];
+    uintx4 fa[2][kTM], fb[2][kTN];
+    auto read = [&](uintx4 (&a)[kTM], uintx4 (&b)[kTN], int s) {             // of the first stage
+#pragma unroll
+        for (int i = 0; i < kTM; ++i) a[i] = read_a(lds, i, s);
+#pragma unroll
+        for (int j = 0; j < kTN; ++j) b[j] = read_b(lds, j, s);
+    };
 
     // segment by segment; a segment's whole stages in this split are [t0, t1)
     for (int s = 0; s < p.segs; ++s) {
@@ -350,31 +377,28 @@ __global__ __launch_bounds__(kThreads) void wide_product_kernel(const Args p)
             asked = 0;
             sa.next = sa.base + t0 * sa.step;
 #pragma unroll
-            for (int g = 0; g < kHalves; ++g) sb[g].next = sb[g].base + t0 * sb[g].step;
+            for (int g = 0; g < kStreams; ++g) sb[g].next = sb[g].base + t0 * sb[g].step;
 #pragma unroll
             for (int i = 0; i < kStages; ++i) {
                 issue(ActTag<0>(), i);
-                issue(ActTag<1>(), i);
-                issue(ActTag<2>(), i);
-                issue(ActTag<3>(), i);
+                if constexpr (kPer > 2) issue(ActTag<1>(), i);
+                if constexpr (kPer > 4) issue(ActTag<2>(), i);
                 if (i == kStages - 1) break;
-                issue(ActTag<4>(), i);
-                issue(ActTag<5>(), i);
-                issue(ActTag<6>(), i);
-                issue(ActTag<7>(), i);
+                issue(ActTag<kPer / 2>(), i);
+                if constexpr (kPer > 2) issue(ActTag<kPer / 2 + (kPer > 2)>(), i);
+                if constexpr (kPer > 4) issue(ActTag<kPer - 1>(), i);
                 advance();
             }
-            arrive<20>();
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { fa[0][i] = read_a(lds, i, 0); fb[0][i] = read_b(lds, i, 0); }
+            arrive<(kStages - 2) * kPer + kPer / 2>();
+            read(fa[0], fb[0], 0);
             int stage = 0;
             for (long t = 0; t < n; ++t) {
-                step(fa[0], fb[0], fa[1], fb[1], lds + stage * kWideStage, 1, ActTag<4>(), (stage + 3) & 3);
+                step(fa[0], fb[0], fa[1], fb[1], lds + stage * kStage, 1, ActTag<kPer / 2>(), stage ? stage - 1 : kStages - 1);
                 advance();
-                arrive<16>();
+                arrive<(kStages - 2) * kPer>();
                 const int freed = stage;
-                stage = (stage + 1) & 3;
-                step(fa[1], fb[1], fa[0], fb[0], lds + stage * kWideStage, 0, ActTag<0>(), freed);
+                stage = stage == kStages - 1 ? 0 : stage + 1;
+                step(fa[1], fb[1], fa[0], fb[0], lds + stage * kStage, 0, ActTag<0>(), freed);
             }
             arrive<0>();
         }
@@ -383,36 +407,32 @@ __global__ __launch_bounds__(kThreads) void wide_product_kernel(const Args p)
         if (left && at.split == p.splits - 1) {
             __syncthreads();
             sa.put_tail(lds, full, left, wave, lane);
-            sb[0].put_tail(lds + kABytes, full, left, wave, lane);
-            if (GATED) sb[kHalves - 1].put_tail(lds + kABytes + kCols * kWideK * 2, full, left, wave, lane);
+#pragma unroll
+            for (int g = 0; g < kStreams; ++g)
+                sb[g].put_tail(lds + kABytes + (kDealt ? dealt * kHalfBytes : g * kHalfBytes), full, left, wave_b, lane);
             __syncthreads();
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
+                read(fa[0], fb[0], q);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) { fa[0][i] = read_a(lds, i, q); fb[0][i] = read_b(lds, i, q); }
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[i][j] = multiply<T>(fb[0][j], fa[0][i], acc[i][j]);
+                for (int i = 0; i < kTM * kTN; ++i) acc[i % kTM][i / kTM] = multiply<T>(fb[0][i / kTM], fa[0][i % kTM], acc[i % kTM][i / kTM]);
             }
         }
         __syncthreads();
     }
-    store_quadrant<T, GATED>(p, acc, lds + wave * kEpilogueBytes, at.member, at.split, m0 + wm * 128,
-                             n0 + (GATED ? wn * 64 : wn * 128), lane);
+    store_piece<T, GATED, S>(p, acc, lds + wave * S::kEpilogueBytes, at.member, at.split, m0 + wm * 32 * kTM,
+                             n0 + wn * 32 * (GATED ? kTN / 2 : kTN), lane);
 }
 
 #define FPN_FF_WIDE(A, B, G)                                                                                                  \
     do {                                                                                                                      \
-        auto kern = wide_product_kernel<T, A, B, G>;                                                                          \
-        const size_t bytes = kStages * kWideStage;                                                                            \
-        static_assert(4 * kEpilogueBytes <= kStages * kWideStage, "the epilogue's pieces lie in the stages");                 \
-        if (!allow_dynamic_lds(reinterpret_cast<const void *>(kern), bytes))                                                  \
-            return fail(FPN_E_LAUNCH, "%zu bytes of LDS refused", bytes);                                                     \
-        hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(kThreads), bytes, stream, p);                                   \
+        auto kern = wide_product_kernel<T, A, B, G, S>;                                                                       \
+        if (!allow_dynamic_lds(reinterpret_cast<const void *>(kern), S::kBytes))                                              \
+            return fail(FPN_E_LAUNCH, "%d bytes of LDS refused", S::kBytes);                                                  \
+        hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(S::kThreads), S::kBytes, stream, p);                            \
     } while (0)
 
-template <class T> int launch_wide(const Args &p, int order_a, int order_b, bool gated, long blocks, hipStream_t stream)
+template <class T, class S> int launch_shape(const Args &p, int order_a, int order_b, bool gated, long blocks, hipStream_t stream)
 {
     if (gated) {
         if (order_b == kOuter) FPN_FF_WIDE(kInner, kOuter, true);
@@ -425,6 +445,13 @@ template <class T> int launch_wide(const Args &p, int order_a, int order_b, bool
         FPN_FF_WIDE(kInner, kInner, false);
     }
     return check_launch("feed-forward product, wide");
+}
+
+template <class T> int launch_wide(const Args &p, int order_a, int order_b, bool gated, int bm, int bn, long blocks, hipStream_t stream)
+{
+    if (bn == 256) return launch_shape<T, Large>(p, order_a, order_b, gated, blocks, stream);
+    if (bm == 256) return launch_shape<T, Medium>(p, order_a, order_b, gated, blocks, stream);
+    return launch_shape<T, Small>(p, order_a, order_b, gated, blocks, stream);
 }
 
 }  // namespace ff
