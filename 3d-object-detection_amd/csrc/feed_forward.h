@@ -689,14 +689,15 @@ template <class T, bool GATED> __global__ __launch_bounds__(kThreads) void join_
 
 // How a product is cut: tile, splits of k, and the bytes of partial sums that takes
 struct Plan {
-    bool wide;              // the 256 x 256 kernel (feed_forward_wide.h)
+    bool few;               // the few-row kernel (feed_forward_few.h), its MT and NT in bm and bn
+    bool wide;              // the kernel of feed_forward_wide.h
     int bm, bn;
     int splits;
     long tiles_per_split;
     size_t partial_bytes;
 };
 // (aligned: every operand consists of whole 16-byte chunks at 16-byte addresses)
-Plan plan_product(int dtype, long m, int n, long k, int segs, int batch, bool gated, bool aligned);
+Plan plan_product(int dtype, long m, int n, long k, int segs, int batch, bool gated, bool aligned, int order_a, int order_b);
 
 // whether an operand consists of whole 16-byte chunks
 inline bool whole_chunks(const void *p, long ld, int order, long extent, int element)
@@ -704,6 +705,7 @@ inline bool whole_chunks(const void *p, long ld, int order, long extent, int ele
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * element % 16 == 0 && (order == kInner || extent * element % 16 == 0);
 }
 
+template <class T> int launch_few(const Args &p, int order_b, bool gated, int mt, int nt, hipStream_t stream);
 template <class T> int launch_wide(const Args &p, int order_a, int order_b, bool gated, int bm, int bn, long blocks, hipStream_t stream);
 
 // Launches a planned product (p.partial and the plan's fields are filled in here)
@@ -715,6 +717,9 @@ extern template int launch_product<__bf16>(Args, int, int, bool, const Plan &, f
 extern template int launch_product<_Float16>(Args, int, int, bool, const Plan &, float *, hipStream_t);
 extern template int launch_wide<__bf16>(const Args &, int, int, bool, int, int, long, hipStream_t);
 extern template int launch_wide<_Float16>(const Args &, int, int, bool, int, int, long, hipStream_t);
+extern template int launch_few<float>(const Args &, int, bool, int, int, hipStream_t);
+extern template int launch_few<__bf16>(const Args &, int, bool, int, int, hipStream_t);
+extern template int launch_few<_Float16>(const Args &, int, bool, int, int, hipStream_t);
 #endif
 
 #define FPN_FF_LAUNCH(A, B, BM_, BN_, WM_, WN_, G)                                                                            \
@@ -742,14 +747,29 @@ int launch_tiles(const Args &p, int order_a, int order_b, bool gated, long block
     return check_launch("feed-forward product");
 }
 
+template <class T> int launch_join(const Args &p, bool gated, hipStream_t stream)
+{
+    const long runs8 = p.m * ((p.n + 7) / 8);
+    const long join_blocks = (runs8 + 31) / 32;
+    if (join_blocks > 0x7fffffffl) return fail(FPN_E_UNSUPPORTED, "a join of %ld workgroups", join_blocks);
+    const dim3 grid((unsigned)join_blocks, p.batch);
+    if (gated) hipLaunchKernelGGL((join_kernel<T, true>), grid, dim3(kThreads), 0, stream, p);
+    else hipLaunchKernelGGL((join_kernel<T, false>), grid, dim3(kThreads), 0, stream, p);
+    return check_launch("join of a split product");
+}
+
 template <class T> int launch_product(Args p, int order_a, int order_b, bool gated, const Plan &plan, float *partial, hipStream_t stream)
 {
-    const int cols = gated ? plan.bn / 2 : plan.bn;
-    p.mt = (p.m + plan.bm - 1) / plan.bm;
-    p.nt = (p.n + cols - 1) / cols;
     p.splits = plan.splits;
     p.tiles_per_split = plan.tiles_per_split;
     p.partial = plan.splits > 1 ? partial : nullptr;
+    if (plan.few) {
+        const int rc = launch_few<T>(p, order_b, gated, plan.bm, plan.bn, stream);
+        return rc != FPN_OK || !p.partial ? rc : launch_join<T>(p, gated, stream);
+    }
+    const int cols = gated ? plan.bn / 2 : plan.bn;
+    p.mt = (p.m + plan.bm - 1) / plan.bm;
+    p.nt = (p.n + cols - 1) / cols;
     const long blocks = p.mt * p.nt * p.splits * p.batch;
     if (blocks > 0x7fffffffl) return fail(FPN_E_UNSUPPORTED, "a product of %ld workgroups", blocks);
     int rc;
@@ -759,13 +779,7 @@ template <class T> int launch_product(Args p, int order_a, int order_b, bool gat
     } else if (plan.bm == 128) rc = launch_tiles<T, 128, 128, 2, 2>(p, order_a, order_b, gated, blocks, stream);
     else rc = launch_tiles<T, 64, 128, 2, 2>(p, order_a, order_b, gated, blocks, stream);
     if (rc != FPN_OK || !p.partial) return rc;
-    const long runs8 = p.m * ((p.n + 7) / 8);
-    const long join_blocks = (runs8 + 31) / 32;
-    if (join_blocks > 0x7fffffffl) return fail(FPN_E_UNSUPPORTED, "a join of %ld workgroups", join_blocks);
-    const dim3 grid((unsigned)join_blocks, p.batch);
-    if (gated) hipLaunchKernelGGL((join_kernel<T, true>), grid, dim3(kThreads), 0, stream, p);
-    else hipLaunchKernelGGL((join_kernel<T, false>), grid, dim3(kThreads), 0, stream, p);
-    return check_launch("join of a split product");
+    return launch_join<T>(p, gated, stream);
 }
 
 }  // namespace ff

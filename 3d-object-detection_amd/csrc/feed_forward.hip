@@ -124,11 +124,15 @@ int launch_grad(GradArgs p, bool gated, void *const (&sums_out)[2], hipStream_t 
 
 int element_size(int dtype) { return dtype == FPN_F32 ? 4 : 2; }
 
-// the larger of the partial sums of a product's two plans
-size_t partial_bytes(int dtype, long m, int n, long k, int segs, int batch, bool gated)
+// the largest of the partial sums that a product's plans ask for, whatever its operands' alignment and b's order
+size_t partial_bytes(int dtype, long m, int n, long k, int segs, int batch, bool gated, int order_a)
 {
-    return std::max(plan_product(dtype, m, n, k, segs, batch, gated, false).partial_bytes,
-                    plan_product(dtype, m, n, k, segs, batch, gated, true).partial_bytes);
+    size_t most = 0;
+    for (int aligned = 0; aligned < 2; ++aligned)
+        for (int order_b : {kInner, kOuter})
+            if (order_a == kInner || order_b == kOuter)
+                most = std::max(most, plan_product(dtype, m, n, k, segs, batch, gated, aligned, order_a, order_b).partial_bytes);
+    return most;
 }
 
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
@@ -136,12 +140,13 @@ size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 int run_product(int dtype, const Args &p, int order_a, int order_b, bool gated, float *partial, size_t partial_bytes, hipStream_t stream)
 {
     bool aligned = true;
-    for (int i = 0; i < p.segs; ++i) aligned = aligned && whole_chunks(p.a[i], p.lda[i], order_a, p.m, element_size(dtype));
+    for (int i = 0; i < p.segs; ++i)
+        aligned = aligned && whole_chunks(p.a[i], order_a == kInner && p.m == 1 ? 0 : p.lda[i], order_a, p.m, element_size(dtype));
     for (int i = 0; i < std::max({p.segs, p.batch, gated ? 2 : 1}); ++i)
         aligned = aligned && whole_chunks(p.b[i], p.ldb[i], order_b, p.n, element_size(dtype));
-    const Plan plan = plan_product(dtype, p.m, p.n, p.k, p.segs, p.batch, gated, aligned);
-    if (plan.partial_bytes > partial_bytes)
-        return fail(FPN_E_INVALID_ARG, "workspace: %zu bytes of partial sums needed, %zu there", plan.partial_bytes, partial_bytes);
+    const Plan plan = plan_product(dtype, p.m, p.n, p.k, p.segs, p.batch, gated, aligned, order_a, order_b);
+    if (plan.partial_bytes && (!partial || plan.partial_bytes > partial_bytes))
+        return fail(FPN_E_INVALID_ARG, "workspace of %zu bytes needed for partial sums, got %zu", plan.partial_bytes, partial ? partial_bytes : 0);
     if (dtype == FPN_F32) return launch_product<float>(p, order_a, order_b, gated, plan, partial, stream);
     if (dtype == FPN_BF16) return launch_product<__bf16>(p, order_a, order_b, gated, plan, partial, stream);
     return launch_product<_Float16>(p, order_a, order_b, gated, plan, partial, stream);
@@ -198,8 +203,9 @@ GradSpace grad_space(int dtype, long rows, int cin, int n, bool gated, bool with
     const int planes = gated ? 2 : 1;
     s.d = with_d ? align256((size_t)rows * n * element_size(dtype)) * planes : 0;
     s.sums = align256((size_t)grad_rows_grid(rows, n) * planes * n * sizeof(float));
-    s.partial = align256(std::max({partial_bytes(dtype, rows, cin, n, planes, 1, false), partial_bytes(dtype, cin, n, rows, 1, planes, false),
-                                   partial_bytes(dtype, n, cin, rows, 1, 1, false)}));
+    s.partial = align256(std::max({partial_bytes(dtype, rows, cin, n, planes, 1, false, kInner),
+                                   partial_bytes(dtype, cin, n, rows, 1, planes, false, kOuter),
+                                   partial_bytes(dtype, n, cin, rows, 1, 1, false, kOuter)}));
     s.total = s.d + s.sums + s.partial;
     return s;
 }
@@ -277,13 +283,35 @@ double join_time(double bytes) { return bytes > 0 ? 4.0 + bytes / 1.5e6 : 0.0; }
 
 }  // namespace
 
-Plan plan_product(int dtype, long m, int n, long k, int segs, int batch, bool gated, bool aligned)
+namespace {
+
+Plan make_plan(int dtype, long m, int n, long k, int segs, int batch, bool gated, bool aligned, int order_a, int order_b, int cus)
 {
     Plan p = {};
-    const int cus = current_device_cus() > 0 ? current_device_cus() : 256;
     auto tiles = [&](int bm, int bn) { return (m + bm - 1) / bm * ((n + (gated ? bn / 2 : bn) - 1) / (gated ? bn / 2 : bn)) * batch; };
     const double plane = (double)batch * (gated ? 2 : 1) * m * n * sizeof(float);
     constexpr double kMostPartial = 128 << 20;
+    // Few rows: the kernel that streams the weights, measured (graphs of calls, bf16, us) against the wide kernel with k split:
+    // 1024 x 512 4.6 : 9 at 1 row, 6 : 9 at 64; 4096 x 4096 held (out,in) 8.2 : 15 at 1 row, 12.6 : 14.3 at 32, 17.5 : 15.5 at 64,
+    // held (in,out) 12.2 : 14.8, 14.3 : 14.2, 17.8 : 15.8; gated 17.5 : 23 and 25 : 27 at 1 row, 20 : 22 and 26 : 23 at 16.
+    const bool big = (double)k * n * (gated ? 2 : 1) * element_size(dtype) > 8e6;
+    if (aligned && m > 0 && segs == 1 && batch == 1 && order_a == kInner &&
+        m <= (dtype == FPN_F32 || !big ? 64 : !gated ? 32 : order_b == kInner ? 16 : 4)) {
+        p.few = true;
+        p.bm = m <= 16 ? 1 : m <= 32 ? 2 : 4;
+        // Columns per workgroup, in 16.  What a CU has on its way is counted in cache lines, so row-major weights want whole
+        // lines (64 columns, 32 floats) and, where that leaves CUs without work, k split over workgroups; weights held (out,in)
+        // and small ones want as many workgroups as there are CUs.
+        p.splits = 1;
+        const int line = dtype == FPN_F32 ? 2 : 4;
+        if (n >= 32 * cus || (order_b == kOuter && !big && dtype != FPN_F32)) p.bn = 2;
+        else if (order_b == kOuter && big && !(gated && p.bm == 4)) {
+            p.bn = line;
+            while (p.splits < 4 && 2l * p.splits * ((n + 16 * line - 1) / (16 * line)) <= cus) p.splits *= 2;
+        } else p.bn = 1;
+        p.partial_bytes = p.splits > 1 ? (size_t)(plane * p.splits) : 0;
+        return p;
+    }
     if (dtype != FPN_F32 && aligned && m > 0) {
         const long full = k / 32 * segs;
         double best = 0;
@@ -316,6 +344,25 @@ Plan plan_product(int dtype, long m, int n, long k, int segs, int batch, bool ga
     return p;
 }
 
+}  // namespace
+
+// A plan depends on the sizes only; a call asks for a few of them, so each thread keeps the last ones it made.
+Plan plan_product(int dtype, long m, int n, long k, int segs, int batch, bool gated, bool aligned, int order_a, int order_b)
+{
+    struct Entry { long key[4]; Plan plan; };
+    constexpr int kKept = 64;
+    static thread_local Entry kept[kKept] = {};
+    const int cus = current_device_cus() > 0 ? current_device_cus() : 256;
+    const long key[4] = {m, k, n, 1 + (dtype | segs << 4 | batch << 8 | (gated ? 1 << 12 : 0) | (aligned ? 1 << 13 : 0) | order_a << 14 | order_b << 15 |
+                                       (long)cus << 16)};
+    Entry &e = kept[(unsigned long)(key[0] * 31 + key[1] * 17 + key[2] * 7 + key[3] * 3 + (key[3] >> 13)) % kKept];
+    if (!std::equal(key, key + 4, e.key)) {
+        e.plan = make_plan(dtype, m, n, k, segs, batch, gated, aligned, order_a, order_b, cus);
+        std::copy(key, key + 4, e.key);
+    }
+    return e.plan;
+}
+
 }  // namespace ff
 }  // namespace fpn
 
@@ -327,7 +374,7 @@ extern "C" {
 size_t fpn_dense_workspace_bytes(int dtype, long rows, int cin, int cout)
 {
     if (check_common(dtype, rows, cin, cout, FPN_ACT_NONE) != FPN_OK) return 0;
-    return partial_bytes(dtype, rows, cout, cin, 1, 1, false);
+    return partial_bytes(dtype, rows, cout, cin, 1, 1, false, kInner);
 }
 
 int fpn_dense(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w, long ldw, int w_transposed,
@@ -342,7 +389,7 @@ int fpn_dense(int dtype, long rows, int cin, int cout, const void *x, long ldx, 
     FPN_FF_TRY(check_vector("bias", bias, dtype));
     if (residual) FPN_FF_TRY(check_matrix("residual", residual, ldr, cout, dtype, true));
     if (pre) FPN_FF_TRY(check_matrix("pre", pre, ldp, cout, dtype));
-    FPN_FF_TRY(check_workspace(workspace, workspace_bytes, fpn_dense_workspace_bytes(dtype, rows, cin, cout)));
+    FPN_FF_TRY(check_workspace(workspace, workspace_bytes, 0));
     Args p = product(rows, cout, cin);
     p.a[0] = x;
     p.lda[0] = ldx;
@@ -427,7 +474,7 @@ int fpn_dense_grad(int dtype, long rows, int cin, int cout, const void *dy, long
 size_t fpn_gated_workspace_bytes(int dtype, long rows, int cin, int cout)
 {
     if (check_common(dtype, rows, cin, cout, FPN_ACT_NONE) != FPN_OK) return 0;
-    return partial_bytes(dtype, rows, cout, cin, 1, 1, true);
+    return partial_bytes(dtype, rows, cout, cin, 1, 1, true, kInner);
 }
 
 int fpn_gated(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w_gate, long ldg, const void *w_up, long ldu,
@@ -445,7 +492,7 @@ int fpn_gated(int dtype, long rows, int cin, int cout, const void *x, long ldx, 
     FPN_FF_TRY(check_vector("bias_up", bias_up, dtype));
     if (gate) FPN_FF_TRY(check_matrix("gate", gate, ldp, cout, dtype));
     if (up) FPN_FF_TRY(check_matrix("up", up, ldp, cout, dtype));
-    FPN_FF_TRY(check_workspace(workspace, workspace_bytes, fpn_gated_workspace_bytes(dtype, rows, cin, cout)));
+    FPN_FF_TRY(check_workspace(workspace, workspace_bytes, 0));
     Args p = product(rows, cout, cin);
     p.a[0] = x;
     p.lda[0] = ldx;

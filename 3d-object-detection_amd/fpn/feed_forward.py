@@ -34,14 +34,13 @@ def _tensor(name, t, like, shape):
     """The checks that every argument gets: a tensor of the call's type, on its device, of this shape."""
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s must be a torch.Tensor, got %s" % (name, type(t).__name__))
+    if t.dtype is not like.dtype:
+        raise ValueError("%s must be %s like x, got %s" % (name, like.dtype, t.dtype))
     if not t.is_cuda:
         raise ValueError("%s must live on a ROCm device (got %s); this package has no CPU path" % (name, t.device))
-    if like is not None:
-        if t.dtype != like.dtype:
-            raise ValueError("%s must be %s like x, got %s" % (name, like.dtype, t.dtype))
-        if t.device != like.device:
-            raise ValueError("all tensors must be on the same device (%s is on %s, x on %s)" % (name, t.device, like.device))
-    if tuple(t.shape) != tuple(shape):
+    if t.get_device() != like.get_device():
+        raise ValueError("all tensors must be on the same device (%s is on %s, x on %s)" % (name, t.device, like.device))
+    if t.shape != shape:
         raise ValueError("%s has shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
 
 
@@ -52,18 +51,19 @@ def _first(name, x):
         raise ValueError("%s must have rank 2, got shape %s" % (name, tuple(x.shape)))
     if x.dtype not in _DTYPES:
         raise ValueError("%s must be float32, bfloat16 or float16, got %s" % (name, x.dtype))
-    _tensor(name, x, None, x.shape)
+    if not x.is_cuda:
+        raise ValueError("%s must live on a ROCm device (got %s); this package has no CPU path" % (name, x.device))
     return _DTYPES[x.dtype]
 
 
 def _rows(name, t, broadcast=False):
     """The row stride of a matrix whose rows are dense (broadcast: one row may stand for all)."""
     rows, cols = t.shape
-    if cols > 1 and t.stride(1) != 1:
+    ld, unit = t.stride()
+    if cols > 1 and unit != 1:
         raise ValueError("%s must have unit column stride, got strides %s" % (name, t.stride()))
     if rows <= 1:
         return cols
-    ld = t.stride(0)
     if ld < cols and not (broadcast and ld == 0):
         raise ValueError("%s: rows %d elements apart overlap (%d columns)" % (name, ld, cols))
     return ld
@@ -82,6 +82,8 @@ def _orders(w):
 
 def _weights(names, ws):
     """(transposed, row strides) of weights that are all (in, out) matrices or all transposed views of (out, in)."""
+    if all(w.is_contiguous() for w in ws):
+        return 0, [w.shape[1] for w in ws]
     orders = [_orders(w) for w in ws]
     for order in (0, 1):
         if all(order in o for o in orders):
@@ -134,21 +136,33 @@ def _output(out, x, rows, cols, inputs, may_be=None):
 def _workspace(size, x):
     """A call's own scratch memory, from torch's allocator on the current stream: calls on other streams and in captured
     graphs have theirs."""
-    return (None, 0) if not size else (torch.empty(size, dtype=torch.uint8, device=x.device), size)
+    return torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
 
 
-def _call(x, name, *args):
-    lib = _lib.load()
-    if torch.cuda.current_device() == x.device.index:
-        _lib.check(getattr(lib, name)(*args, _lib.stream_of(x)))
+def _p(t):
+    """Device pointer of a tensor (None -> NULL)."""
+    return None if t is None else t.data_ptr()
+
+
+def _call(x, function, *args):
+    index = x.get_device()
+    if torch._C._cuda_getDevice() == index:
+        status = function(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(x.device):
-            _lib.check(getattr(lib, name)(*args, _lib.stream_of(x)))
+        with torch.cuda.device(index):
+            status = function(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(status)
 
 
 def _recorded(*tensors):
     """Whether autograd has to see the call."""
-    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            break
+    else:
+        return False
+    if not torch.is_grad_enabled():
         return False
     _no_capture()
     return True
@@ -170,6 +184,7 @@ def dense(x, w, bias=None, activation=None, residual=None, out=None, keep=False)
     being x w + bias in x's type, or None where there is no activation."""
     dtype = _first("x", x)
     act = _activation(activation)
+    lib = _lib.load()
     rows, cin = x.shape
     if not isinstance(w, torch.Tensor) or w.dim() != 2:
         raise ValueError("w must be a (cin, cout) tensor")
@@ -187,10 +202,10 @@ def dense(x, w, bias=None, activation=None, residual=None, out=None, keep=False)
     ldr = _rows("residual", residual, broadcast=True) if residual is not None else 0
     y, ldy = _output(out, x, rows, cout, (("x", x), ("w", w), ("bias", bias)), residual)
     pre = torch.empty((rows, cout), dtype=x.dtype, device=x.device) if keep and act else None
-    ws, size = _workspace(_lib.load().fpn_dense_workspace_bytes(dtype, rows, cin, cout), x)
-    p = _lib.ptr
-    _call(x, "fpn_dense", dtype, rows, cin, cout, p(x), ldx, p(w), ldw, transposed, p(bias), act, p(residual), ldr, p(y), ldy,
-          p(pre), cout, p(ws), size)
+    size = lib.fpn_dense_workspace_bytes(dtype, rows, cin, cout)
+    ws = _workspace(size, x)
+    _call(x, lib.fpn_dense, dtype, rows, cin, cout, _p(x), ldx, _p(w), ldw, transposed, _p(bias), act, _p(residual), ldr, _p(y), ldy,
+          _p(pre), cout, _p(ws), size)
     return (y, pre) if keep else y
 
 
@@ -199,6 +214,7 @@ def dense_grad(dy, x, w, pre=None, activation=None, bias=False, need_x=True, nee
     stored as w is.  `pre` is what keep=True returned.  The residual's gradient is dy."""
     dtype = _first("x", x)
     act = _activation(activation)
+    lib = _lib.load()
     rows, cin = x.shape
     if not isinstance(w, torch.Tensor) or w.dim() != 2:
         raise ValueError("w must be a (cin, cout) tensor")
@@ -217,10 +233,10 @@ def dense_grad(dy, x, w, pre=None, activation=None, bias=False, need_x=True, nee
         dx = torch.empty((rows, cin), dtype=x.dtype, device=x.device) if need_x else None
         dw = _like_weights(w, transposed) if need_w else None
         db = torch.empty(cout, dtype=x.dtype, device=x.device) if bias else None
-    ws, size = _workspace(_lib.load().fpn_dense_grad_workspace_bytes(dtype, rows, cin, cout, act), x)
-    p = _lib.ptr
-    _call(x, "fpn_dense_grad", dtype, rows, cin, cout, p(dy), lddy, p(x), ldx, p(w), ldw, transposed, p(pre) if act else None, ldp,
-          act, p(dx), cin, p(dw), cin if transposed else cout, p(db), p(ws), size)
+    size = lib.fpn_dense_grad_workspace_bytes(dtype, rows, cin, cout, act)
+    ws = _workspace(size, x)
+    _call(x, lib.fpn_dense_grad, dtype, rows, cin, cout, _p(dy), lddy, _p(x), ldx, _p(w), ldw, transposed, _p(pre) if act else None, ldp,
+          act, _p(dx), cin, _p(dw), cin if transposed else cout, _p(db), _p(ws), size)
     return dx, dw, db
 
 
@@ -277,6 +293,7 @@ def gated(x, w_gate, w_up, bias_gate=None, bias_up=None, activation="silu", out=
     sums in x's type."""
     dtype, rows, cin, cout = _check_gated(x, w_gate, w_up)
     act = _activation(activation)
+    lib = _lib.load()
     _vector("bias_gate", bias_gate, x, cout)
     _vector("bias_up", bias_up, x, cout)
     if not keep and _recorded(x, w_gate, w_up, bias_gate, bias_up):
@@ -289,10 +306,10 @@ def gated(x, w_gate, w_up, bias_gate=None, bias_up=None, activation="silu", out=
     gate = up = None
     if keep:
         gate, up = (torch.empty((rows, cout), dtype=x.dtype, device=x.device) for _ in range(2))
-    ws, size = _workspace(_lib.load().fpn_gated_workspace_bytes(dtype, rows, cin, cout), x)
-    p = _lib.ptr
-    _call(x, "fpn_gated", dtype, rows, cin, cout, p(x), ldx, p(w_gate), ldg, p(w_up), ldu, transposed, p(bias_gate), p(bias_up), act,
-          p(h), ldh, p(gate), p(up), cout, p(ws), size)
+    size = lib.fpn_gated_workspace_bytes(dtype, rows, cin, cout)
+    ws = _workspace(size, x)
+    _call(x, lib.fpn_gated, dtype, rows, cin, cout, _p(x), ldx, _p(w_gate), ldg, _p(w_up), ldu, transposed, _p(bias_gate), _p(bias_up), act,
+          _p(h), ldh, _p(gate), _p(up), cout, _p(ws), size)
     return (h, gate, up) if keep else h
 
 
@@ -301,6 +318,7 @@ def gated_grad(dh, x, w_gate, w_up, gate, up, activation="silu", bias=False, nee
     (bias=True asks for the last two).  `gate` and `up` are what keep=True returned."""
     dtype, rows, cin, cout = _check_gated(x, w_gate, w_up)
     act = _activation(activation)
+    lib = _lib.load()
     for name, t in (("dh", dh), ("gate", gate), ("up", up)):
         _tensor(name, t, x, (rows, cout))
     lddh, ldx, ldp = _rows("dh", dh), _rows("x", x, broadcast=True), _rows("gate", gate)
@@ -311,10 +329,10 @@ def gated_grad(dh, x, w_gate, w_up, gate, up, activation="silu", bias=False, nee
         dx = torch.empty((rows, cin), dtype=x.dtype, device=x.device) if need_x else None
         dwg, dwu = (_like_weights(w_gate, transposed) for _ in range(2)) if need_w else (None, None)
         dbg, dbu = (torch.empty(cout, dtype=x.dtype, device=x.device) for _ in range(2)) if bias else (None, None)
-    ws, size = _workspace(_lib.load().fpn_gated_grad_workspace_bytes(dtype, rows, cin, cout), x)
-    p = _lib.ptr
-    _call(x, "fpn_gated_grad", dtype, rows, cin, cout, p(dh), lddh, p(x), ldx, p(w_gate), ldg, p(w_up), ldu, transposed, p(gate), p(up),
-          ldp, act, p(dx), cin, p(dwg), p(dwu), cin if transposed else cout, p(dbg), p(dbu), p(ws), size)
+    size = lib.fpn_gated_grad_workspace_bytes(dtype, rows, cin, cout)
+    ws = _workspace(size, x)
+    _call(x, lib.fpn_gated_grad, dtype, rows, cin, cout, _p(dh), lddh, _p(x), ldx, _p(w_gate), ldg, _p(w_up), ldu, transposed, _p(gate), _p(up),
+          ldp, act, _p(dx), cin, _p(dwg), _p(dwu), cin if transposed else cout, _p(dbg), _p(dbu), _p(ws), size)
     return dx, dwg, dwu, dbg, dbu
 
 
