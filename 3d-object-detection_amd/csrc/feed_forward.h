@@ -50,8 +50,13 @@ struct Args {
     long ldr;
     void *c[2];
     long ldc;
-    void *pre[2];               // pre-activations, for the backward pass (or null)
+    bool c_float;               // c is fp32 whatever the operands' type
+    float *pre[2];              // pre-activations, for the backward pass (or null)
     long ldp;
+    // the gated block's backward epilogue (or null): the sums are dh, from which dg = dh up act'(gate) and du = dh act(gate)
+    // go to c[0] and c[1]; `sums` (or null): their column sums, one row of (2, n) per 32 TM output rows
+    const float *gate, *up;
+    float *sums;
     float *partial;             // split k: (batch, splits, 1 or 2, m, n) sums, joined by join_kernel
     int splits;
     long tiles_per_split;       // k tiles
@@ -234,10 +239,9 @@ __device__ inline void finish8(const Args &p, int member, long m, int n, float (
         for (int i = 0; i < 8; ++i) v2[i] += w[i];
     }
     if (p.pre[0]) {
-        // rounded to the operands' type: the backward pass rounds dpre to that type for its products anyway, and the
-        // two pre-activations are the largest tensors that a training step keeps
-        store8(reinterpret_cast<T *>(p.pre[0]) + m * p.ldp + n, left, v);
-        if (GATED) store8(reinterpret_cast<T *>(p.pre[1]) + m * p.ldp + n, left, v2);
+        // kept in fp32: rounded to 16 bits, gate and up would double the error of dx and dw
+        store8(p.pre[0] + m * p.ldp + n, left, v);
+        if (GATED) store8(p.pre[1] + m * p.ldp + n, left, v2);
     }
     if (p.act != FPN_ACT_NONE)
         for_activation(p.act, [&](auto tag) {
@@ -253,7 +257,8 @@ __device__ inline void finish8(const Args &p, int member, long m, int n, float (
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] += w[i];
     }
-    store8(reinterpret_cast<T *>(p.c[member]) + m * p.ldc + n, left, v);
+    if (p.c_float) store8(reinterpret_cast<float *>(p.c[member]) + m * p.ldc + n, left, v);
+    else store8(reinterpret_cast<T *>(p.c[member]) + m * p.ldc + n, left, v);
 }
 
 // ---- tiles ------------------------------------------------------------------------------------------------------

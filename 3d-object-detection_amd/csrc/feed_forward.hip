@@ -16,9 +16,9 @@ namespace {
 struct GradArgs {
     long rows;
     int n;
-    const void *dy;
+    const void *dy;          // of the kernel's DY type
     long lddy;
-    const void *pre[2];      // null where the activation is the identity
+    const float *pre[2];     // null where the activation is the identity
     long ldp;
     int act;
     void *d[2];              // (rows, n) dense, or null: column sums only
@@ -26,7 +26,7 @@ struct GradArgs {
     long rows_per_block;
 };
 
-template <class T, bool GATED> __global__ __launch_bounds__(kThreads) void grad_kernel(const GradArgs p)
+template <class T, class DY, bool GATED> __global__ __launch_bounds__(kThreads) void grad_kernel(const GradArgs p)
 {
     constexpr bool EXACT = sizeof(T) == 4;
     __shared__ float part[8][32][8];
@@ -40,9 +40,9 @@ template <class T, bool GATED> __global__ __launch_bounds__(kThreads) void grad_
             constexpr int ACT = decltype(tag)::value;
             for (long m = m0 + r; m < m1; m += 8) {
                 float d[8], g[8], u[8], du[8];
-                load8(reinterpret_cast<const T *>(p.dy) + m * p.lddy + n, left, d);
-                if (GATED || ACT != FPN_ACT_NONE) load8(reinterpret_cast<const T *>(p.pre[0]) + m * p.ldp + n, left, g);
-                if (GATED) load8(reinterpret_cast<const T *>(p.pre[1]) + m * p.ldp + n, left, u);
+                load8(reinterpret_cast<const DY *>(p.dy) + m * p.lddy + n, left, d);
+                if (GATED || ACT != FPN_ACT_NONE) load8(p.pre[0] + m * p.ldp + n, left, g);
+                if (GATED) load8(p.pre[1] + m * p.ldp + n, left, u);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     float value = 0.f;
@@ -107,17 +107,24 @@ int grad_rows_grid(long rows, int n)
 }
 
 template <class T>
-int launch_grad(GradArgs p, bool gated, void *const (&sums_out)[2], hipStream_t stream)
+int launch_column_join(int n, int blocks, bool gated, const float *sums, void *const (&sums_out)[2], hipStream_t stream)
+{
+    hipLaunchKernelGGL((column_join_kernel<T>), dim3((n + 31) / 32, gated ? 2 : 1), dim3(kThreads), 0, stream, n, blocks, gated ? 2 : 1,
+                       sums, reinterpret_cast<T *>(sums_out[0]), reinterpret_cast<T *>(sums_out[1]));
+    return check_launch("bias gradient");
+}
+
+template <class T>
+int launch_grad(GradArgs p, bool gated, bool dy_float, void *const (&sums_out)[2], hipStream_t stream)
 {
     const int gy = grad_rows_grid(p.rows, p.n), gx = (p.n + 255) / 256;
     p.rows_per_block = (p.rows + gy - 1) / gy;
-    if (gated) hipLaunchKernelGGL((grad_kernel<T, true>), dim3(gx, gy), dim3(kThreads), 0, stream, p);
-    else hipLaunchKernelGGL((grad_kernel<T, false>), dim3(gx, gy), dim3(kThreads), 0, stream, p);
+    if (gated && dy_float) hipLaunchKernelGGL((grad_kernel<T, float, true>), dim3(gx, gy), dim3(kThreads), 0, stream, p);
+    else if (gated) hipLaunchKernelGGL((grad_kernel<T, T, true>), dim3(gx, gy), dim3(kThreads), 0, stream, p);
+    else hipLaunchKernelGGL((grad_kernel<T, T, false>), dim3(gx, gy), dim3(kThreads), 0, stream, p);
     int rc = check_launch("feed-forward gradient");
     if (rc != FPN_OK || !p.sums) return rc;
-    hipLaunchKernelGGL((column_join_kernel<T>), dim3((p.n + 31) / 32, gated ? 2 : 1), dim3(kThreads), 0, stream, p.n, gy, gated ? 2 : 1,
-                       p.sums, reinterpret_cast<T *>(sums_out[0]), reinterpret_cast<T *>(sums_out[1]));
-    return check_launch("bias gradient");
+    return launch_column_join<T>(p.n, gy, gated, p.sums, sums_out, stream);
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------
@@ -137,14 +144,19 @@ size_t partial_bytes(int dtype, long m, int n, long k, int segs, int batch, bool
 
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
-int run_product(int dtype, const Args &p, int order_a, int order_b, bool gated, float *partial, size_t partial_bytes, hipStream_t stream)
+Plan plan_of(int dtype, const Args &p, int order_a, int order_b, bool gated)
 {
     bool aligned = true;
     for (int i = 0; i < p.segs; ++i)
         aligned = aligned && whole_chunks(p.a[i], order_a == kInner && p.m == 1 ? 0 : p.lda[i], order_a, p.m, element_size(dtype));
     for (int i = 0; i < std::max({p.segs, p.batch, gated ? 2 : 1}); ++i)
         aligned = aligned && whole_chunks(p.b[i], p.ldb[i], order_b, p.n, element_size(dtype));
-    const Plan plan = plan_product(dtype, p.m, p.n, p.k, p.segs, p.batch, gated, aligned, order_a, order_b);
+    return plan_product(dtype, p.m, p.n, p.k, p.segs, p.batch, gated, aligned, order_a, order_b);
+}
+
+int run_product(int dtype, const Args &p, int order_a, int order_b, bool gated, float *partial, size_t partial_bytes, hipStream_t stream)
+{
+    const Plan plan = plan_of(dtype, p, order_a, order_b, gated);
     if (plan.partial_bytes && (!partial || plan.partial_bytes > partial_bytes))
         return fail(FPN_E_INVALID_ARG, "workspace of %zu bytes needed for partial sums, got %zu", plan.partial_bytes, partial ? partial_bytes : 0);
     if (dtype == FPN_F32) return launch_product<float>(p, order_a, order_b, gated, plan, partial, stream);
@@ -195,18 +207,21 @@ int check_workspace(const void *ws, size_t have, size_t need)
 // The parts of a backward pass' workspace: dpre (one matrix, or two where gated), the workgroups' column sums, and
 // the partial sums of dx and dw, which run one after the other
 struct GradSpace {
-    size_t d, sums, partial, total;
+    size_t d, sums, dh, partial, total;
 };
-GradSpace grad_space(int dtype, long rows, int cin, int n, bool gated, bool with_d)
+// (down: the width of the block's result where dh is formed from its gradient, else 0)
+GradSpace grad_space(int dtype, long rows, int cin, int n, bool gated, bool with_d, int down = 0)
 {
     GradSpace s;
     const int planes = gated ? 2 : 1;
     s.d = with_d ? align256((size_t)rows * n * element_size(dtype)) * planes : 0;
-    s.sums = align256((size_t)grad_rows_grid(rows, n) * planes * n * sizeof(float));
+    s.sums = align256((size_t)std::max<long>(grad_rows_grid(rows, n), down ? (rows + 255) / 256 * 8 : 0) * planes * n * sizeof(float));
+    s.dh = down ? align256((size_t)rows * n * sizeof(float)) : 0;
     s.partial = align256(std::max({partial_bytes(dtype, rows, cin, n, planes, 1, false, kInner),
                                    partial_bytes(dtype, cin, n, rows, 1, planes, false, kOuter),
                                    partial_bytes(dtype, n, cin, rows, 1, 1, false, kOuter)}));
-    s.total = s.d + s.sums + s.partial;
+    if (down) s.partial = std::max(s.partial, align256(partial_bytes(dtype, rows, n, down, 1, 1, false, kInner)));
+    s.total = s.d + s.sums + s.dh + s.partial;
     return s;
 }
 
@@ -249,11 +264,18 @@ int weight_gradients(int dtype, long rows, int cin, int n, const void *x, long l
     return FPN_OK;
 }
 
-int run_grad(int dtype, const GradArgs &p, bool gated, void *const (&sums_out)[2], hipStream_t stream)
+int run_grad(int dtype, const GradArgs &p, bool gated, bool dy_float, void *const (&sums_out)[2], hipStream_t stream)
 {
-    if (dtype == FPN_F32) return launch_grad<float>(p, gated, sums_out, stream);
-    if (dtype == FPN_BF16) return launch_grad<__bf16>(p, gated, sums_out, stream);
-    return launch_grad<_Float16>(p, gated, sums_out, stream);
+    if (dtype == FPN_F32) return launch_grad<float>(p, gated, dy_float, sums_out, stream);
+    if (dtype == FPN_BF16) return launch_grad<__bf16>(p, gated, dy_float, sums_out, stream);
+    return launch_grad<_Float16>(p, gated, dy_float, sums_out, stream);
+}
+
+int run_column_join(int dtype, int n, int blocks, const float *sums, void *const (&out)[2], hipStream_t stream)
+{
+    if (dtype == FPN_F32) return launch_column_join<float>(n, blocks, true, sums, out, stream);
+    if (dtype == FPN_BF16) return launch_column_join<__bf16>(n, blocks, true, sums, out, stream);
+    return launch_column_join<_Float16>(n, blocks, true, sums, out, stream);
 }
 
 }  // namespace
@@ -378,7 +400,7 @@ size_t fpn_dense_workspace_bytes(int dtype, long rows, int cin, int cout)
 }
 
 int fpn_dense(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w, long ldw, int w_transposed,
-              const void *bias, int activation, const void *residual, long ldr, void *y, long ldy, void *pre, long ldp,
+              const void *bias, int activation, const void *residual, long ldr, void *y, long ldy, float *pre, long ldp,
               void *workspace, size_t workspace_bytes, void *stream)
 {
     FPN_FF_TRY(check_common(dtype, rows, cin, cout, activation));
@@ -388,7 +410,7 @@ int fpn_dense(int dtype, long rows, int cin, int cout, const void *x, long ldx, 
     FPN_FF_TRY(check_matrix("y", y, ldy, cout, dtype));
     FPN_FF_TRY(check_vector("bias", bias, dtype));
     if (residual) FPN_FF_TRY(check_matrix("residual", residual, ldr, cout, dtype, true));
-    if (pre) FPN_FF_TRY(check_matrix("pre", pre, ldp, cout, dtype));
+    if (pre) FPN_FF_TRY(check_matrix("pre", pre, ldp, cout, FPN_F32));
     FPN_FF_TRY(check_workspace(workspace, workspace_bytes, 0));
     Args p = product(rows, cout, cin);
     p.a[0] = x;
@@ -414,14 +436,14 @@ size_t fpn_dense_grad_workspace_bytes(int dtype, long rows, int cin, int cout, i
 }
 
 int fpn_dense_grad(int dtype, long rows, int cin, int cout, const void *dy, long lddy, const void *x, long ldx, const void *w,
-                   long ldw, int w_transposed, const void *pre, long ldp, int activation, void *dx, long lddx, void *dw, long lddw,
+                   long ldw, int w_transposed, const float *pre, long ldp, int activation, void *dx, long lddx, void *dw, long lddw,
                    void *dbias, void *workspace, size_t workspace_bytes, void *stream)
 {
     FPN_FF_TRY(check_common(dtype, rows, cin, cout, activation));
     const bool act = activation != FPN_ACT_NONE;
     if (rows > 0) {
         FPN_FF_TRY(check_matrix("dy", dy, lddy, cout, dtype));
-        if (act) FPN_FF_TRY(check_matrix("pre", pre, ldp, cout, dtype));
+        if (act) FPN_FF_TRY(check_matrix("pre", pre, ldp, cout, FPN_F32));
         if (dw) FPN_FF_TRY(check_matrix("x", x, ldx, cin, dtype, true));
         if (dx) FPN_FF_TRY(check_matrix("w", w, ldw, w_transposed ? cin : cout, dtype));
         if (dx) FPN_FF_TRY(check_matrix("dx", dx, lddx, cin, dtype));
@@ -431,7 +453,7 @@ int fpn_dense_grad(int dtype, long rows, int cin, int cout, const void *dy, long
     const GradSpace space = grad_space(dtype, rows, cin, cout, false, act);
     FPN_FF_TRY(check_workspace(workspace, workspace_bytes, space.total));
     char *ws = reinterpret_cast<char *>(workspace);
-    float *partial = reinterpret_cast<float *>(ws + space.d + space.sums);
+    float *partial = reinterpret_cast<float *>(ws + space.d + space.sums + space.dh);
     const hipStream_t st = as_stream(stream);
 
     const void *d[2] = {dy, nullptr};
@@ -452,7 +474,7 @@ int fpn_dense_grad(int dtype, long rows, int cin, int cout, const void *dy, long
         }
         g.sums = dbias ? reinterpret_cast<float *>(ws + space.d) : nullptr;
         void *const out[2] = {dbias, nullptr};
-        FPN_FF_TRY(run_grad(dtype, g, false, out, st));
+        FPN_FF_TRY(run_grad(dtype, g, false, false, out, st));
     }
     if (dx && rows > 0) {
         Args p = product(rows, cin, cout);
@@ -478,7 +500,7 @@ size_t fpn_gated_workspace_bytes(int dtype, long rows, int cin, int cout)
 }
 
 int fpn_gated(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w_gate, long ldg, const void *w_up, long ldu,
-              int w_transposed, const void *bias_gate, const void *bias_up, int activation, void *h, long ldh, void *gate, void *up,
+              int w_transposed, const void *bias_gate, const void *bias_up, int activation, void *h, long ldh, float *gate, float *up,
               long ldp, void *workspace, size_t workspace_bytes, void *stream)
 {
     FPN_FF_TRY(check_common(dtype, rows, cin, cout, activation));
@@ -490,8 +512,8 @@ int fpn_gated(int dtype, long rows, int cin, int cout, const void *x, long ldx, 
     FPN_FF_TRY(check_matrix("h", h, ldh, cout, dtype));
     FPN_FF_TRY(check_vector("bias_gate", bias_gate, dtype));
     FPN_FF_TRY(check_vector("bias_up", bias_up, dtype));
-    if (gate) FPN_FF_TRY(check_matrix("gate", gate, ldp, cout, dtype));
-    if (up) FPN_FF_TRY(check_matrix("up", up, ldp, cout, dtype));
+    if (gate) FPN_FF_TRY(check_matrix("gate", gate, ldp, cout, FPN_F32));
+    if (up) FPN_FF_TRY(check_matrix("up", up, ldp, cout, FPN_F32));
     FPN_FF_TRY(check_workspace(workspace, workspace_bytes, 0));
     Args p = product(rows, cout, cin);
     p.a[0] = x;
@@ -512,23 +534,26 @@ int fpn_gated(int dtype, long rows, int cin, int cout, const void *x, long ldx, 
                        as_stream(stream));
 }
 
-size_t fpn_gated_grad_workspace_bytes(int dtype, long rows, int cin, int cout)
+size_t fpn_gated_grad_workspace_bytes(int dtype, long rows, int cin, int cout, int cdown)
 {
-    if (check_common(dtype, rows, cin, cout, FPN_ACT_NONE) != FPN_OK) return 0;
-    return grad_space(dtype, rows, cin, cout, true, true).total;
+    if (check_common(dtype, rows, cin, cout, FPN_ACT_NONE) != FPN_OK || cdown < 0 || cdown > kMostLd) return 0;
+    return grad_space(dtype, rows, cin, cout, true, true, cdown).total;
 }
 
-int fpn_gated_grad(int dtype, long rows, int cin, int cout, const void *dh, long lddh, const void *x, long ldx, const void *w_gate,
-                   long ldg, const void *w_up, long ldu, int w_transposed, const void *gate, const void *up, long ldp, int activation,
-                   void *dx, long lddx, void *dw_gate, void *dw_up, long lddw, void *dbias_gate, void *dbias_up, void *workspace,
-                   size_t workspace_bytes, void *stream)
+int fpn_gated_grad(int dtype, long rows, int cin, int cout, int cdown, const void *dh, long lddh, const void *w_down, long ldd,
+                   int down_transposed, const void *x, long ldx, const void *w_gate, long ldg, const void *w_up, long ldu,
+                   int w_transposed, const float *gate, const float *up, long ldp, int activation, void *dx, long lddx, void *dw_gate,
+                   void *dw_up, long lddw, void *dbias_gate, void *dbias_up, void *workspace, size_t workspace_bytes, void *stream)
 {
     FPN_FF_TRY(check_common(dtype, rows, cin, cout, activation));
+    FPN_REQUIRE(cdown >= 0, "cdown %d is negative", cdown);
+    if (cdown > kMostLd) return fail(FPN_E_UNSUPPORTED, "widths up to %ld are supported, got %d", kMostLd, cdown);
     FPN_REQUIRE(!dw_gate == !dw_up && !dbias_gate == !dbias_up, "the gradients of gate and up are wanted together or not at all");
     if (rows > 0) {
-        FPN_FF_TRY(check_matrix("dh", dh, lddh, cout, dtype));
-        FPN_FF_TRY(check_matrix("gate", gate, ldp, cout, dtype));
-        FPN_FF_TRY(check_matrix("up", up, ldp, cout, dtype));
+        FPN_FF_TRY(check_matrix("dh", dh, lddh, cdown ? cdown : cout, dtype));
+        if (cdown) FPN_FF_TRY(check_matrix("w_down", w_down, ldd, down_transposed ? cout : cdown, dtype));
+        FPN_FF_TRY(check_matrix("gate", gate, ldp, cout, FPN_F32));
+        FPN_FF_TRY(check_matrix("up", up, ldp, cout, FPN_F32));
         if (dw_gate) FPN_FF_TRY(check_matrix("x", x, ldx, cin, dtype, true));
         if (dx) {
             FPN_FF_TRY(check_matrix("w_gate", w_gate, ldg, w_transposed ? cin : cout, dtype));
@@ -542,10 +567,10 @@ int fpn_gated_grad(int dtype, long rows, int cin, int cout, const void *dh, long
     }
     FPN_FF_TRY(check_vector("dbias_gate", dbias_gate, dtype));
     FPN_FF_TRY(check_vector("dbias_up", dbias_up, dtype));
-    const GradSpace space = grad_space(dtype, rows, cin, cout, true, true);
+    const GradSpace space = grad_space(dtype, rows, cin, cout, true, true, cdown);
     FPN_FF_TRY(check_workspace(workspace, workspace_bytes, space.total));
     char *ws = reinterpret_cast<char *>(workspace);
-    float *partial = reinterpret_cast<float *>(ws + space.d + space.sums);
+    float *partial = reinterpret_cast<float *>(ws + space.d + space.sums + space.dh);
     const hipStream_t st = as_stream(stream);
 
     GradArgs g = {};
@@ -561,7 +586,39 @@ int fpn_gated_grad(int dtype, long rows, int cin, int cout, const void *dh, long
     g.d[1] = ws + space.d / 2;
     g.sums = dbias_gate ? reinterpret_cast<float *>(ws + space.d) : nullptr;
     void *const sums_out[2] = {dbias_gate, dbias_up};
-    FPN_FF_TRY(run_grad(dtype, g, true, sums_out, st));
+    bool done = false;
+    if (cdown && rows > 0) {                      // dh = dy w_down^T, never rounded to 16 bits
+        const int order_b = down_transposed ? kOuter : kInner;
+        Args p = product(rows, cout, cdown);
+        p.a[0] = dh;
+        p.lda[0] = lddh;
+        p.b[0] = w_down;
+        p.ldb[0] = ldd;
+        const Plan plan = plan_of(dtype, p, kInner, order_b, false);
+        done = plan.wide && plan.splits == 1;
+        if (done) {                               // dg and du straight from the product's epilogue
+            p.c[0] = g.d[0];
+            p.c[1] = g.d[1];
+            p.ldc = cout;
+            p.act = activation;
+            p.gate = gate;
+            p.up = up;
+            p.ldp = ldp;
+            p.sums = g.sums;
+        } else {
+            p.c[0] = ws + space.d + space.sums;
+            p.ldc = cout;
+            p.c_float = true;
+            g.dy = p.c[0];
+            g.lddy = cout;
+        }
+        FPN_FF_TRY(run_product(dtype, p, kInner, order_b, false, partial, space.partial, st));
+        if (done && g.sums) {
+            const int rows_each = plan.bm == 256 ? 128 : 32;       // (of a wave: 32 TM)
+            FPN_FF_TRY(run_column_join(dtype, cout, (int)((rows + plan.bm - 1) / plan.bm * (plan.bm / rows_each)), g.sums, sums_out, st));
+        }
+    }
+    if (!done) FPN_FF_TRY(run_grad(dtype, g, true, cdown && rows > 0, sums_out, st));
     if (dx && rows > 0) {                         // dg Wg^T + du Wu^T: one sum over both
         Args p = product(rows, cin, cout);
         p.segs = 2;

@@ -140,13 +140,14 @@ template <class T, bool GATED> __device__ inline void finish1(const Args &p, lon
     if (p.bias[0]) v += (float)reinterpret_cast<const T *>(p.bias[0])[n];
     if (GATED && p.bias[1]) v2 += (float)reinterpret_cast<const T *>(p.bias[1])[n];
     if (p.pre[0]) {
-        reinterpret_cast<T *>(p.pre[0])[m * p.ldp + n] = (T)v;
-        if (GATED) reinterpret_cast<T *>(p.pre[1])[m * p.ldp + n] = (T)v2;
+        p.pre[0][m * p.ldp + n] = v;
+        if (GATED) p.pre[1][m * p.ldp + n] = v2;
     }
     if (p.act != FPN_ACT_NONE) for_activation(p.act, [&](auto tag) { v = activate<decltype(tag)::value, EXACT>(v); });
     if (GATED) v *= v2;
     if (p.residual) v += (float)reinterpret_cast<const T *>(p.residual)[m * p.ldr + n];
-    reinterpret_cast<T *>(p.c[0])[m * p.ldc + n] = (T)v;
+    if (p.c_float) reinterpret_cast<float *>(p.c[0])[m * p.ldc + n] = v;
+    else reinterpret_cast<T *>(p.c[0])[m * p.ldc + n] = (T)v;
 }
 
 template <class T, int ORDER_B, int MT, int NT, bool GATED>

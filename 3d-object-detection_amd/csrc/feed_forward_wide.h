@@ -164,13 +164,16 @@ template <class T, int ORDER, int R, int TILES> struct StreamReader {
 // consecutive columns of one row), read back as runs of eight columns of consecutive rows - whole lines for the
 // loads and stores, one copy of the epilogue's arithmetic, bias loaded once.  `lds` is the wave's:
 // kEpilogueBytes; nobody else uses it.
-template <class T, bool GATED, class S>
+// MODE: a plain product, a gated one, or the gated block's backward epilogue on a plain one
+enum { kPlainMode = 0, kGatedMode = 1, kGateGradMode = 2 };
+
+template <class T, int MODE, class S>
 __device__ inline void store_piece(const Args &p, const floatx16 (&acc)[S::TM][S::TN], char *lds, int member, int split, long m0, int n0, int lane)
 {
-    constexpr bool EXACT = sizeof(T) == 4;
+    constexpr bool EXACT = sizeof(T) == 4, GATED = MODE == kGatedMode;
     constexpr int kTN = S::TN, kEpilogueRow = S::kEpilogueRow;
     const int l31 = lane & 31, h = lane >> 5;
-    constexpr int kRuns = GATED ? 2 * kTN : 4 * kTN, kRowsAtOnce = 64 / kRuns, kBatch = 2;     // runs of eight columns per row
+    constexpr int kRuns = GATED ? 2 * kTN : 4 * kTN, kRowsAtOnce = 64 / kRuns, kBatch = MODE == kGateGradMode ? 1 : 2;     // runs of eight columns per row
     const int run = lane % kRuns, row0 = lane / kRuns;
     const int n = n0 + run * 8;
     const long left = p.n - n;
@@ -186,7 +189,7 @@ __device__ inline void store_piece(const Args &p, const floatx16 (&acc)[S::TM][S
             }
     };
     float bias[8] = {}, bias2[8] = {};
-    if (left > 0 && p.bias[GATED ? 0 : member]) load8(reinterpret_cast<const T *>(p.bias[GATED ? 0 : member]) + n, left, bias);
+    if (MODE != kGateGradMode && left > 0 && p.bias[GATED ? 0 : member]) load8(reinterpret_cast<const T *>(p.bias[GATED ? 0 : member]) + n, left, bias);
     if (GATED && left > 0 && p.bias[1]) load8(reinterpret_cast<const T *>(p.bias[1]) + n, left, bias2);
 #pragma unroll 1
     for (int i = 0; i < S::TM; ++i) {
@@ -201,7 +204,7 @@ __device__ inline void store_piece(const Args &p, const floatx16 (&acc)[S::TM][S
         for (int r = row0; r < 32; r += kRowsAtOnce * kBatch) {
             const long m = m0 + 32 * i + r;
             float v[kBatch][8], v2[GATED ? kBatch : 1][8], res[kBatch][8];
-            if (p.residual)
+            if (MODE != kGateGradMode && p.residual)
 #pragma unroll
                 for (int b = 0; b < kBatch; ++b)
                     load8(reinterpret_cast<const T *>(p.residual) + min(m + b * kRowsAtOnce, p.m - 1) * p.ldr + n, left, res[b]);
@@ -213,6 +216,40 @@ __device__ inline void store_piece(const Args &p, const floatx16 (&acc)[S::TM][S
                     v[b][e] = from[e];
                     if (GATED) v2[b][e] = from[16 * kTN + e];
                 }
+            }
+            if constexpr (MODE == kGateGradMode) {
+                // the gated block's backward pass: dh in, dg and du out (no bias in such a product: its registers
+                // take the column sums)
+                float g[kBatch][8], u[kBatch][8];
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b) {
+                    const long row = min(m + b * kRowsAtOnce, p.m - 1);
+                    load8(p.gate + row * p.ldp + n, left, g[b]);
+                    load8(p.up + row * p.ldp + n, left, u[b]);
+                }
+                for_activation(p.act, [&](auto tag) {
+#pragma unroll
+                    for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            float value;
+                            const float slope = activate_grad<decltype(tag)::value, EXACT>(g[b][e], value);
+                            g[b][e] = v[b][e] * u[b][e] * slope;
+                            u[b][e] = v[b][e] * value;
+                        }
+                });
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b)
+                    if (m + b * kRowsAtOnce < p.m) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            bias[e] += g[b][e];
+                            bias2[e] += u[b][e];
+                        }
+                        store8(reinterpret_cast<T *>(p.c[0]) + (m + b * kRowsAtOnce) * p.ldc + n, left, g[b]);
+                        store8(reinterpret_cast<T *>(p.c[1]) + (m + b * kRowsAtOnce) * p.ldc + n, left, u[b]);
+                    }
+                continue;
             }
             if (p.partial) {
 #pragma unroll
@@ -235,8 +272,8 @@ __device__ inline void store_piece(const Args &p, const floatx16 (&acc)[S::TM][S
 #pragma unroll
                 for (int b = 0; b < kBatch; ++b)
                     if (m + b * kRowsAtOnce < p.m) {
-                        store8(reinterpret_cast<T *>(p.pre[0]) + (m + b * kRowsAtOnce) * p.ldp + n, left, v[b]);
-                        if (GATED) store8(reinterpret_cast<T *>(p.pre[1]) + (m + b * kRowsAtOnce) * p.ldp + n, left, v2[b]);
+                        store8(p.pre[0] + (m + b * kRowsAtOnce) * p.ldp + n, left, v[b]);
+                        if (GATED) store8(p.pre[1] + (m + b * kRowsAtOnce) * p.ldp + n, left, v2[b]);
                     }
             if (p.act != FPN_ACT_NONE)
                 for_activation(p.act, [&](auto tag) {
@@ -252,16 +289,36 @@ __device__ inline void store_piece(const Args &p, const floatx16 (&acc)[S::TM][S
                     if (GATED) v[b][e] *= v2[b][e];
                     if (p.residual) v[b][e] += res[b][e];
                 }
-                if (m + b * kRowsAtOnce < p.m) store8(reinterpret_cast<T *>(p.c[member]) + (m + b * kRowsAtOnce) * p.ldc + n, left, v[b]);
+                if (m + b * kRowsAtOnce < p.m) {
+                    if (p.c_float) store8(reinterpret_cast<float *>(p.c[member]) + (m + b * kRowsAtOnce) * p.ldc + n, left, v[b]);
+                    else store8(reinterpret_cast<T *>(p.c[member]) + (m + b * kRowsAtOnce) * p.ldc + n, left, v[b]);
+                }
             }
+        }
+    }
+    if constexpr (MODE == kGateGradMode) {
+        if (!p.sums) return;
+        // the column sums of this wave's rows: the lanes of one run of columns, in a fixed order
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int far = kRuns; far < 64; far *= 2) {
+                bias[e] += __shfl_xor(bias[e], far);
+                bias2[e] += __shfl_xor(bias2[e], far);
+            }
+        if (row0 == 0 && left > 0) {
+            float *to = p.sums + m0 / (32 * S::TM) * 2 * p.n + n;
+            store8(to, left, bias);
+            store8(to + p.n, left, bias2);
         }
     }
 }
 
-template <class T, int ORDER_A, int ORDER_B, bool GATED, class S>
+template <class T, int ORDER_A, int ORDER_B, int MODE, class S>
 __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void wide_product_kernel(const Args p)
 {
     extern __shared__ char lds[];
+    constexpr bool GATED = MODE == kGatedMode;
     constexpr int kWaves = S::kWaves, kStages = S::kStages, kStage = S::kStage, kTM = S::TM, kTN = S::TN, BM = S::BM;
     constexpr int kHalves = GATED ? 2 : 1, kCols = S::BN / kHalves, kABytes = BM * kWideK * 2, kHalfBytes = kCols * kWideK * 2;
     // (where a half of b is less than a request per wave, half of the waves request each)
@@ -420,7 +477,7 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void wide_product_kernel(
         }
         __syncthreads();
     }
-    store_piece<T, GATED, S>(p, acc, lds + wave * S::kEpilogueBytes, at.member, at.split, m0 + wm * 32 * kTM,
+    store_piece<T, MODE, S>(p, acc, lds + wave * S::kEpilogueBytes, at.member, at.split, m0 + wm * 32 * kTM,
                              n0 + wn * 32 * (GATED ? kTN / 2 : kTN), lane);
 }
 
@@ -435,14 +492,17 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void wide_product_kernel(
 template <class T, class S> int launch_shape(const Args &p, int order_a, int order_b, bool gated, long blocks, hipStream_t stream)
 {
     if (gated) {
-        if (order_b == kOuter) FPN_FF_WIDE(kInner, kOuter, true);
-        else FPN_FF_WIDE(kInner, kInner, true);
+        if (order_b == kOuter) FPN_FF_WIDE(kInner, kOuter, kGatedMode);
+        else FPN_FF_WIDE(kInner, kInner, kGatedMode);
+    } else if (p.gate) {
+        if (order_b == kOuter) FPN_FF_WIDE(kInner, kOuter, kGateGradMode);
+        else FPN_FF_WIDE(kInner, kInner, kGateGradMode);
     } else if (order_a == kOuter) {
-        FPN_FF_WIDE(kOuter, kOuter, false);
+        FPN_FF_WIDE(kOuter, kOuter, kPlainMode);
     } else if (order_b == kOuter) {
-        FPN_FF_WIDE(kInner, kOuter, false);
+        FPN_FF_WIDE(kInner, kOuter, kPlainMode);
     } else {
-        FPN_FF_WIDE(kInner, kInner, false);
+        FPN_FF_WIDE(kInner, kInner, kPlainMode);
     }
     return check_launch("feed-forward product, wide");
 }

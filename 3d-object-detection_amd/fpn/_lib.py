@@ -91,8 +91,8 @@ SIGNATURES = {
     "fpn_dense": [_i, _l, _i, _i, _vp, _l, _vp, _l, _i, _vp, _i, _vp, _l, _vp, _l, _vp, _l, _vp, _sz, _vp],
     "fpn_dense_grad": [_i, _l, _i, _i, _vp, _l, _vp, _l, _vp, _l, _i, _vp, _l, _i, _vp, _l, _vp, _l, _vp, _vp, _sz, _vp],
     "fpn_gated": [_i, _l, _i, _i, _vp, _l, _vp, _l, _vp, _l, _i, _vp, _vp, _i, _vp, _l, _vp, _vp, _l, _vp, _sz, _vp],
-    "fpn_gated_grad": [_i, _l, _i, _i, _vp, _l, _vp, _l, _vp, _l, _vp, _l, _i, _vp, _vp, _l, _i, _vp, _l, _vp, _vp, _l, _vp, _vp,
-                       _vp, _sz, _vp],
+    "fpn_gated_grad": [_i, _l, _i, _i, _i, _vp, _l, _vp, _l, _i, _vp, _l, _vp, _l, _vp, _l, _i, _vp, _vp, _l, _i, _vp, _l, _vp, _vp,
+                       _l, _vp, _vp, _vp, _sz, _vp],
     "fpn_mask_gather": [_i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
 }
 
@@ -102,7 +102,7 @@ SIZES = {
     "fpn_dense_workspace_bytes": [_i, _l, _i, _i],
     "fpn_dense_grad_workspace_bytes": [_i, _l, _i, _i, _i],
     "fpn_gated_workspace_bytes": [_i, _l, _i, _i],
-    "fpn_gated_grad_workspace_bytes": [_i, _l, _i, _i],
+    "fpn_gated_grad_workspace_bytes": [_i, _l, _i, _i, _i],
 }
 
 _lib = None

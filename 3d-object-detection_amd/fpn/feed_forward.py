@@ -181,7 +181,8 @@ def dense(x, w, bias=None, activation=None, residual=None, out=None, keep=False)
 
     activation: None, "relu", "silu", "sigmoid", "gelu" (exact) or "gelu_tanh".  `out` receives y (it may be the
     residual itself, but share memory with no other argument).  keep=True returns (y, pre) for `dense_grad`, pre
-    being x w + bias in x's type, or None where there is no activation."""
+    being x w + bias in float32 (rounded further it would cost the gradients digits), or None where there is no
+    activation."""
     dtype = _first("x", x)
     act = _activation(activation)
     lib = _lib.load()
@@ -201,7 +202,7 @@ def dense(x, w, bias=None, activation=None, residual=None, out=None, keep=False)
     transposed, (ldw,) = _weights(("w",), (w,))
     ldr = _rows("residual", residual, broadcast=True) if residual is not None else 0
     y, ldy = _output(out, x, rows, cout, (("x", x), ("w", w), ("bias", bias)), residual)
-    pre = torch.empty((rows, cout), dtype=x.dtype, device=x.device) if keep and act else None
+    pre = torch.empty((rows, cout), dtype=torch.float32, device=x.device) if keep and act else None
     size = lib.fpn_dense_workspace_bytes(dtype, rows, cin, cout)
     ws = _workspace(size, x)
     _call(x, lib.fpn_dense, dtype, rows, cin, cout, _p(x), ldx, _p(w), ldw, transposed, _p(bias), act, _p(residual), ldr, _p(y), ldy,
@@ -227,8 +228,7 @@ def dense_grad(dy, x, w, pre=None, activation=None, bias=False, need_x=True, nee
     if act:
         if pre is None:
             raise ValueError("pre (from dense(..., keep=True)) is needed where there is an activation")
-        _tensor("pre", pre, x, (rows, cout))
-        ldp = _rows("pre", pre)
+        ldp = _kept("pre", pre, x, (rows, cout))
     with torch.no_grad():
         dx = torch.empty((rows, cin), dtype=x.dtype, device=x.device) if need_x else None
         dw = _like_weights(w, transposed) if need_w else None
@@ -238,6 +238,13 @@ def dense_grad(dy, x, w, pre=None, activation=None, bias=False, need_x=True, nee
     _call(x, lib.fpn_dense_grad, dtype, rows, cin, cout, _p(dy), lddy, _p(x), ldx, _p(w), ldw, transposed, _p(pre) if act else None, ldp,
           act, _p(dx), cin, _p(dw), cin if transposed else cout, _p(db), _p(ws), size)
     return dx, dw, db
+
+
+def _kept(name, t, x, shape):
+    """The row stride of a pre-activation that a forward pass kept."""
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or not t.is_cuda or t.get_device() != x.get_device() or t.shape != shape:
+        raise ValueError("%s must be the float32 %s tensor on %s that keep=True returned" % (name, tuple(shape), x.device))
+    return _rows(name, t)
 
 
 def _like_weights(w, transposed):
@@ -290,7 +297,7 @@ def gated(x, w_gate, w_up, bias_gate=None, bias_up=None, activation="silu", out=
     same way round, columns of one matrix will do -, biases (cout,), h (rows, cout).
 
     `out` receives h (it may share memory with no argument).  keep=True returns (h, gate, up) for `gated_grad`, the two
-    sums in x's type."""
+    sums in float32."""
     dtype, rows, cin, cout = _check_gated(x, w_gate, w_up)
     act = _activation(activation)
     lib = _lib.load()
@@ -305,7 +312,7 @@ def gated(x, w_gate, w_up, bias_gate=None, bias_up=None, activation="silu", out=
     h, ldh = _output(out, x, rows, cout, (("x", x), ("w_gate", w_gate), ("w_up", w_up), ("bias_gate", bias_gate), ("bias_up", bias_up)))
     gate = up = None
     if keep:
-        gate, up = (torch.empty((rows, cout), dtype=x.dtype, device=x.device) for _ in range(2))
+        gate, up = (torch.empty((rows, cout), dtype=torch.float32, device=x.device) for _ in range(2))
     size = lib.fpn_gated_workspace_bytes(dtype, rows, cin, cout)
     ws = _workspace(size, x)
     _call(x, lib.fpn_gated, dtype, rows, cin, cout, _p(x), ldx, _p(w_gate), ldg, _p(w_up), ldu, transposed, _p(bias_gate), _p(bias_up), act,
@@ -313,26 +320,37 @@ def gated(x, w_gate, w_up, bias_gate=None, bias_up=None, activation="silu", out=
     return (h, gate, up) if keep else h
 
 
-def gated_grad(dh, x, w_gate, w_up, gate, up, activation="silu", bias=False, need_x=True, need_w=True):
+def gated_grad(dh, x, w_gate, w_up, gate, up, activation="silu", bias=False, need_x=True, need_w=True, w_down=None):
     """The gradients of `gated`: (dx, dw_gate, dw_up, dbias_gate, dbias_up), each None where it is not asked for
-    (bias=True asks for the last two).  `gate` and `up` are what keep=True returned."""
+    (bias=True asks for the last two).  `gate` and `up` are what keep=True returned.
+
+    With w_down (cout, cdown) the first argument is the gradient of gated(...) @ w_down: the way back through that product
+    is taken on the way, without rounding its result."""
     dtype, rows, cin, cout = _check_gated(x, w_gate, w_up)
     act = _activation(activation)
     lib = _lib.load()
-    for name, t in (("dh", dh), ("gate", gate), ("up", up)):
-        _tensor(name, t, x, (rows, cout))
-    lddh, ldx, ldp = _rows("dh", dh), _rows("x", x, broadcast=True), _rows("gate", gate)
-    if _rows("up", up) != ldp:
+    cdown, ldd, down_transposed = 0, 0, 0
+    if w_down is not None:
+        if not isinstance(w_down, torch.Tensor) or w_down.dim() != 2:
+            raise ValueError("w_down must be a (cout, cdown) tensor")
+        cdown = w_down.shape[1]
+        _tensor("w_down", w_down, x, (cout, cdown))
+        down_transposed, (ldd,) = _weights(("w_down",), (w_down,))
+    _tensor("dh", dh, x, (rows, cdown or cout))
+    ldp = _kept("gate", gate, x, (rows, cout))
+    if _kept("up", up, x, (rows, cout)) != ldp:
         raise ValueError("gate and up must have the same row stride")
+    lddh, ldx = _rows("dh", dh), _rows("x", x, broadcast=True)
     transposed, (ldg, ldu) = _weights(("w_gate", "w_up"), (w_gate, w_up))
     with torch.no_grad():
         dx = torch.empty((rows, cin), dtype=x.dtype, device=x.device) if need_x else None
         dwg, dwu = (_like_weights(w_gate, transposed) for _ in range(2)) if need_w else (None, None)
         dbg, dbu = (torch.empty(cout, dtype=x.dtype, device=x.device) for _ in range(2)) if bias else (None, None)
-    size = lib.fpn_gated_grad_workspace_bytes(dtype, rows, cin, cout)
+    size = lib.fpn_gated_grad_workspace_bytes(dtype, rows, cin, cout, cdown)
     ws = _workspace(size, x)
-    _call(x, lib.fpn_gated_grad, dtype, rows, cin, cout, _p(dh), lddh, _p(x), ldx, _p(w_gate), ldg, _p(w_up), ldu, transposed, _p(gate), _p(up),
-          ldp, act, _p(dx), cin, _p(dwg), _p(dwu), cin if transposed else cout, _p(dbg), _p(dbu), _p(ws), size)
+    _call(x, lib.fpn_gated_grad, dtype, rows, cin, cout, cdown, _p(dh), lddh, _p(w_down), ldd, down_transposed, _p(x), ldx, _p(w_gate),
+          ldg, _p(w_up), ldu, transposed, _p(gate), _p(up), ldp, act, _p(dx), cin, _p(dwg), _p(dwu), cin if transposed else cout,
+          _p(dbg), _p(dbu), _p(ws), size)
     return dx, dwg, dwu, dbg, dbu
 
 
@@ -360,5 +378,36 @@ class _Gated(torch.autograd.Function):
 def gated_feed_forward(x, w_gate, w_up, w_down, bias_gate=None, bias_up=None, bias_down=None, activation="silu", residual=None,
                        out=None):
     """y = gated(x) w_down + bias_down + residual: `gated` and then `dense` with the residual in its epilogue."""
+    if isinstance(x, torch.Tensor) and isinstance(w_down, torch.Tensor) and \
+            _recorded(x, w_gate, w_up, w_down, bias_gate, bias_up, bias_down, residual):
+        if out is not None:
+            raise ValueError("out cannot be given for tensors that require gradients")
+        return _GatedFeedForward.apply(x, w_gate, w_up, w_down, bias_gate, bias_up, bias_down, activation, residual)
     h = gated(x, w_gate, w_up, bias_gate, bias_up, activation)
     return dense(h, w_down, bias_down, None, residual, out)
+
+
+class _GatedFeedForward(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down, bias_gate, bias_up, bias_down, activation, residual):
+        h, gate, up = gated(x, w_gate, w_up, bias_gate, bias_up, activation, keep=True)
+        y, _ = dense(h, w_down, bias_down, None, residual, keep=True)
+        ctx.save_for_backward(x, w_gate, w_up, w_down, h, gate, up)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        _no_capture()
+        x, w_gate, w_up, w_down, h, gate, up = ctx.saved_tensors
+        need_x, need_g, need_u, need_d, need_bg, need_bu, need_bd, _, need_r = ctx.needs_input_grad
+        dx = dwg = dwu = dwd = dbg = dbu = dbd = None
+        d = _dense_rows(dy)
+        if need_d or need_bd:
+            _, dwd, dbd = dense_grad(d, h, w_down, None, None, need_bd, False, need_d)
+        if need_x or need_g or need_u or need_bg or need_bu:
+            dx, dwg, dwu, dbg, dbu = gated_grad(d, x, w_gate, w_up, gate, up, ctx.activation, need_bg or need_bu, need_x,
+                                                need_g or need_u, w_down)
+        return (dx, dwg if need_g else None, dwu if need_u else None, dwd, dbg if need_bg else None, dbu if need_bu else None, dbd, None,
+                dy if need_r else None)

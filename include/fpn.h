@@ -770,11 +770,11 @@ int fpn_detection_records(int b, int n, const float *mask_logits, const float *b
 
 /*
  * y = act(x w + bias) + residual.   x (rows,cin), w (cin,cout), bias (cout) or NULL, residual (rows,cout) or NULL,
- * y (rows,cout); pre (rows,cout) or NULL receives x w + bias for fpn_dense_grad.
+ * y (rows,cout); pre (rows,cout), always float, or NULL receives x w + bias for fpn_dense_grad.
  */
 size_t fpn_dense_workspace_bytes(int dtype, long rows, int cin, int cout);
 int fpn_dense(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w, long ldw, int w_transposed,
-              const void *bias, int activation, const void *residual, long ldr, void *y, long ldy, void *pre, long ldp,
+              const void *bias, int activation, const void *residual, long ldr, void *y, long ldy, float *pre, long ldp,
               void *workspace, size_t workspace_bytes, void *stream);
 
 /*
@@ -784,29 +784,32 @@ int fpn_dense(int dtype, long rows, int cin, int cout, const void *x, long ldx, 
  */
 size_t fpn_dense_grad_workspace_bytes(int dtype, long rows, int cin, int cout, int activation);
 int fpn_dense_grad(int dtype, long rows, int cin, int cout, const void *dy, long lddy, const void *x, long ldx, const void *w,
-                   long ldw, int w_transposed, const void *pre, long ldp, int activation, void *dx, long lddx, void *dw, long lddw,
+                   long ldw, int w_transposed, const float *pre, long ldp, int activation, void *dx, long lddx, void *dw, long lddw,
                    void *dbias, void *workspace, size_t workspace_bytes, void *stream);
 
 /*
  * h = act(x w_gate + bias_gate) * (x w_up + bias_up).   Both weights (cin,cout) or both (cout,cin), each with its own
- * row stride (halves of one matrix will do); gate and up (rows,cout), row stride ldp, receive the two sums for
- * fpn_gated_grad, or are both NULL.
+ * row stride (halves of one matrix will do); gate and up (rows,cout), always float, row stride ldp, receive the
+ * two sums for fpn_gated_grad, or are both NULL.
  */
 size_t fpn_gated_workspace_bytes(int dtype, long rows, int cin, int cout);
 int fpn_gated(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w_gate, long ldg, const void *w_up,
-              long ldu, int w_transposed, const void *bias_gate, const void *bias_up, int activation, void *h, long ldh, void *gate,
-              void *up, long ldp, void *workspace, size_t workspace_bytes, void *stream);
+              long ldu, int w_transposed, const void *bias_gate, const void *bias_up, int activation, void *h, long ldh, float *gate,
+              float *up, long ldp, void *workspace, size_t workspace_bytes, void *stream);
 
 /*
  * Its gradients, dg = dh up act'(gate), du = dh act(gate):  dx = dg w_gate^T + du w_up^T, dw_gate = x^T dg,
  * dw_up = x^T du (both in the weights' storage order, row stride lddw), and the column sums of dg and du.
  * dx, the pair of dw and the pair of dbias may each be NULL.
+ * cdown > 0: the block's down projection y = h w_down is gone back through first - `dh` is then dy (rows,cdown), and
+ * dh = dy w_down^T is formed here and never rounded (w_down (cout,cdown), or (cdown,cout) where down_transposed);
+ * cdown 0: w_down is not read.
  */
-size_t fpn_gated_grad_workspace_bytes(int dtype, long rows, int cin, int cout);
-int fpn_gated_grad(int dtype, long rows, int cin, int cout, const void *dh, long lddh, const void *x, long ldx, const void *w_gate,
-                   long ldg, const void *w_up, long ldu, int w_transposed, const void *gate, const void *up, long ldp, int activation,
-                   void *dx, long lddx, void *dw_gate, void *dw_up, long lddw, void *dbias_gate, void *dbias_up, void *workspace,
-                   size_t workspace_bytes, void *stream);
+size_t fpn_gated_grad_workspace_bytes(int dtype, long rows, int cin, int cout, int cdown);
+int fpn_gated_grad(int dtype, long rows, int cin, int cout, int cdown, const void *dh, long lddh, const void *w_down, long ldd,
+                   int down_transposed, const void *x, long ldx, const void *w_gate, long ldg, const void *w_up, long ldu,
+                   int w_transposed, const float *gate, const float *up, long ldp, int activation, void *dx, long lddx, void *dw_gate,
+                   void *dw_up, long lddw, void *dbias_gate, void *dbias_up, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -40,7 +40,7 @@ def gated(**kw):
 
 
 def gated_grad(**kw):
-    a = dict(dtype=BF16, rows=4, cin=8, cout=16, dh=P, lddh=16, x=P, ldx=8, wg=P, ldg=16, wu=P, ldu=16, tr=0, gate=P, up=P, ldp=16,
+    a = dict(dtype=BF16, rows=4, cin=8, cout=16, cdown=0, dh=P, lddh=16, wd=None, ldd=0, trd=0, x=P, ldx=8, wg=P, ldg=16, wu=P, ldu=16, tr=0, gate=P, up=P, ldp=16,
              act=2, dx=P, lddx=8, dwg=P, dwu=P, lddw=16, dbg=None, dbu=None, ws=P, size=BIG)
     a.update(kw)
     return lib().fpn_gated_grad(*a.values(), None)
@@ -69,6 +69,10 @@ def test_bad_arguments(call, bad, code, text):
     (dense_grad, dict(size=10), "workspace"),
     (gated, dict(wu=None), "w_up is null"), (gated, dict(ldu=1), "w_up: row stride"), (gated, dict(gate=P, ldp=16), "together"),
     (gated, dict(gate=P, up=P, ldp=15), "gate"), (gated, dict(ldh=2), "h: row stride"), (gated, dict(bu=ODD), "bias_up"),
+    (gated_grad, dict(cdown=-1), "cdown"), (gated_grad, dict(cdown=24, lddh=24), "w_down is null"),
+    (gated_grad, dict(cdown=24, lddh=24, wd=P, ldd=23), "w_down: row stride"), (gated_grad, dict(cdown=24, wd=P, ldd=24), "dh: row stride"),
+    (gated_grad, dict(cdown=24, lddh=24, wd=P, ldd=15, trd=1), "w_down: row stride"),
+    (gated_grad, dict(gate=ctypes.c_void_p(258)), "gate is not aligned"),
     (gated_grad, dict(gate=None), "gate is null"), (gated_grad, dict(dwu=None), "together"), (gated_grad, dict(dbu=P), "together"),
     (gated_grad, dict(lddw=3), "dw_gate"), (gated_grad, dict(ws=None), "workspace")])
 def test_bad_arguments_of_one(call, bad, text):
@@ -89,7 +93,7 @@ def test_workspace_sizes():
     for t, size in ((F32, 4), (BF16, 2), (F16, 2)):
         d = 1000 * 512 * size
         assert L.fpn_dense_grad_workspace_bytes(t, 1000, 64, 512, 2) >= d
-        assert L.fpn_gated_grad_workspace_bytes(t, 1000, 64, 512) >= 2 * d
+        assert L.fpn_gated_grad_workspace_bytes(t, 1000, 64, 512, 0) >= 2 * d
         # partial sums of a split product: whole copies of the result
         need = L.fpn_dense_workspace_bytes(t, 16, 8192, 256)
         assert need % (16 * 256 * 4) == 0

@@ -5,9 +5,9 @@ it adds
   * fp32 accumulation of K products: at most K 2^-24 of the sum of their magnitudes, in practice its square root;
     taken as 2^-24 (4 + sqrt K) of the root of the sum of the squared products, times the largest of the output's
     values in units of its standard deviation (6);
-  * in the backward pass of 16-bit types the rounded pre-activations (gate, up) and the rounded dpre (dg, du), each a
-    relative half step on one factor of every product: sqrt(4) u of the same root;
-  * in gated_feed_forward h, gate, up and dh likewise: sqrt(6) u.
+  * in the backward pass of 16-bit types the rounded dpre (dg, du), a relative half step on one factor of every product:
+    u of the same root (pre-activations are kept in fp32);
+  * in gated_feed_forward h likewise: sqrt(2) u.
   * in the backward pass the forward sums' own error: a pre-activation is off by delta = 6 2^-24 (4 + sqrt cin) S(x, w)
     + u |pre|; slopes move by at most delta (curvature <= 1), values by 1.13 delta, and the products' terms with them
     (`moved`).
@@ -91,16 +91,16 @@ def dense_case(device, t, rows, cin, cout, act, bias, residual, cols, seed=0):
     s = root(x, w) + a.abs() + want.abs()
     check(y, want, 1.2 * s, cin, u, what="y")
     if act:
-        check(pre, p, s + p.abs(), cin, u, what="pre")
+        check(pre, p, s + p.abs(), cin, 2.0 ** -24, what="pre")
     dx, dw, db = F.dense_grad(d["dy"], d["x"], d["w"], pre, act, bias=True)
     if act == "relu":                                     # the step of the derivative goes by the kernel's own sums
         slope = (f64(pre) > 0).double()
     e = dy * slope
     spread = dy.abs() * (1.2 + p.abs())                   # what a half step of pre and of e is relative to
     off = dy.abs() * sum_error(x, w, cin) if act else 0 * dy
-    check(dx, e @ w.t(), root(spread, w.t()), cout, u, 2 if act else 0, "dx", root(off, w.t()))
-    check(dw, x.t() @ e, root(x.t(), spread), rows, u, 2 if act else 0, "dw", root(x.t(), off))
-    check(db, e.sum(0), spread.square().sum(0).sqrt(), rows, u, 2 if act else 0, "db", off.square().sum(0).sqrt())
+    check(dx, e @ w.t(), root(spread, w.t()), cout, u, 1 if act else 0, "dx", root(off, w.t()))
+    check(dw, x.t() @ e, root(x.t(), spread), rows, u, 1 if act else 0, "dw", root(x.t(), off))
+    check(db, e.sum(0), spread.square().sum(0).sqrt(), rows, u, 1 if act else 0, "db", off.square().sum(0).sqrt())
 
 
 SIZES = [(1, 1, 1), (1, 5, 3), (2, 3, 7), (5, 4, 8), (1, 1027, 512), (7, 64, 64), (33, 63, 65), (64, 128, 128), (65, 129, 127),
@@ -132,8 +132,8 @@ def gated_case(device, t, rows, cin, cout, act, bias, cols, seed=0):
     pg, pu = x @ wg + (f64(bg) if bias else 0), x @ wu + (f64(bu) if bias else 0)
     a, slope = act64(pg, act)
     sg, su = root(x, wg) + pg.abs(), root(x, wu) + pu.abs()
-    check(gate, pg, sg, cin, u, what="gate")
-    check(up, pu, su, cin, u, what="up")
+    check(gate, pg, sg, cin, 2.0 ** -24, what="gate")
+    check(up, pu, su, cin, 2.0 ** -24, what="up")
     check(h, a * pu, 1.2 * sg * pu.abs() + su * a.abs() + (a * pu).abs(), cin, u, what="h")
     dx, dwg, dwu, dbg, dbu = F.gated_grad(d["dh"], d["x"], d["wg"], d["wu"], gate, up, act, bias=True)
     if act == "relu":
@@ -142,12 +142,12 @@ def gated_case(device, t, rows, cin, cout, act, bias, cols, seed=0):
     tg, tu = dh.abs() * (pu.abs() + 2.0 ** -24 * su) * (1.2 + pg.abs()), dh.abs() * (1.2 * pg.abs() + a.abs())
     og = dh.abs() * (1.13 * sum_error(x, wu, cin) + pu.abs() * sum_error(x, wg, cin))
     ou = dh.abs() * 1.13 * sum_error(x, wg, cin)
-    check(dx, eg @ wg.t() + eu @ wu.t(), (root(tg, wg.t()).square() + root(tu, wu.t()).square()).sqrt(), 2 * cout, u, 2, "dx",
+    check(dx, eg @ wg.t() + eu @ wu.t(), (root(tg, wg.t()).square() + root(tu, wu.t()).square()).sqrt(), 2 * cout, u, 1, "dx",
           root(og, wg.t()) + root(ou, wu.t()))
-    check(dwg, x.t() @ eg, root(x.t(), tg), rows, u, 2, "dwg", root(x.t(), og))
-    check(dwu, x.t() @ eu, root(x.t(), tu), rows, u, 2, "dwu", root(x.t(), ou))
-    check(dbg, eg.sum(0), tg.square().sum(0).sqrt(), rows, u, 2, "dbg", og.square().sum(0).sqrt())
-    check(dbu, eu.sum(0), tu.square().sum(0).sqrt(), rows, u, 2, "dbu", ou.square().sum(0).sqrt())
+    check(dwg, x.t() @ eg, root(x.t(), tg), rows, u, 1, "dwg", root(x.t(), og))
+    check(dwu, x.t() @ eu, root(x.t(), tu), rows, u, 1, "dwu", root(x.t(), ou))
+    check(dbg, eg.sum(0), tg.square().sum(0).sqrt(), rows, u, 1, "dbg", og.square().sum(0).sqrt())
+    check(dbu, eu.sum(0), tu.square().sum(0).sqrt(), rows, u, 1, "dbu", ou.square().sum(0).sqrt())
 
 
 @pytest.mark.parametrize("t", list(TYPES))
@@ -305,7 +305,7 @@ def test_no_rows(device):
 
 
 @pytest.mark.parametrize("t", list(TYPES))
-@pytest.mark.parametrize("rows,cin,hidden", [(1, 64, 256), (3, 130, 67), (200, 96, 256)])
+@pytest.mark.parametrize("rows,cin,hidden", [(1, 64, 256), (3, 130, 67), (200, 96, 256), (333, 160, 328), (700, 64, 2048), (130, 72, 24)])
 def test_block_runs_together_and_its_gradients(device, t, rows, cin, hidden):
     """gated_feed_forward with its residual through autograd, against the formula's gradients in float64."""
     from fpn import feed_forward as F
@@ -325,10 +325,32 @@ def test_block_runs_together_and_its_gradients(device, t, rows, cin, hidden):
     Y = h @ WD + BD + RES
     want = torch.autograd.grad(Y, l64, f64(d["dy"]))
     s = root(h.detach(), WD.detach()) + root(X.detach(), WG.detach()).mean() + Y.detach().abs()
-    check(y, Y.detach(), 2 * s, hidden, u, 2.5, "y")
+    check(y, Y.detach(), 2 * s, hidden, u, 1.5, "y")
     for name, g, w_ in zip(names, grads, want):
         scale = w_.square().mean().sqrt()                  # (every gradient's terms have about its own spread)
-        check(g, w_, 2 * (w_.abs() + scale), max(rows, hidden, cin), u, 2.5, "d" + name)
+        check(g, w_, 2 * (w_.abs() + scale), max(rows, hidden, cin), u, 1.5, "d" + name)
+
+
+@pytest.mark.parametrize("t", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,cin,hidden,cols", [(5, 24, 40, False), (260, 96, 520, False), (260, 96, 520, True), (1100, 64, 1024, False),
+                                                  (257, 33, 70, True)])
+def test_gradient_through_the_down_projection(device, t, rows, cin, hidden, cols):
+    """gated_grad with w_down, for the kernel that makes dg and du in the product's epilogue and for the one that does not:
+    against gated_grad on dh = dy w_down^T formed in float64 (rounded once, which is what the call saves: a relative u on
+    every term)."""
+    from fpn import feed_forward as F
+    dtype, u = TYPES[t]
+    d = make(device, dtype, rows, cin, cin, seed=8, hidden=hidden, cols=cols)
+    for act in ("silu", "gelu_tanh"):
+        _, gate, up = F.gated(d["x"], d["wg"], d["wu"], d["bg"], d["bu"], act, keep=True)
+        got = F.gated_grad(d["dy"], d["x"], d["wg"], d["wu"], gate, up, act, bias=True, w_down=d["wd"])
+        dh = (d["dy"].double() @ d["wd"].double().t()).to(dtype)
+        want = F.gated_grad(dh, d["x"], d["wg"], d["wu"], gate, up, act, bias=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, F.gated_grad(d["dy"], d["x"], d["wg"], d["wu"], gate, up, act, bias=True, w_down=d["wd"])))
+        for name, a, b in zip(("dx", "dwg", "dwu", "dbg", "dbu"), got, want):
+            # both sides round the result (u each) and dg, du (u each); dh's rounding and fp32 sums add u and 2^-24 sqrt k
+            off = float((a.double() - b.double()).norm() / b.double().norm())
+            assert off <= 5 ** 0.5 * u + 4 * 2.0 ** -24 * max(rows, cin, hidden) ** 0.5, (name, off)
 
 
 def test_gradients_against_differences(device):
