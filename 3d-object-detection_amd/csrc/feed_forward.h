@@ -12,8 +12,8 @@
 //
 // A workgroup of four waves owns a BM x BN tile; each wave a grid of 32 x 32 MFMA tiles.  The MFMA's A operand is the
 // b side (lane = output column), its B operand the a side (lane = output row), so a lane's accumulators run along
-// an output ROW and v_permlane32_swap turns them into runs of eight columns: bias, residual and result move as
-// 16-byte vectors.
+// an output ROW, and a pass through LDS turns them into runs of eight columns of consecutive rows: bias, residual and
+// result move as 16-byte vectors.
 #pragma once
 #include <algorithm>
 #include <cstdint>
@@ -490,21 +490,161 @@ template <class T> __device__ inline floatx16 multiply(uintx4 b, uintx4 a, float
     }
 }
 
-// An accumulator tile (lane l31 = row, register r = column (r & 3) + 8 (r >> 2) + 4 h) as two runs of eight columns
-// from 8 h and from 16 + 8 h on
-__device__ inline void runs(const floatx16 &c, float (&v)[2][8])
+// A wave's accumulators to memory through its own piece of LDS, 32 rows at a time: written as they lie (a lane has four
+// consecutive columns of one row), read back as runs of eight columns of consecutive rows - whole lines for the
+// loads and stores, bias loaded once, and one copy of the epilogue's arithmetic: unrolled over a wave's tiles it was 200 KB of
+// code, which small products spent their time fetching (a gated fp32 product of 777 x 259 x 515: 21 us against XX).  `lds` is
+// the wave's, epilogue_bytes(TN); nobody else uses it.
+constexpr int epilogue_bytes(int tn) { return 32 * (32 * tn * 4 + 16); }
+
+// MODE: a plain product, a gated one, or the gated block's backward epilogue on a plain one
+enum { kPlainMode = 0, kGatedMode = 1, kGateGradMode = 2 };
+
+template <class T, int MODE, int TM, int TN>
+__device__ inline void store_piece(const Args &p, const floatx16 (&acc)[TM][TN], char *lds, int member, int split, long m0, int n0, int lane)
 {
+    constexpr bool EXACT = sizeof(T) == 4, GATED = MODE == kGatedMode;
+    constexpr int kTN = TN, kEpilogueRow = 32 * kTN * 4 + 16;
+    const int l31 = lane & 31, h = lane >> 5;
+    constexpr int kRuns = GATED ? 2 * kTN : 4 * kTN, kRowsAtOnce = 64 / kRuns, kBatch = EXACT || MODE == kGateGradMode ? 1 : 2;     // runs of eight columns per row
+    const int run = lane % kRuns, row0 = lane / kRuns;
+    const int n = n0 + run * 8;
+    const long left = p.n - n;
+    auto put = [&](const floatx16 (&c)[kTN]) {
 #pragma unroll
-    for (int q = 0; q < 2; ++q)
+        for (int j = 0; j < kTN; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            // (values first: a bit cast of a vector's element reads the vector's first)
-            const float lo = c[8 * q + i], hi = c[8 * q + 4 + i];
-            const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, lo), __builtin_bit_cast(unsigned, hi), false, false);
-            const unsigned r0 = r[0], r1 = r[1];
-            v[q][i] = __builtin_bit_cast(float, r0);
-            v[q][4 + i] = __builtin_bit_cast(float, r1);
+            for (int q = 0; q < 4; ++q) {
+                floatx4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = c[j][4 * q + e];
+                *reinterpret_cast<floatx4 *>(lds + l31 * kEpilogueRow + (32 * j + 8 * q + 4 * h) * 4) = v;
+            }
+    };
+    float bias[8] = {}, bias2[8] = {};
+    if (MODE != kGateGradMode && left > 0 && p.bias[GATED ? 0 : member]) load8(reinterpret_cast<const T *>(p.bias[GATED ? 0 : member]) + n, left, bias);
+    if (GATED && left > 0 && p.bias[1]) load8(reinterpret_cast<const T *>(p.bias[1]) + n, left, bias2);
+#pragma unroll 1
+    for (int i = 0; i < TM; ++i) {
+        if (i == 0) put(acc[0]);
+        else if (TM == 2 || i == 1) put(acc[TM > 1 ? 1 : 0]);
+        else if (i == 2) put(acc[TM > 2 ? 2 : 0]);
+        else put(acc[TM > 2 ? 3 : 0]);
+        if (left <= 0) continue;
+        // two rows' loads at a time, then their arithmetic, then their stores: with one wave per SIMD nothing else
+        // would cover the latency
+#pragma unroll 1
+        for (int r = row0; r < 32; r += kRowsAtOnce * kBatch) {
+            const long m = m0 + 32 * i + r;
+            float v[kBatch][8], v2[GATED ? kBatch : 1][8], res[kBatch][8];
+            if (MODE != kGateGradMode && p.residual)
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b)
+                    load8(reinterpret_cast<const T *>(p.residual) + min(m + b * kRowsAtOnce, p.m - 1) * p.ldr + n, left, res[b]);
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                const float *from = reinterpret_cast<const float *>(lds + (r + b * kRowsAtOnce) * kEpilogueRow) + run * 8;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    v[b][e] = from[e];
+                    if (GATED) v2[b][e] = from[16 * kTN + e];
+                }
+            }
+            if constexpr (MODE == kGateGradMode) {
+                // the gated block's backward pass: dh in, dg and du out (no bias in such a product: its registers
+                // take the column sums)
+                float g[kBatch][8], u[kBatch][8];
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b) {
+                    const long row = min(m + b * kRowsAtOnce, p.m - 1);
+                    load8(p.gate + row * p.ldp + n, left, g[b]);
+                    load8(p.up + row * p.ldp + n, left, u[b]);
+                }
+                for_activation(p.act, [&](auto tag) {
+#pragma unroll
+                    for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            float value;
+                            const float slope = activate_grad<decltype(tag)::value, EXACT>(g[b][e], value);
+                            g[b][e] = v[b][e] * u[b][e] * slope;
+                            u[b][e] = v[b][e] * value;
+                        }
+                });
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b)
+                    if (m + b * kRowsAtOnce < p.m) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            bias[e] += g[b][e];
+                            bias2[e] += u[b][e];
+                        }
+                        store8(reinterpret_cast<T *>(p.c[0]) + (m + b * kRowsAtOnce) * p.ldc + n, left, g[b]);
+                        store8(reinterpret_cast<T *>(p.c[1]) + (m + b * kRowsAtOnce) * p.ldc + n, left, u[b]);
+                    }
+                continue;
+            }
+            if (p.partial) {
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b)
+                    if (m + b * kRowsAtOnce < p.m) {
+                        float *to = p.partial + ((((long)member * p.splits + split) * (GATED ? 2 : 1)) * p.m + m + b * kRowsAtOnce) * p.n + n;
+                        store8(to, left, v[b]);
+                        if (GATED) store8(to + p.m * p.n, left, v2[b]);
+                    }
+                continue;
+            }
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    v[b][e] += bias[e];
+                    if (GATED) v2[b][e] += bias2[e];
+                }
+            if (p.pre[0])
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b)
+                    if (m + b * kRowsAtOnce < p.m) {
+                        store8(p.pre[0] + (m + b * kRowsAtOnce) * p.ldp + n, left, v[b]);
+                        if (GATED) store8(p.pre[1] + (m + b * kRowsAtOnce) * p.ldp + n, left, v2[b]);
+                    }
+            if (p.act != FPN_ACT_NONE)
+                for_activation(p.act, [&](auto tag) {
+#pragma unroll
+                    for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[b][e] = activate<decltype(tag)::value, EXACT>(v[b][e]);
+                });
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (GATED) v[b][e] *= v2[b][e];
+                    if (p.residual) v[b][e] += res[b][e];
+                }
+                if (m + b * kRowsAtOnce < p.m) {
+                    if (p.c_float) store8(reinterpret_cast<float *>(p.c[member]) + (m + b * kRowsAtOnce) * p.ldc + n, left, v[b]);
+                    else store8(reinterpret_cast<T *>(p.c[member]) + (m + b * kRowsAtOnce) * p.ldc + n, left, v[b]);
+                }
+            }
         }
+    }
+    if constexpr (MODE == kGateGradMode) {
+        if (!p.sums) return;
+        // the column sums of this wave's rows: the lanes of one run of columns, in a fixed order
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int far = kRuns; far < 64; far *= 2) {
+                bias[e] += __shfl_xor(bias[e], far);
+                bias2[e] += __shfl_xor(bias2[e], far);
+            }
+        if (row0 == 0 && left > 0) {
+            float *to = p.sums + m0 / (32 * TM) * 2 * p.n + n;
+            store8(to, left, bias);
+            store8(to + p.n, left, bias2);
+        }
+    }
 }
 
 // Workgroup -> (output tile, batch member, split).  Workgroups go round the eight XCDs; each XCD takes a contiguous
@@ -620,30 +760,7 @@ __global__ __launch_bounds__(kThreads) void product_kernel(const Args p)
         __syncthreads();
     }
 
-    const int l31 = lane & 31, h = lane >> 5;
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-        const long m = m0 + am[i] + l31;
-        if (m >= p.m) continue;
-#pragma unroll
-        for (int j = 0; j < (GATED ? TN / 2 : TN); ++j) {
-            float v[2][8], v2[2][8];
-            runs(acc[i][j], v);
-            if (GATED) runs(acc[i][(j + TN / 2) % TN], v2);
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const int n = n0 + bn[j] + 16 * q + 8 * h;
-                if (n >= p.n) continue;
-                if (p.partial) {
-                    float *to = p.partial + ((((long)at.member * p.splits + at.split) * (GATED ? 2 : 1)) * p.m + m) * p.n + n;
-                    store8(to, p.n - n, v[q]);
-                    if (GATED) store8(to + p.m * p.n, p.n - n, v2[q]);
-                } else {
-                    finish8<T, GATED>(p, at.member, m, n, v[q], v2[q]);
-                }
-            }
-        }
-    }
+    store_piece<T, GATED ? kGatedMode : kPlainMode, TM, TN>(p, acc, lds + wave * epilogue_bytes(TN), at.member, at.split, m0 + am[0], n0 + bn[0], lane);
 }
 
 // Joins the partial sums of a split product: a workgroup takes 32 runs of eight columns, its eight rows of threads
@@ -730,9 +847,9 @@ extern template int launch_few<_Float16>(const Args &, int, bool, int, int, hipS
 #define FPN_FF_LAUNCH(A, B, BM_, BN_, WM_, WN_, G)                                                                            \
     do {                                                                                                                      \
         auto kern = product_kernel<T, A, B, BM_, BN_, WM_, WN_, G>;                                                           \
-        const size_t bytes = 2 * (size_t)(BM_ + BN_) * kTileBytes;                                                            \
+        constexpr int bytes = std::max(2 * (BM_ + BN_) * kTileBytes, WM_ * WN_ * epilogue_bytes(BN_ / WN_ / 32));             \
         if (!allow_dynamic_lds(reinterpret_cast<const void *>(kern), bytes))                                                  \
-            return fail(FPN_E_LAUNCH, "%zu bytes of LDS refused", bytes);                                                     \
+            return fail(FPN_E_LAUNCH, "%d bytes of LDS refused", bytes);                                                      \
         hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(kThreads), bytes, stream, p);                                   \
     } while (0)
 

@@ -25,8 +25,7 @@ template <int BM_, int BN_, int WM_, int WN_, int STAGES, int PER_CU> struct Sha
     static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves, TM = BM / WM / 32, TN = BN / WN / 32;
     static constexpr int kStage = (BM + BN) * kWideK * 2;            // bytes: BM rows of a, BN of b
     static constexpr int kPerSimd = kWaves * PER_CU / 4;
-    // the epilogue's piece of LDS of a wave: 32 rows of its columns, as floats
-    static constexpr int kEpilogueRow = 32 * TN * 4 + 16, kEpilogueBytes = 32 * kEpilogueRow;
+    static constexpr int kEpilogueBytes = epilogue_bytes(TN);
     static constexpr int kBytes = std::max(kStages * kStage, kWaves * kEpilogueBytes);
 };
 using Large = Shape<256, 256, 2, 4, 4, 1>;
@@ -159,160 +158,6 @@ template <class T, int ORDER, int R, int TILES> struct StreamReader {
         return v;
     }
 };
-
-// A wave's accumulators to memory through its own piece of LDS, 32 rows at a time: written as they lie (a lane has four
-// consecutive columns of one row), read back as runs of eight columns of consecutive rows - whole lines for the
-// loads and stores, one copy of the epilogue's arithmetic, bias loaded once.  `lds` is the wave's:
-// kEpilogueBytes; nobody else uses it.
-// MODE: a plain product, a gated one, or the gated block's backward epilogue on a plain one
-enum { kPlainMode = 0, kGatedMode = 1, kGateGradMode = 2 };
-
-template <class T, int MODE, class S>
-__device__ inline void store_piece(const Args &p, const floatx16 (&acc)[S::TM][S::TN], char *lds, int member, int split, long m0, int n0, int lane)
-{
-    constexpr bool EXACT = sizeof(T) == 4, GATED = MODE == kGatedMode;
-    constexpr int kTN = S::TN, kEpilogueRow = S::kEpilogueRow;
-    const int l31 = lane & 31, h = lane >> 5;
-    constexpr int kRuns = GATED ? 2 * kTN : 4 * kTN, kRowsAtOnce = 64 / kRuns, kBatch = MODE == kGateGradMode ? 1 : 2;     // runs of eight columns per row
-    const int run = lane % kRuns, row0 = lane / kRuns;
-    const int n = n0 + run * 8;
-    const long left = p.n - n;
-    auto put = [&](const floatx16 (&c)[kTN]) {
-#pragma unroll
-        for (int j = 0; j < kTN; ++j)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                floatx4 v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = c[j][4 * q + e];
-                *reinterpret_cast<floatx4 *>(lds + l31 * kEpilogueRow + (32 * j + 8 * q + 4 * h) * 4) = v;
-            }
-    };
-    float bias[8] = {}, bias2[8] = {};
-    if (MODE != kGateGradMode && left > 0 && p.bias[GATED ? 0 : member]) load8(reinterpret_cast<const T *>(p.bias[GATED ? 0 : member]) + n, left, bias);
-    if (GATED && left > 0 && p.bias[1]) load8(reinterpret_cast<const T *>(p.bias[1]) + n, left, bias2);
-#pragma unroll 1
-    for (int i = 0; i < S::TM; ++i) {
-        if (i == 0) put(acc[0]);
-        else if (S::TM == 2 || i == 1) put(acc[S::TM > 1 ? 1 : 0]);
-        else if (i == 2) put(acc[S::TM > 2 ? 2 : 0]);
-        else put(acc[S::TM > 2 ? 3 : 0]);
-        if (left <= 0) continue;
-        // two rows' loads at a time, then their arithmetic, then their stores: with one wave per SIMD nothing else
-        // would cover the latency
-#pragma unroll 1
-        for (int r = row0; r < 32; r += kRowsAtOnce * kBatch) {
-            const long m = m0 + 32 * i + r;
-            float v[kBatch][8], v2[GATED ? kBatch : 1][8], res[kBatch][8];
-            if (MODE != kGateGradMode && p.residual)
-#pragma unroll
-                for (int b = 0; b < kBatch; ++b)
-                    load8(reinterpret_cast<const T *>(p.residual) + min(m + b * kRowsAtOnce, p.m - 1) * p.ldr + n, left, res[b]);
-#pragma unroll
-            for (int b = 0; b < kBatch; ++b) {
-                const float *from = reinterpret_cast<const float *>(lds + (r + b * kRowsAtOnce) * kEpilogueRow) + run * 8;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    v[b][e] = from[e];
-                    if (GATED) v2[b][e] = from[16 * kTN + e];
-                }
-            }
-            if constexpr (MODE == kGateGradMode) {
-                // the gated block's backward pass: dh in, dg and du out (no bias in such a product: its registers
-                // take the column sums)
-                float g[kBatch][8], u[kBatch][8];
-#pragma unroll
-                for (int b = 0; b < kBatch; ++b) {
-                    const long row = min(m + b * kRowsAtOnce, p.m - 1);
-                    load8(p.gate + row * p.ldp + n, left, g[b]);
-                    load8(p.up + row * p.ldp + n, left, u[b]);
-                }
-                for_activation(p.act, [&](auto tag) {
-#pragma unroll
-                    for (int b = 0; b < kBatch; ++b)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            float value;
-                            const float slope = activate_grad<decltype(tag)::value, EXACT>(g[b][e], value);
-                            g[b][e] = v[b][e] * u[b][e] * slope;
-                            u[b][e] = v[b][e] * value;
-                        }
-                });
-#pragma unroll
-                for (int b = 0; b < kBatch; ++b)
-                    if (m + b * kRowsAtOnce < p.m) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            bias[e] += g[b][e];
-                            bias2[e] += u[b][e];
-                        }
-                        store8(reinterpret_cast<T *>(p.c[0]) + (m + b * kRowsAtOnce) * p.ldc + n, left, g[b]);
-                        store8(reinterpret_cast<T *>(p.c[1]) + (m + b * kRowsAtOnce) * p.ldc + n, left, u[b]);
-                    }
-                continue;
-            }
-            if (p.partial) {
-#pragma unroll
-                for (int b = 0; b < kBatch; ++b)
-                    if (m + b * kRowsAtOnce < p.m) {
-                        float *to = p.partial + ((((long)member * p.splits + split) * (GATED ? 2 : 1)) * p.m + m + b * kRowsAtOnce) * p.n + n;
-                        store8(to, left, v[b]);
-                        if (GATED) store8(to + p.m * p.n, left, v2[b]);
-                    }
-                continue;
-            }
-#pragma unroll
-            for (int b = 0; b < kBatch; ++b)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    v[b][e] += bias[e];
-                    if (GATED) v2[b][e] += bias2[e];
-                }
-            if (p.pre[0])
-#pragma unroll
-                for (int b = 0; b < kBatch; ++b)
-                    if (m + b * kRowsAtOnce < p.m) {
-                        store8(p.pre[0] + (m + b * kRowsAtOnce) * p.ldp + n, left, v[b]);
-                        if (GATED) store8(p.pre[1] + (m + b * kRowsAtOnce) * p.ldp + n, left, v2[b]);
-                    }
-            if (p.act != FPN_ACT_NONE)
-                for_activation(p.act, [&](auto tag) {
-#pragma unroll
-                    for (int b = 0; b < kBatch; ++b)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[b][e] = activate<decltype(tag)::value, EXACT>(v[b][e]);
-                });
-#pragma unroll
-            for (int b = 0; b < kBatch; ++b) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if (GATED) v[b][e] *= v2[b][e];
-                    if (p.residual) v[b][e] += res[b][e];
-                }
-                if (m + b * kRowsAtOnce < p.m) {
-                    if (p.c_float) store8(reinterpret_cast<float *>(p.c[member]) + (m + b * kRowsAtOnce) * p.ldc + n, left, v[b]);
-                    else store8(reinterpret_cast<T *>(p.c[member]) + (m + b * kRowsAtOnce) * p.ldc + n, left, v[b]);
-                }
-            }
-        }
-    }
-    if constexpr (MODE == kGateGradMode) {
-        if (!p.sums) return;
-        // the column sums of this wave's rows: the lanes of one run of columns, in a fixed order
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-#pragma unroll
-            for (int far = kRuns; far < 64; far *= 2) {
-                bias[e] += __shfl_xor(bias[e], far);
-                bias2[e] += __shfl_xor(bias2[e], far);
-            }
-        if (row0 == 0 && left > 0) {
-            float *to = p.sums + m0 / (32 * S::TM) * 2 * p.n + n;
-            store8(to, left, bias);
-            store8(to + p.n, left, bias2);
-        }
-    }
-}
 
 template <class T, int ORDER_A, int ORDER_B, int MODE, class S>
 __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void wide_product_kernel(const Args p)
@@ -477,7 +322,7 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void wide_product_kernel(
         }
         __syncthreads();
     }
-    store_piece<T, MODE, S>(p, acc, lds + wave * S::kEpilogueBytes, at.member, at.split, m0 + wm * 32 * kTM,
+    store_piece<T, MODE, kTM, kTN>(p, acc, lds + wave * S::kEpilogueBytes, at.member, at.split, m0 + wm * 32 * kTM,
                              n0 + wn * 32 * (GATED ? kTN / 2 : kTN), lane);
 }
 
