@@ -288,7 +288,7 @@ __device__ inline uintx4 shift_right(uintx4 v, int bits)       // the 128-bit nu
 //
 // Ends: rows beyond the last repeat it (their results are never stored).  Along the contiguous direction a chunk
 // that would pass the end is read from the last 16 bytes inside and shifted into place, which also puts zeros
-// behind the end: no access leaves the operand, whatever its width and alignment.  Widths under one chunk are read
+// behind the end: no access leaves the operand, whatever its width and alignment.  Operands under one chunk wide are read
 // element by element.
 template <class T, int ORDER, int R> struct Tile {
     static constexpr int E = Type<T>::kE;
@@ -301,6 +301,7 @@ template <class T, int ORDER, int R> struct Tile {
     long ld;
     long k;                  // of the segment
     long outer;              // rows or columns from this tile's first to the operand's end
+    bool narrow;             // the operand is under one chunk wide
     unsigned off[kChunks];   // byte offsets of this thread's chunks in an inner k tile
     unsigned put_at[kChunks];
     int pos;                 // kInner: first k of this thread's chunks; kOuter: its first m / n
@@ -308,9 +309,10 @@ template <class T, int ORDER, int R> struct Tile {
     unsigned zero;           // bit i: chunk i of the last loaded tile lies behind the last k
     uintx4 reg[kChunks];
 
-    __device__ void init(long outer_left, int tid)
+    __device__ void init(long outer_left, long all, long k_, int tid)
     {
         outer = outer_left;
+        narrow = (ORDER == kInner ? k_ : all) < E;
         shift = 0;
         zero = 0;
         if (ORDER == kInner) {
@@ -338,7 +340,7 @@ template <class T, int ORDER, int R> struct Tile {
             const int g = (((kk & 1) << 1) ^ ((kk >> 1 & 1) * 5)) & (R / 16 - 1);
             return kk * kRowBytes + (((n >> 4) ^ g) << 5) + (n & 15) * 2;
         }
-        return kk * kRowBytes + ((n ^ ((kk >> 2 & 1) << 5)) << 2);
+        return kk * kRowBytes + ((n ^ (R > 32 ? (kk >> 2 & 1) << 5 : 0)) << 2);
     }
 
     // a new segment: where its memory is, and this thread's offsets
@@ -354,11 +356,13 @@ template <class T, int ORDER, int R> struct Tile {
                 off[i] = (unsigned)(r * ld * (long)sizeof(T)) + (tid & 7) * 16;
             }
         } else {
-            const long n = min((long)pos, max(outer - E, 0l));
+            // (a tile that keeps less than a chunk starts reading that much before its own first column)
+            const long before = narrow ? 0 : max(E - outer, 0l), n = min((long)pos, max(outer - E, -before));
             shift = (int)(pos - n);
+            base -= before * (long)sizeof(T);
 #pragma unroll
             for (int i = 0; i < kChunks; ++i)
-                off[i] = (unsigned)(((tid / kPerRow + i * (kThreads / kPerRow)) * ld + n) * (long)sizeof(T));
+                off[i] = (unsigned)(((tid / kPerRow + i * (kThreads / kPerRow)) * ld + n + before) * (long)sizeof(T));
         }
     }
 
@@ -368,7 +372,7 @@ template <class T, int ORDER, int R> struct Tile {
         const long k0 = kt * BK;
         const char *at = base + (ORDER == kInner ? k0 : k0 * ld) * (long)sizeof(T);
         const bool tail = k0 + BK > k;
-        if ((ORDER == kInner ? k : outer) < E) {              // (uniform) under one chunk wide
+        if (narrow) {
             load_elements(at, k - k0, tid);
             return;
         }
@@ -686,9 +690,9 @@ __global__ __launch_bounds__(kThreads) void product_kernel(const Args p)
 
     Tile<T, ORDER_A, BM> ta;
     Tile<T, ORDER_B, kCols> tb[GATED ? 2 : 1];                 // GATED: the gate half, the up half
-    ta.init(p.m - m0, tid);
+    ta.init(p.m - m0, p.m, p.k, tid);
 #pragma unroll
-    for (int g = 0; g < (GATED ? 2 : 1); ++g) tb[g].init(p.n - n0, tid);
+    for (int g = 0; g < (GATED ? 2 : 1); ++g) tb[g].init(p.n - n0, p.n, p.k, tid);
 
     int am[TM], bn[TN];
 #pragma unroll
@@ -837,6 +841,7 @@ template <class T> int launch_product(Args p, int order_a, int order_b, bool gat
 extern template int launch_product<float>(Args, int, int, bool, const Plan &, float *, hipStream_t);
 extern template int launch_product<__bf16>(Args, int, int, bool, const Plan &, float *, hipStream_t);
 extern template int launch_product<_Float16>(Args, int, int, bool, const Plan &, float *, hipStream_t);
+extern template int launch_wide<float>(const Args &, int, int, bool, int, int, long, hipStream_t);
 extern template int launch_wide<__bf16>(const Args &, int, int, bool, int, int, long, hipStream_t);
 extern template int launch_wide<_Float16>(const Args &, int, int, bool, int, int, long, hipStream_t);
 extern template int launch_few<float>(const Args &, int, bool, int, int, hipStream_t);
@@ -895,10 +900,8 @@ template <class T> int launch_product(Args p, int order_a, int order_b, bool gat
     const long blocks = p.mt * p.nt * p.splits * p.batch;
     if (blocks > 0x7fffffffl) return fail(FPN_E_UNSUPPORTED, "a product of %ld workgroups", blocks);
     int rc;
-    if (plan.wide) {
-        if constexpr (sizeof(T) == 2) rc = launch_wide<T>(p, order_a, order_b, gated, plan.bm, plan.bn, blocks, stream);
-        else return fail(FPN_E_UNSUPPORTED, "no wide kernel for this type");
-    } else if (plan.bm == 128) rc = launch_tiles<T, 128, 128, 2, 2>(p, order_a, order_b, gated, blocks, stream);
+    if (plan.wide) rc = launch_wide<T>(p, order_a, order_b, gated, plan.bm, plan.bn, blocks, stream);
+    else if (plan.bm == 128) rc = launch_tiles<T, 128, 128, 2, 2>(p, order_a, order_b, gated, blocks, stream);
     else rc = launch_tiles<T, 64, 128, 2, 2>(p, order_a, order_b, gated, blocks, stream);
     if (rc != FPN_OK || !p.partial) return rc;
     return launch_join<T>(p, gated, stream);

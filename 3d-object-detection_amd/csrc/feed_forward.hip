@@ -167,6 +167,7 @@ int run_product(int dtype, const Args &p, int order_a, int order_b, bool gated, 
     return launch_product<_Float16>(p, order_a, order_b, gated, plan, partial, stream);
 }
 
+constexpr int kStretchBytes = 64;             // of k per stage of the wide kernel
 constexpr long kMostLd = (1l << 21) - 1;      // a tile's byte offsets inside an operand are 32 bits
 
 int check_common(int dtype, long rows, int cin, int cout, int activation)
@@ -285,26 +286,40 @@ int run_column_join(int dtype, int n, int blocks, const float *sums, void *const
 
 namespace {
 
-// The time of a launch of `tiles` workgroups of one shape, in us, from what these took on a 256-CU chip at 8192 x 4096 x 4096,
-// 4096 x 2048 x 2048, 2048 x 2048 x 2048 and 1024 x 4096 x 4096 (bf16): a stage of 32 k with the shape's number of workgroups on
-// every CU, one with half as many, and what a round of workgroups costs besides (first loads, epilogue).
-struct Pace { int bm, bn, per_cu; double stage, half, round; };
+// The time of a launch of `tiles` workgroups of one shape, in us, from what these took on a 256-CU chip: a stage of k (32
+// sixteen-bit elements, 16 floats) with workgroups on few CUs, with one on every CU and with `per_cu` on every CU - the
+// sixteen-bit shapes share the L2's bandwidth, 50 bytes/ns and CU -, and what a round of workgroups costs besides (first loads,
+// epilogue).  Measured against predicted, bf16, us:   large  medium  small  tiny
+//   8192 x 4096 x 4096                                 239     276    311   502
+//   4096 x 2048 x 2048                                  53      44     45    64
+//   2048 x 2048 x 2048                                  48      36     26    35
+//   1024 x 1024 x 1024                                  29      21     14    11
+//   4096 x 8192 x 1024, k split by 1 / 2 / 4    146/108/85 104/92/99 80/96/106 124/150/152
+struct Pace { int bm, bn, per_cu; double few, one, full, round; };
 constexpr Pace kWide[] = {
-    {256, 256, 1, 0.88, 0.88, 8.0},        // 235 us at 8192 x 4096 x 4096 (medium 270, small 306)
-    {256, 128, 2, 1.00, 0.58, 6.0},        // 43 us at 4096 x 2048 x 2048 (large 52, small 44)
-    {128, 128, 2, 0.64, 0.34, 4.0},        // 26 us at 2048 x 2048 x 2048 (large 46, medium 35)
+    {256, 256, 1, 0.50, 0.88, 0.88, 8.0},
+    {256, 128, 2, 0.36, 0.58, 1.00, 6.0},
+    {128, 128, 2, 0.28, 0.31, 0.62, 5.0},
+    {64, 64, 4, 0.20, 0.22, 0.48, 3.0},
+};
+// fp32: bound by its matrix rate, so the smallest tiles that keep it fed (us: small 264, tiny 263 at 1024 x 4096 x 4096,
+// 71 and 42 at 1024 x 1024 x 1024, 104 and 130 at 131072 x 128 x 256)
+constexpr Pace kWideF32[] = {
+    {128, 128, 2, 1.00, 1.08, 2.00, 6.0},
+    {64, 64, 4, 0.55, 0.60, 1.20, 3.0},
 };
 
 double launch_time(const Pace &p, long tiles, double stages, int cus)
 {
     const long at_once = (long)cus * p.per_cu, rounds = tiles / at_once, rest = tiles - rounds * at_once;
-    double us = rounds * (p.stage * stages + p.round);
-    if (rest) us += (rest > cus ? p.stage : p.half) * stages + p.round;
+    double us = rounds * (p.full * stages + p.round);
+    if (rest > cus) us += (p.one + (p.full - p.one) * ((rest - 1) / cus) / (p.per_cu - 1)) * stages + p.round;
+    else if (rest) us += (p.few + (p.one - p.few) * rest / cus) * stages + p.round;
     return us;
 }
 
-// writing and reading the partial sums of a split (3 GB/ms as a join reaches it), and the join's launch
-double join_time(double bytes) { return bytes > 0 ? 4.0 + bytes / 1.5e6 : 0.0; }
+// writing and reading the partial sums of a split, and the join's launch
+double join_time(double bytes) { return 4.0 + bytes / 4e6; }
 
 }  // namespace
 
@@ -337,19 +352,21 @@ Plan make_plan(int dtype, long m, int n, long k, int segs, int batch, bool gated
         p.partial_bytes = p.splits > 1 ? (size_t)(plane * p.splits) : 0;
         return p;
     }
-    if (dtype != FPN_F32 && aligned && m > 0) {
-        const long full = k / 32 * segs;
+    if (aligned && m > 0) {
+        const long full = k / (kStretchBytes / element_size(dtype)) * segs;
         double best = 0;
-        for (const Pace &s : kWide)
+        const Pace *const first = dtype == FPN_F32 ? kWideF32 : kWide;
+        const Pace *const last = first + (dtype == FPN_F32 ? sizeof kWideF32 : sizeof kWide) / sizeof(Pace);
+        for (const Pace *q = first; q < last; ++q)
             for (long splits = 1; splits <= 256; splits *= 2) {
                 const long each = std::max(1l, (full + splits - 1) / splits);
                 if (splits > 1 && (each < 8 || plane * splits > kMostPartial)) break;
-                const double us = launch_time(s, tiles(s.bm, s.bn) * splits, (double)each, cus) + (splits > 1 ? join_time(plane * splits) : 0);
+                const double us = launch_time(*q, tiles(q->bm, q->bn) * splits, (double)each, cus) + (splits > 1 ? join_time(plane * splits) : 0);
                 if (!p.wide || us < best) {
                     best = us;
                     p.wide = true;
-                    p.bm = s.bm;
-                    p.bn = s.bn;
+                    p.bm = q->bm;
+                    p.bn = q->bn;
                     p.tiles_per_split = each;
                     p.splits = (int)std::max(1l, (full + each - 1) / each);
                 }
@@ -617,7 +634,7 @@ int fpn_gated_grad(int dtype, long rows, int cin, int cout, int cdown, const voi
         }
         FPN_FF_TRY(run_product(dtype, p, kInner, order_b, false, partial, space.partial, st));
         if (done && g.sums) {
-            const int rows_each = plan.bm == 256 ? 128 : 32;       // (of a wave: 32 TM)
+            const int rows_each = plan.bm == 256 ? 128 : 32;       // (of a wave: 32 TM of feed_forward_wide.h)
             FPN_FF_TRY(run_column_join(dtype, cout, (int)((rows + plan.bm - 1) / plan.bm * (plan.bm / rows_each)), g.sums, sums_out, st));
         }
     }

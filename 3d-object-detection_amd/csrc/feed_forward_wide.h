@@ -18,19 +18,20 @@
 namespace fpn {
 namespace ff {
 
-constexpr int kWideK = 32;                                  // k per stage
+constexpr int kStretch = 64;                                // bytes of k per stage: 32 sixteen-bit elements, 16 floats
 // A shape of workgroup: BM x BN tile, WM x WN waves of TM x TN MFMA tiles, stages of 32 k in LDS, workgroups per CU.
 template <int BM_, int BN_, int WM_, int WN_, int STAGES, int PER_CU> struct Shape {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, kStages = STAGES;
     static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves, TM = BM / WM / 32, TN = BN / WN / 32;
-    static constexpr int kStage = (BM + BN) * kWideK * 2;            // bytes: BM rows of a, BN of b
-    static constexpr int kPerSimd = kWaves * PER_CU / 4;
+    static constexpr int kStage = (BM + BN) * kStretch;            // bytes: BM rows of a, BN of b
+    static constexpr int kPerSimd = kWaves * PER_CU / 4;               // waves
     static constexpr int kEpilogueBytes = epilogue_bytes(TN);
     static constexpr int kBytes = std::max(kStages * kStage, kWaves * kEpilogueBytes);
 };
 using Large = Shape<256, 256, 2, 4, 4, 1>;
 using Medium = Shape<256, 128, 2, 2, 3, 2>;
 using Small = Shape<128, 128, 4, 2, 4, 2>;
+using Tiny = Shape<64, 64, 2, 1, 4, 4>;
 
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"             // (m0 is reserved: nothing here indexes registers through it)
@@ -65,8 +66,9 @@ __device__ inline unsigned lds_address(const char *p)
 // chunks of row r permuted by r >> 2 & 3; kOuter 2 or 4 rows (k) of R elements, permuted as in Tile.  The permutation is on
 // the source side: the lane that fills a slot fetches the chunk that belongs there.
 template <class T, int ORDER, int R, int WAVES> struct Stream {
-    static constexpr int kPer = R * 64 / 1024 / WAVES; // requests per wave
-    static constexpr int kRowBytes = R * 2;                 // kOuter
+    static constexpr int E = Type<T>::kE, BK = kStretch / (int)sizeof(T);
+    static constexpr int kPer = R * kStretch / 1024 / WAVES;    // requests per wave
+    static constexpr int kRowBytes = R * (int)sizeof(T);        // kOuter
     const char *base;                                       // uniform: k = 0 of the segment
     const char *next;                                       // the stage to be requested next
     long step;                                              // bytes between stages
@@ -78,26 +80,26 @@ template <class T, int ORDER, int R, int WAVES> struct Stream {
         const int q = wave * kPer + i;
         if (ORDER == kInner) {
             row = q * 16 + (lane >> 2);
-            first = ((lane & 3) ^ (row >> 2 & 3)) * 8;
+            first = ((lane & 3) ^ (row >> 2 & 3)) * E;
         } else {
             constexpr int kLanes = kRowBytes / 16;
             row = q * (64 / kLanes) + lane / kLanes;
-            const int g = (((row & 1) << 1) ^ ((row >> 1 & 1) * 5)) & (R / 16 - 1);
-            first = ((lane % kLanes >> 1) ^ g) * 16 + (lane & 1) * 8;
+            // (the place whose image is the slot: both permutations are their own inverses)
+            first = (int)(Tile<T, kOuter, R>::outer_at(row, lane % kLanes * E) - row * kRowBytes) / (int)sizeof(T);
         }
     }
 
-    // (widths along kOuter rows are multiples of 8; chunks beyond the end repeat the last, rows likewise)
+    // (widths along kOuter rows are whole chunks; chunks beyond the end repeat the last, rows likewise)
     __device__ void init(const void *p, long ld, long start, long left, int wave, int lane)
     {
-        base = reinterpret_cast<const char *>(p) + (ORDER == kInner ? start * ld : start) * 2;
-        step = (ORDER == kInner ? 1 : ld) * kWideK * 2;
+        base = reinterpret_cast<const char *>(p) + (ORDER == kInner ? start * ld : start) * (long)sizeof(T);
+        step = (ORDER == kInner ? 1 : ld) * BK * (long)sizeof(T);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             int row, first;
             slot(i, wave, lane, row, first);
-            if (ORDER == kInner) off[i] = (unsigned)((min((long)row, left - 1) * ld + first) * 2);
-            else off[i] = (unsigned)((row * ld + min((long)first, left - 8)) * 2);
+            if (ORDER == kInner) off[i] = (unsigned)((min((long)row, left - 1) * ld + first) * (long)sizeof(T));
+            else off[i] = (unsigned)((row * ld + min((long)first, left - E)) * (long)sizeof(T));
         }
     }
 
@@ -112,15 +114,15 @@ template <class T, int ORDER, int R, int WAVES> struct Stream {
         for (int i = 0; i < kPer; ++i) {
             int row, first;
             slot(i, wave, lane, row, first);
-            const int inside = ORDER == kInner ? left_k - first : (row < left_k ? 8 : 0);
+            const int inside = ORDER == kInner ? left_k - first : (row < left_k ? E : 0);
             uintx4 v = {0, 0, 0, 0};
-            if (inside >= 8) {
+            if (inside >= E) {
                 v = *reinterpret_cast<const uintx4_u *>(at + off[i]);
             } else if (inside > 0) {
-                typedef T vec __attribute__((ext_vector_type(8)));
+                typedef T vec __attribute__((ext_vector_type(E)));
                 vec e;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) e[j] = j < inside ? reinterpret_cast<const T *>(at + off[i])[min(j, inside - 1)] : (T)0.f;
+                for (int j = 0; j < E; ++j) e[j] = j < inside ? reinterpret_cast<const T *>(at + off[i])[min(j, inside - 1)] : (T)0.f;
                 v = __builtin_bit_cast(uintx4, e);
             }
             *reinterpret_cast<uintx4 *>(lds + (wave * kPer + i) * 1024 + lane * 16) = v;
@@ -130,7 +132,7 @@ template <class T, int ORDER, int R, int WAVES> struct Stream {
 
 // A lane's operands of TILES 32-row groups, 16 of k at a time
 template <class T, int ORDER, int R, int TILES> struct StreamReader {
-    static constexpr int kRowBytes = R * 2;
+    static constexpr int kRowBytes = R * (int)sizeof(T);
     unsigned at[ORDER == kInner ? 2 : TILES];
 
     __device__ void init(const int (&first)[TILES], int lane)
@@ -142,13 +144,20 @@ template <class T, int ORDER, int R, int TILES> struct StreamReader {
         } else {
 #pragma unroll
             for (int t = 0; t < TILES; ++t)
-                at[t] = Tile<T, kOuter, R>::outer_at(8 * h + (lane >> 2 & 3), first[t] + (lane & 16) + 4 * (lane & 3));
+                at[t] = sizeof(T) == 2 ? Tile<T, kOuter, R>::outer_at(8 * h + (lane >> 2 & 3), first[t] + (lane & 16) + 4 * (lane & 3))
+                                       : Tile<T, kOuter, R>::outer_at(4 * h, first[t] + l31);
         }
     }
 
     __device__ uintx4 frag(const char *lds, int first, int t, int s) const
     {
         if (ORDER == kInner) return *reinterpret_cast<const uintx4 *>(lds + at[s] + first * 64);
+        if (sizeof(T) == 4) {
+            uintx4 f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[j] = *reinterpret_cast<const unsigned *>(lds + at[t] + (8 * s + j) * kRowBytes);
+            return f;
+        }
         typedef __attribute__((address_space(3))) shortx4 lds_vec;
         const char *p = lds + at[t] + s * 16 * kRowBytes;
         const uintx2 lo = __builtin_bit_cast(uintx2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_vec *)(p)));
@@ -165,7 +174,7 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void wide_product_kernel(
     extern __shared__ char lds[];
     constexpr bool GATED = MODE == kGatedMode;
     constexpr int kWaves = S::kWaves, kStages = S::kStages, kStage = S::kStage, kTM = S::TM, kTN = S::TN, BM = S::BM;
-    constexpr int kHalves = GATED ? 2 : 1, kCols = S::BN / kHalves, kABytes = BM * kWideK * 2, kHalfBytes = kCols * kWideK * 2;
+    constexpr int kHalves = GATED ? 2 : 1, kCols = S::BN / kHalves, kABytes = BM * kStretch, kHalfBytes = kCols * kStretch;
     // (where a half of b is less than a request per wave, half of the waves request each)
     constexpr bool kDealt = GATED && kHalfBytes / 1024 < kWaves;
     constexpr int kStreams = kDealt ? 1 : kHalves, kWavesB = kDealt ? kWaves / 2 : kWaves;
@@ -195,12 +204,12 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void wide_product_kernel(
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-    const long full = p.k / kWideK;                         // whole stages of a segment
+    Stream<T, ORDER_A, BM, kWaves> sa;
+    Stream<T, ORDER_B, kCols, kWavesB> sb[kStreams];
+    const long full = p.k / decltype(sa)::BK;               // whole stages of a segment
     const long first = at.split * p.tiles_per_split, last = min(first + p.tiles_per_split, full * p.segs);
     const unsigned lds0 = lds_address(lds);
 
-    Stream<T, ORDER_A, BM, kWaves> sa;
-    Stream<T, ORDER_B, kCols, kWavesB> sb[kStreams];
     auto segment = [&](int s) {
         sa.init(p.a[s], p.lda[s], m0, p.m - m0, wave, lane);
         if (kDealt) {
@@ -305,7 +314,7 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void wide_product_kernel(
             arrive<0>();
         }
         // what is left of k, with the last split
-        const int left = (int)(p.k - full * kWideK);
+        const int left = (int)(p.k - full * decltype(sa)::BK);
         if (left && at.split == p.splits - 1) {
             __syncthreads();
             sa.put_tail(lds, full, left, wave, lane);
@@ -354,9 +363,12 @@ template <class T, class S> int launch_shape(const Args &p, int order_a, int ord
 
 template <class T> int launch_wide(const Args &p, int order_a, int order_b, bool gated, int bm, int bn, long blocks, hipStream_t stream)
 {
-    if (bn == 256) return launch_shape<T, Large>(p, order_a, order_b, gated, blocks, stream);
-    if (bm == 256) return launch_shape<T, Medium>(p, order_a, order_b, gated, blocks, stream);
-    return launch_shape<T, Small>(p, order_a, order_b, gated, blocks, stream);
+    if constexpr (sizeof(T) == 2) {                         // (fp32 is bound by its matrix rate with any tile)
+        if (bn == 256) return launch_shape<T, Large>(p, order_a, order_b, gated, blocks, stream);
+        if (bm == 256) return launch_shape<T, Medium>(p, order_a, order_b, gated, blocks, stream);
+    }
+    if (bm == 128) return launch_shape<T, Small>(p, order_a, order_b, gated, blocks, stream);
+    return launch_shape<T, Tiny>(p, order_a, order_b, gated, blocks, stream);
 }
 
 }  // namespace ff
