@@ -42,6 +42,8 @@ struct Args {
     long k;                     // length of one k segment
     int segs;                   // 1, or 2: the sum runs over (a[0],b[0]) and then (a[1],b[1])
     int batch;                  // 1, or 2: separate products a[0] b[i] -> c[i]
+    long load_m;                // what may be read of kOuter operands' rows: m and n, or more where rows are padded
+    int load_n;
     const void *a[2], *b[2];    // b: [segment], [batch member], or gate and up where GATED
     long lda[2], ldb[2];        // elements between two rows of memory
     const void *bias[2];

@@ -21,7 +21,8 @@ struct GradArgs {
     const float *pre[2];     // null where the activation is the identity
     long ldp;
     int act;
-    void *d[2];              // (rows, n) dense, or null: column sums only
+    void *d[2];              // (rows, n), or null: column sums only
+    long ldd;
     float *sums;             // (gridDim.y, 1 or 2, n), or null
     long rows_per_block;
 };
@@ -57,8 +58,8 @@ template <class T, class DY, bool GATED> __global__ __launch_bounds__(kThreads) 
                     sum[0][i] += d[i];
                 }
                 if (p.d[0]) {
-                    store8(reinterpret_cast<T *>(p.d[0]) + m * p.n + n, left, d);
-                    if (GATED) store8(reinterpret_cast<T *>(p.d[1]) + m * p.n + n, left, du);
+                    store8(reinterpret_cast<T *>(p.d[0]) + m * p.ldd + n, left, d);
+                    if (GATED) store8(reinterpret_cast<T *>(p.d[1]) + m * p.ldd + n, left, du);
                 }
             }
         });
@@ -130,6 +131,36 @@ int launch_grad(GradArgs p, bool gated, bool dy_float, void *const (&sums_out)[2
     return launch_column_join<T>(p.n, gy, gated, p.sums, sums_out, stream);
 }
 
+// ---- copies of operands whose rows do not consist of whole 16-byte chunks ------------------------------------------
+//
+// Such rows cannot be brought straight into LDS, and reading them at their own alignment costs the load path several
+// passes per instruction.  Where there is enough to multiply they are copied once, rows padded with zeros to whole chunks
+// (a dense product of 1999 x 1091 x 515 fp16: 28 us without, XX with).
+struct CopyArgs {
+    struct { const void *from; void *to; long rows, ld, ldto; int cols; } of[3];
+};
+
+template <class T> __global__ __launch_bounds__(kThreads) void copy_kernel(const CopyArgs p)
+{
+    constexpr int E = Type<T>::kE;
+    const auto &o = p.of[blockIdx.y];
+    const long chunks = o.ldto / E, all = o.rows * chunks;
+    for (long i = (long)blockIdx.x * kThreads + threadIdx.x; i < all; i += (long)gridDim.x * kThreads) {
+        const long row = i / chunks;
+        const int first = (int)(i - row * chunks) * E, inside = o.cols - first;
+        const T *from = reinterpret_cast<const T *>(o.from) + row * o.ld + first;
+        typedef T vec __attribute__((ext_vector_type(E)));
+        vec v;
+        if (inside >= E) {
+            v = __builtin_bit_cast(vec, (uintx4)*reinterpret_cast<const uintx4_u *>(from));
+        } else {
+#pragma unroll
+            for (int j = 0; j < E; ++j) v[j] = j < inside ? from[j] : (T)0.f;
+        }
+        *reinterpret_cast<vec *>(reinterpret_cast<T *>(o.to) + row * o.ldto + first) = v;
+    }
+}
+
 // ---- host side --------------------------------------------------------------------------------------------------
 
 int element_size(int dtype) { return dtype == FPN_F32 ? 4 : 2; }
@@ -151,9 +182,9 @@ Plan plan_of(int dtype, const Args &p, int order_a, int order_b, bool gated)
 {
     bool aligned = true;
     for (int i = 0; i < p.segs; ++i)
-        aligned = aligned && whole_chunks(p.a[i], order_a == kInner && p.m == 1 ? 0 : p.lda[i], order_a, p.m, element_size(dtype));
+        aligned = aligned && whole_chunks(p.a[i], order_a == kInner && p.m == 1 ? 0 : p.lda[i], order_a, p.load_m, element_size(dtype));
     for (int i = 0; i < std::max({p.segs, p.batch, gated ? 2 : 1}); ++i)
-        aligned = aligned && whole_chunks(p.b[i], p.ldb[i], order_b, p.n, element_size(dtype));
+        aligned = aligned && whole_chunks(p.b[i], p.ldb[i], order_b, p.load_n, element_size(dtype));
     return plan_product(dtype, p.m, p.n, p.k, p.segs, p.batch, gated, aligned, order_a, order_b);
 }
 
@@ -211,21 +242,91 @@ int check_workspace(const void *ws, size_t have, size_t need)
 // The parts of a backward pass' workspace: dpre (one matrix, or two where gated), the workgroups' column sums, and
 // the partial sums of dx and dw, which run one after the other
 struct GradSpace {
-    size_t d, sums, dh, partial, total;
+    size_t d, sums, dh, partial, copies, total;
 };
-// (down: the width of the block's result where dh is formed from its gradient, else 0)
-GradSpace grad_space(int dtype, long rows, int cin, int n, bool gated, bool with_d, int down = 0)
+// a row length in whole chunks
+long padded(int dtype, long cols)
+{
+    const int e = 16 / element_size(dtype);
+    return (cols + e - 1) / e * e;
+}
+
+// whether operands with ragged rows are copied: a copy's launch and traffic (4 us and more) against what the pipelined
+// kernel saves, which takes half the time from about 10^8 operations on
+bool worth_copies(long rows, int cin, int cout) { return rows > 64 && cin >= 64 && cout >= 64 && 2.0 * rows * cin * cout >= 1e8; }
+
+// the bytes of copies of a matrix in either storage order
+size_t copy_bytes(int dtype, long rows, long cols) { return align256((size_t)rows * padded(dtype, cols) * element_size(dtype)); }
+size_t weight_copy_bytes(int dtype, int cin, int cout) { return std::max(copy_bytes(dtype, cin, cout), copy_bytes(dtype, cout, cin)); }
+
+// A matrix of a call, which may be replaced by its copy.  `wide`: what may be read of its rows.
+struct Matrix {
+    const void *p;
+    long ld, rows;
+    int cols;
+    long wide;
+};
+
+// Collects the copies that a call makes, and makes them in one launch
+struct Copies {
+    CopyArgs args = {};
+    int count = 0;
+    char *at;
+    size_t left;
+    int dtype;
+
+    Copies(int dtype_, void *space, size_t bytes) : at(reinterpret_cast<char *>(space)), left(space ? bytes : 0), dtype(dtype_) {}
+
+    // outer: the matrix is read along its rows' direction in chunks (kOuter), so that its width counts too
+    void take(Matrix &m, bool outer)
+    {
+        const int e = element_size(dtype);
+        if (reinterpret_cast<uintptr_t>(m.p) % 16 == 0 && m.ld * e % 16 == 0 && (!outer || m.wide * e % 16 == 0)) return;
+        const size_t bytes = copy_bytes(dtype, m.rows, m.cols);
+        if (bytes > left || count == 3) return;                        // (no room: the kernel that reads any rows takes it)
+        const long ld = padded(dtype, m.cols);
+        args.of[count++] = {m.p, at, m.rows, m.ld, ld, m.cols};
+        m = {at, ld, m.rows, m.cols, ld};
+        at += bytes;
+        left -= bytes;
+    }
+
+    int make(hipStream_t stream)
+    {
+        if (!count) return FPN_OK;
+        long most = 0;
+        for (int i = 0; i < count; ++i) most = std::max(most, args.of[i].rows * args.of[i].ldto);
+        const long blocks = std::min(2048l, (most * element_size(dtype) / 16 + kThreads - 1) / kThreads);
+        const dim3 grid((unsigned)blocks, count);
+        if (dtype == FPN_F32) hipLaunchKernelGGL((copy_kernel<float>), grid, dim3(kThreads), 0, stream, args);
+        else if (dtype == FPN_BF16) hipLaunchKernelGGL((copy_kernel<__bf16>), grid, dim3(kThreads), 0, stream, args);
+        else hipLaunchKernelGGL((copy_kernel<_Float16>), grid, dim3(kThreads), 0, stream, args);
+        return check_launch("copy of ragged operands");
+    }
+};
+
+Matrix weights(const void *p, long ld, int cin, int cout, int transposed)
+{
+    return transposed ? Matrix{p, ld, cout, cin, cin} : Matrix{p, ld, cin, cout, cout};
+}
+
+// (down: the width of the block's result where dh is formed from its gradient, else 0; whole: no operand will be copied)
+GradSpace grad_space(int dtype, long rows, int cin, int n, bool gated, bool with_d, bool whole, int down = 0)
 {
     GradSpace s;
     const int planes = gated ? 2 : 1;
-    s.d = with_d ? align256((size_t)rows * n * element_size(dtype)) * planes : 0;
+    s.d = with_d ? align256((size_t)rows * padded(dtype, n) * element_size(dtype)) * planes : 0;
     s.sums = align256((size_t)std::max<long>(grad_rows_grid(rows, n), down ? (rows + 255) / 256 * 8 : 0) * planes * n * sizeof(float));
     s.dh = down ? align256((size_t)rows * n * sizeof(float)) : 0;
     s.partial = align256(std::max({partial_bytes(dtype, rows, cin, n, planes, 1, false, kInner),
                                    partial_bytes(dtype, cin, n, rows, 1, planes, false, kOuter),
                                    partial_bytes(dtype, n, cin, rows, 1, 1, false, kOuter)}));
     if (down) s.partial = std::max(s.partial, align256(partial_bytes(dtype, rows, n, down, 1, 1, false, kInner)));
-    s.total = s.d + s.sums + s.dh + s.partial;
+    s.copies = 0;
+    if (!whole && worth_copies(rows, cin, n))
+        s.copies = copy_bytes(dtype, rows, cin) + planes * weight_copy_bytes(dtype, cin, n) + (with_d ? 0 : copy_bytes(dtype, rows, n));
+    if (!whole && down && worth_copies(rows, down, n)) s.copies += copy_bytes(dtype, rows, down) + weight_copy_bytes(dtype, n, down);
+    s.total = s.d + s.sums + s.dh + s.partial + s.copies;
     return s;
 }
 
@@ -238,34 +339,51 @@ Args product(long m, int n, long k)
     p.segs = 1;
     p.batch = 1;
     p.act = FPN_ACT_NONE;
+    p.load_m = m;
+    p.load_n = n;
     return p;
 }
 
 // dw = x^T d for one or two d, in the weights' own storage order
-int weight_gradients(int dtype, long rows, int cin, int n, const void *x, long ldx, const void *const (&d)[2], long ldd, int members,
-                     void *const (&dw)[2], long lddw, int transposed, float *partial, size_t partial_bytes, hipStream_t stream)
+int weight_gradients(int dtype, const Matrix &x, const Matrix (&d)[2], int members, void *const (&dw)[2], long lddw, int transposed,
+                     float *partial, size_t partial_bytes, hipStream_t stream)
 {
     if (!transposed) {
-        Args p = product(cin, n, rows);
-        p.a[0] = x;
-        p.lda[0] = ldx;
+        Args p = product(x.cols, d[0].cols, x.rows);
+        p.load_m = x.wide;
+        p.load_n = (int)d[0].wide;
+        p.a[0] = x.p;
+        p.lda[0] = x.ld;
         p.batch = members;
-        for (int i = 0; i < members; ++i) { p.b[i] = d[i]; p.ldb[i] = ldd; p.c[i] = dw[i]; }
+        for (int i = 0; i < members; ++i) { p.b[i] = d[i].p; p.ldb[i] = d[i].ld; p.c[i] = dw[i]; }
         p.ldc = lddw;
         return run_product(dtype, p, kOuter, kOuter, false, partial, partial_bytes, stream);
     }
     // held (out,in): the operands change places (one product each, x is the b side of both)
     for (int i = 0; i < members; ++i) {
-        Args p = product(n, cin, rows);
-        p.a[0] = d[i];
-        p.lda[0] = ldd;
-        p.b[0] = x;
-        p.ldb[0] = ldx;
+        Args p = product(d[i].cols, x.cols, x.rows);
+        p.load_m = d[i].wide;
+        p.load_n = (int)x.wide;
+        p.a[0] = d[i].p;
+        p.lda[0] = d[i].ld;
+        p.b[0] = x.p;
+        p.ldb[0] = x.ld;
         p.c[0] = dw[i];
         p.ldc = lddw;
         FPN_FF_TRY(run_product(dtype, p, kOuter, kOuter, false, partial, partial_bytes, stream));
     }
     return FPN_OK;
+}
+
+// the operands of a forward product (or two, gated)
+void set_operands(Args &p, const Matrix &x, const Matrix *w, int count)
+{
+    p.a[0] = x.p;
+    p.lda[0] = x.ld;
+    for (int i = 0; i < count; ++i) {
+        p.b[i] = w[i].p;
+        p.ldb[i] = w[i].ld;
+    }
 }
 
 int run_grad(int dtype, const GradArgs &p, bool gated, bool dy_float, void *const (&sums_out)[2], hipStream_t stream)
@@ -413,10 +531,12 @@ using namespace fpn::ff;
 
 extern "C" {
 
-size_t fpn_dense_workspace_bytes(int dtype, long rows, int cin, int cout)
+size_t fpn_dense_workspace_bytes(int dtype, long rows, int cin, int cout, int whole)
 {
     if (check_common(dtype, rows, cin, cout, FPN_ACT_NONE) != FPN_OK) return 0;
-    return partial_bytes(dtype, rows, cout, cin, 1, 1, false, kInner);
+    const size_t partial = partial_bytes(dtype, rows, cout, cin, 1, 1, false, kInner);
+    if (whole || !worth_copies(rows, cin, cout)) return partial;
+    return align256(partial) + copy_bytes(dtype, rows, cin) + weight_copy_bytes(dtype, cin, cout);
 }
 
 int fpn_dense(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w, long ldw, int w_transposed,
@@ -432,11 +552,23 @@ int fpn_dense(int dtype, long rows, int cin, int cout, const void *x, long ldx, 
     if (residual) FPN_FF_TRY(check_matrix("residual", residual, ldr, cout, dtype, true));
     if (pre) FPN_FF_TRY(check_matrix("pre", pre, ldp, cout, FPN_F32));
     FPN_FF_TRY(check_workspace(workspace, workspace_bytes, 0));
+    const int order_b = w_transposed ? kInner : kOuter;
+    const hipStream_t st = as_stream(stream);
+    Matrix mx = {x, ldx, rows, cin, cin}, mw = weights(w, ldw, cin, cout, w_transposed);
+    size_t partial_space = workspace_bytes;
+    if (worth_copies(rows, cin, cout)) {
+        const size_t partial = align256(partial_bytes(dtype, rows, cout, cin, 1, 1, false, kInner));
+        if (workspace && workspace_bytes > partial) {
+            Copies copies(dtype, reinterpret_cast<char *>(workspace) + partial, workspace_bytes - partial);
+            copies.take(mx, false);
+            copies.take(mw, order_b == kOuter);
+            FPN_FF_TRY(copies.make(st));
+            partial_space = partial;
+        }
+    }
     Args p = product(rows, cout, cin);
-    p.a[0] = x;
-    p.lda[0] = ldx;
-    p.b[0] = w;
-    p.ldb[0] = ldw;
+    set_operands(p, mx, &mw, 1);
+    if (order_b == kOuter) p.load_n = (int)mw.wide;
     p.bias[0] = bias;
     p.act = activation;
     p.residual = residual;
@@ -445,14 +577,13 @@ int fpn_dense(int dtype, long rows, int cin, int cout, const void *x, long ldx, 
     p.ldc = ldy;
     p.pre[0] = pre;
     p.ldp = ldp;
-    return run_product(dtype, p, kInner, w_transposed ? kInner : kOuter, false, reinterpret_cast<float *>(workspace), workspace_bytes,
-                       as_stream(stream));
+    return run_product(dtype, p, kInner, order_b, false, reinterpret_cast<float *>(workspace), partial_space, st);
 }
 
-size_t fpn_dense_grad_workspace_bytes(int dtype, long rows, int cin, int cout, int activation)
+size_t fpn_dense_grad_workspace_bytes(int dtype, long rows, int cin, int cout, int activation, int whole)
 {
     if (check_common(dtype, rows, cin, cout, activation) != FPN_OK) return 0;
-    return grad_space(dtype, rows, cin, cout, false, activation != FPN_ACT_NONE).total;
+    return grad_space(dtype, rows, cin, cout, false, activation != FPN_ACT_NONE, whole).total;
 }
 
 int fpn_dense_grad(int dtype, long rows, int cin, int cout, const void *dy, long lddy, const void *x, long ldx, const void *w,
@@ -470,14 +601,21 @@ int fpn_dense_grad(int dtype, long rows, int cin, int cout, const void *dy, long
     }
     if (dw) FPN_FF_TRY(check_matrix("dw", dw, lddw, w_transposed ? cin : cout, dtype));
     FPN_FF_TRY(check_vector("dbias", dbias, dtype));
-    const GradSpace space = grad_space(dtype, rows, cin, cout, false, act);
+    // (with a smaller workspace than ragged operands' copies take, the products read them as they are)
+    GradSpace space = grad_space(dtype, rows, cin, cout, false, act, true);
     FPN_FF_TRY(check_workspace(workspace, workspace_bytes, space.total));
     char *ws = reinterpret_cast<char *>(workspace);
     float *partial = reinterpret_cast<float *>(ws + space.d + space.sums + space.dh);
     const hipStream_t st = as_stream(stream);
 
-    const void *d[2] = {dy, nullptr};
-    long ldd = lddy;
+    Matrix mx = {x, ldx, rows, cin, cin}, mw = weights(w, ldw, cin, cout, w_transposed), md[2] = {{dy, lddy, rows, cout, cout}, {}};
+    if (worth_copies(rows, cin, cout)) {
+        Copies copies(dtype, ws + space.total, workspace_bytes - space.total);
+        if (dw) copies.take(mx, true);
+        if (dx) copies.take(mw, w_transposed);
+        if (!act) copies.take(md[0], dw);
+        FPN_FF_TRY(copies.make(st));
+    }
     if (act || dbias) {
         GradArgs g = {};
         g.rows = rows;
@@ -488,9 +626,10 @@ int fpn_dense_grad(int dtype, long rows, int cin, int cout, const void *dy, long
         g.ldp = ldp;
         g.act = activation;
         if (act) {
+            const long ldd = padded(dtype, cout);
             g.d[0] = ws;
-            d[0] = ws;
-            ldd = cout;
+            g.ldd = ldd;
+            md[0] = {ws, ldd, rows, cout, ldd};
         }
         g.sums = dbias ? reinterpret_cast<float *>(ws + space.d) : nullptr;
         void *const out[2] = {dbias, nullptr};
@@ -498,25 +637,25 @@ int fpn_dense_grad(int dtype, long rows, int cin, int cout, const void *dy, long
     }
     if (dx && rows > 0) {
         Args p = product(rows, cin, cout);
-        p.a[0] = d[0];
-        p.lda[0] = ldd;
-        p.b[0] = w;
-        p.ldb[0] = ldw;
+        set_operands(p, md[0], &mw, 1);
+        if (w_transposed) p.load_n = (int)mw.wide;
         p.c[0] = dx;
         p.ldc = lddx;
         FPN_FF_TRY(run_product(dtype, p, kInner, w_transposed ? kOuter : kInner, false, partial, space.partial, st));
     }
     if (dw) {
         void *const out[2] = {dw, nullptr};
-        FPN_FF_TRY(weight_gradients(dtype, rows, cin, cout, x, ldx, d, ldd, 1, out, lddw, w_transposed, partial, space.partial, st));
+        FPN_FF_TRY(weight_gradients(dtype, mx, md, 1, out, lddw, w_transposed, partial, space.partial, st));
     }
     return FPN_OK;
 }
 
-size_t fpn_gated_workspace_bytes(int dtype, long rows, int cin, int cout)
+size_t fpn_gated_workspace_bytes(int dtype, long rows, int cin, int cout, int whole)
 {
     if (check_common(dtype, rows, cin, cout, FPN_ACT_NONE) != FPN_OK) return 0;
-    return partial_bytes(dtype, rows, cout, cin, 1, 1, true, kInner);
+    const size_t partial = partial_bytes(dtype, rows, cout, cin, 1, 1, true, kInner);
+    if (whole || !worth_copies(rows, cin, cout)) return partial;
+    return align256(partial) + copy_bytes(dtype, rows, cin) + 2 * weight_copy_bytes(dtype, cin, cout);
 }
 
 int fpn_gated(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w_gate, long ldg, const void *w_up, long ldu,
@@ -535,13 +674,24 @@ int fpn_gated(int dtype, long rows, int cin, int cout, const void *x, long ldx, 
     if (gate) FPN_FF_TRY(check_matrix("gate", gate, ldp, cout, FPN_F32));
     if (up) FPN_FF_TRY(check_matrix("up", up, ldp, cout, FPN_F32));
     FPN_FF_TRY(check_workspace(workspace, workspace_bytes, 0));
+    const int order_b = w_transposed ? kInner : kOuter;
+    const hipStream_t st = as_stream(stream);
+    Matrix mx = {x, ldx, rows, cin, cin}, mw[2] = {weights(w_gate, ldg, cin, cout, w_transposed), weights(w_up, ldu, cin, cout, w_transposed)};
+    size_t partial_space = workspace_bytes;
+    if (worth_copies(rows, cin, cout)) {
+        const size_t partial = align256(partial_bytes(dtype, rows, cout, cin, 1, 1, true, kInner));
+        if (workspace && workspace_bytes > partial) {
+            Copies copies(dtype, reinterpret_cast<char *>(workspace) + partial, workspace_bytes - partial);
+            copies.take(mx, false);
+            copies.take(mw[0], order_b == kOuter);
+            copies.take(mw[1], order_b == kOuter);
+            FPN_FF_TRY(copies.make(st));
+            partial_space = partial;
+        }
+    }
     Args p = product(rows, cout, cin);
-    p.a[0] = x;
-    p.lda[0] = ldx;
-    p.b[0] = w_gate;
-    p.b[1] = w_up;
-    p.ldb[0] = ldg;
-    p.ldb[1] = ldu;
+    set_operands(p, mx, mw, 2);
+    if (order_b == kOuter) p.load_n = (int)std::min(mw[0].wide, mw[1].wide);
     p.bias[0] = bias_gate;
     p.bias[1] = bias_up;
     p.act = activation;
@@ -550,14 +700,13 @@ int fpn_gated(int dtype, long rows, int cin, int cout, const void *x, long ldx, 
     p.pre[0] = gate;
     p.pre[1] = up;
     p.ldp = ldp;
-    return run_product(dtype, p, kInner, w_transposed ? kInner : kOuter, true, reinterpret_cast<float *>(workspace), workspace_bytes,
-                       as_stream(stream));
+    return run_product(dtype, p, kInner, order_b, true, reinterpret_cast<float *>(workspace), partial_space, st);
 }
 
-size_t fpn_gated_grad_workspace_bytes(int dtype, long rows, int cin, int cout, int cdown)
+size_t fpn_gated_grad_workspace_bytes(int dtype, long rows, int cin, int cout, int cdown, int whole)
 {
     if (check_common(dtype, rows, cin, cout, FPN_ACT_NONE) != FPN_OK || cdown < 0 || cdown > kMostLd) return 0;
-    return grad_space(dtype, rows, cin, cout, true, true, cdown).total;
+    return grad_space(dtype, rows, cin, cout, true, true, whole, cdown).total;
 }
 
 int fpn_gated_grad(int dtype, long rows, int cin, int cout, int cdown, const void *dh, long lddh, const void *w_down, long ldd,
@@ -587,12 +736,31 @@ int fpn_gated_grad(int dtype, long rows, int cin, int cout, int cdown, const voi
     }
     FPN_FF_TRY(check_vector("dbias_gate", dbias_gate, dtype));
     FPN_FF_TRY(check_vector("dbias_up", dbias_up, dtype));
-    const GradSpace space = grad_space(dtype, rows, cin, cout, true, true, cdown);
+    // (with a smaller workspace than ragged operands' copies take, the products read them as they are)
+    const GradSpace space = grad_space(dtype, rows, cin, cout, true, true, true, cdown);
     FPN_FF_TRY(check_workspace(workspace, workspace_bytes, space.total));
     char *ws = reinterpret_cast<char *>(workspace);
     float *partial = reinterpret_cast<float *>(ws + space.d + space.sums + space.dh);
     const hipStream_t st = as_stream(stream);
+    const int order_down = down_transposed ? kOuter : kInner;
 
+    Matrix mx = {x, ldx, rows, cin, cin}, mw[2] = {weights(w_gate, ldg, cin, cout, w_transposed), weights(w_up, ldu, cin, cout, w_transposed)};
+    Matrix mdy = {dh, lddh, rows, cdown, cdown}, mdown = weights(w_down, ldd, cout, cdown, down_transposed);
+    Copies copies(dtype, ws + space.total, workspace_bytes - space.total);
+    if (worth_copies(rows, cin, cout)) {
+        if (dw_gate) copies.take(mx, true);
+        if (dx) copies.take(mw[0], w_transposed);
+        if (dx) copies.take(mw[1], w_transposed);
+        FPN_FF_TRY(copies.make(st));
+    }
+    if (cdown && rows > 0 && worth_copies(rows, cdown, cout)) {
+        Copies more(dtype, copies.at, copies.left);
+        more.take(mdy, false);
+        more.take(mdown, order_down == kOuter);
+        FPN_FF_TRY(more.make(st));
+    }
+
+    const long ldd_own = padded(dtype, cout);
     GradArgs g = {};
     g.rows = rows;
     g.n = cout;
@@ -604,22 +772,21 @@ int fpn_gated_grad(int dtype, long rows, int cin, int cout, int cdown, const voi
     g.act = activation;
     g.d[0] = ws;
     g.d[1] = ws + space.d / 2;
+    g.ldd = ldd_own;
+    const Matrix md[2] = {{g.d[0], ldd_own, rows, cout, ldd_own}, {g.d[1], ldd_own, rows, cout, ldd_own}};
     g.sums = dbias_gate ? reinterpret_cast<float *>(ws + space.d) : nullptr;
     void *const sums_out[2] = {dbias_gate, dbias_up};
     bool done = false;
     if (cdown && rows > 0) {                      // dh = dy w_down^T, never rounded to 16 bits
-        const int order_b = down_transposed ? kOuter : kInner;
         Args p = product(rows, cout, cdown);
-        p.a[0] = dh;
-        p.lda[0] = lddh;
-        p.b[0] = w_down;
-        p.ldb[0] = ldd;
-        const Plan plan = plan_of(dtype, p, kInner, order_b, false);
+        set_operands(p, mdy, &mdown, 1);
+        if (order_down == kOuter) p.load_n = (int)mdown.wide;
+        const Plan plan = plan_of(dtype, p, kInner, order_down, false);
         done = plan.wide && plan.splits == 1;
         if (done) {                               // dg and du straight from the product's epilogue
             p.c[0] = g.d[0];
             p.c[1] = g.d[1];
-            p.ldc = cout;
+            p.ldc = ldd_own;
             p.act = activation;
             p.gate = gate;
             p.up = up;
@@ -632,7 +799,7 @@ int fpn_gated_grad(int dtype, long rows, int cin, int cout, int cdown, const voi
             g.dy = p.c[0];
             g.lddy = cout;
         }
-        FPN_FF_TRY(run_product(dtype, p, kInner, order_b, false, partial, space.partial, st));
+        FPN_FF_TRY(run_product(dtype, p, kInner, order_down, false, partial, space.partial, st));
         if (done && g.sums) {
             const int rows_each = plan.bm == 256 ? 128 : 32;       // (of a wave: 32 TM of feed_forward_wide.h)
             FPN_FF_TRY(run_column_join(dtype, cout, (int)((rows + plan.bm - 1) / plan.bm * (plan.bm / rows_each)), g.sums, sums_out, st));
@@ -642,21 +809,17 @@ int fpn_gated_grad(int dtype, long rows, int cin, int cout, int cdown, const voi
     if (dx && rows > 0) {                         // dg Wg^T + du Wu^T: one sum over both
         Args p = product(rows, cin, cout);
         p.segs = 2;
-        p.a[0] = g.d[0];
-        p.a[1] = g.d[1];
-        p.lda[0] = p.lda[1] = cout;
-        p.b[0] = w_gate;
-        p.b[1] = w_up;
-        p.ldb[0] = ldg;
-        p.ldb[1] = ldu;
+        set_operands(p, md[0], mw, 2);
+        p.a[1] = md[1].p;
+        p.lda[1] = md[1].ld;
+        if (w_transposed) p.load_n = (int)std::min(mw[0].wide, mw[1].wide);
         p.c[0] = dx;
         p.ldc = lddx;
         FPN_FF_TRY(run_product(dtype, p, kInner, w_transposed ? kOuter : kInner, false, partial, space.partial, st));
     }
     if (dw_gate) {
-        const void *const d[2] = {g.d[0], g.d[1]};
         void *const out[2] = {dw_gate, dw_up};
-        FPN_FF_TRY(weight_gradients(dtype, rows, cin, cout, x, ldx, d, cout, 2, out, lddw, w_transposed, partial, space.partial, st));
+        FPN_FF_TRY(weight_gradients(dtype, mx, md, 2, out, lddw, w_transposed, partial, space.partial, st));
     }
     return FPN_OK;
 }

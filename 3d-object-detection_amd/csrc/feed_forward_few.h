@@ -168,7 +168,7 @@ __global__ __launch_bounds__((FewShape<MT, NT, GATED>::kThreads)) void few_produ
     TileB tb[kHalves];
     ta.init(p.a[0], p.lda[0], 0, p.m, lane);
 #pragma unroll
-    for (int g = 0; g < kHalves; ++g) tb[g].init(p.b[g], p.ldb[g], n0, p.n - n0, lane);
+    for (int g = 0; g < kHalves; ++g) tb[g].init(p.b[g], p.ldb[g], n0, (ORDER_B == kOuter ? p.load_n : p.n) - n0, lane);
     const int full = (int)(p.k / BK);                       // (k is a layer's width here: below 2^21)
     const int share = split * kWaves + wave, shares = p.splits * kWaves;
     const int s0 = (int)((long)full * share / shares), len = (int)((long)full * (share + 1) / shares) - s0;

@@ -210,15 +210,16 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void wide_product_kernel(
     const long first = at.split * p.tiles_per_split, last = min(first + p.tiles_per_split, full * p.segs);
     const unsigned lds0 = lds_address(lds);
 
+    const long left_n = (ORDER_B == kOuter ? p.load_n : p.n) - n0;
     auto segment = [&](int s) {
-        sa.init(p.a[s], p.lda[s], m0, p.m - m0, wave, lane);
+        sa.init(p.a[s], p.lda[s], m0, (ORDER_A == kOuter ? p.load_m : p.m) - m0, wave, lane);
         if (kDealt) {
-            sb[0].init(dealt ? p.b[1] : p.b[0], dealt ? p.ldb[1] : p.ldb[0], n0, p.n - n0, wave_b, lane);
+            sb[0].init(dealt ? p.b[1] : p.b[0], dealt ? p.ldb[1] : p.ldb[0], n0, left_n, wave_b, lane);
         } else if (GATED) {
-            sb[0].init(p.b[0], p.ldb[0], n0, p.n - n0, wave, lane);
-            sb[kStreams - 1].init(p.b[1], p.ldb[1], n0, p.n - n0, wave, lane);
+            sb[0].init(p.b[0], p.ldb[0], n0, left_n, wave, lane);
+            sb[kStreams - 1].init(p.b[1], p.ldb[1], n0, left_n, wave, lane);
         } else {
-            sb[0].init(p.b[s + at.member], p.ldb[s + at.member], n0, p.n - n0, wave, lane);
+            sb[0].init(p.b[s + at.member], p.ldb[s + at.member], n0, left_n, wave, lane);
         }
     };
     // request Q of a wave's kPer of a stage

@@ -99,10 +99,10 @@ SIGNATURES = {
 # functions that return a size
 SIZES = {
     "fpn_shared_mlp_workspace_bytes": [_l, _i, _i],
-    "fpn_dense_workspace_bytes": [_i, _l, _i, _i],
-    "fpn_dense_grad_workspace_bytes": [_i, _l, _i, _i, _i],
-    "fpn_gated_workspace_bytes": [_i, _l, _i, _i],
-    "fpn_gated_grad_workspace_bytes": [_i, _l, _i, _i, _i],
+    "fpn_dense_workspace_bytes": [_i, _l, _i, _i, _i],
+    "fpn_dense_grad_workspace_bytes": [_i, _l, _i, _i, _i, _i],
+    "fpn_gated_workspace_bytes": [_i, _l, _i, _i, _i],
+    "fpn_gated_grad_workspace_bytes": [_i, _l, _i, _i, _i, _i],
 }
 
 _lib = None

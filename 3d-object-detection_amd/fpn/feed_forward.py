@@ -139,6 +139,18 @@ def _workspace(size, x):
     return torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
 
 
+def _whole(dtype, widths, *operands):
+    """Whether every operand (tensor, row stride) starts at and moves by whole 16-byte chunks, and so do the widths."""
+    bits = 0
+    for n in widths:
+        bits |= n
+    for t, ld in operands:
+        bits |= ld
+        if t.data_ptr() & 15:
+            return 0
+    return int(bits & (3 if dtype == 0 else 7) == 0)
+
+
 def _p(t):
     """Device pointer of a tensor (None -> NULL)."""
     return None if t is None else t.data_ptr()
@@ -203,7 +215,7 @@ def dense(x, w, bias=None, activation=None, residual=None, out=None, keep=False)
     ldr = _rows("residual", residual, broadcast=True) if residual is not None else 0
     y, ldy = _output(out, x, rows, cout, (("x", x), ("w", w), ("bias", bias)), residual)
     pre = torch.empty((rows, cout), dtype=torch.float32, device=x.device) if keep and act else None
-    size = lib.fpn_dense_workspace_bytes(dtype, rows, cin, cout)
+    size = lib.fpn_dense_workspace_bytes(dtype, rows, cin, cout, _whole(dtype, (cin, cout), (x, ldx), (w, ldw)))
     ws = _workspace(size, x)
     _call(x, lib.fpn_dense, dtype, rows, cin, cout, _p(x), ldx, _p(w), ldw, transposed, _p(bias), act, _p(residual), ldr, _p(y), ldy,
           _p(pre), cout, _p(ws), size)
@@ -233,7 +245,7 @@ def dense_grad(dy, x, w, pre=None, activation=None, bias=False, need_x=True, nee
         dx = torch.empty((rows, cin), dtype=x.dtype, device=x.device) if need_x else None
         dw = _like_weights(w, transposed) if need_w else None
         db = torch.empty(cout, dtype=x.dtype, device=x.device) if bias else None
-    size = lib.fpn_dense_grad_workspace_bytes(dtype, rows, cin, cout, act)
+    size = lib.fpn_dense_grad_workspace_bytes(dtype, rows, cin, cout, act, _whole(dtype, (cin, cout), (x, ldx), (w, ldw), (dy, lddy)))
     ws = _workspace(size, x)
     _call(x, lib.fpn_dense_grad, dtype, rows, cin, cout, _p(dy), lddy, _p(x), ldx, _p(w), ldw, transposed, _p(pre) if act else None, ldp,
           act, _p(dx), cin, _p(dw), cin if transposed else cout, _p(db), _p(ws), size)
@@ -313,7 +325,7 @@ def gated(x, w_gate, w_up, bias_gate=None, bias_up=None, activation="silu", out=
     gate = up = None
     if keep:
         gate, up = (torch.empty((rows, cout), dtype=torch.float32, device=x.device) for _ in range(2))
-    size = lib.fpn_gated_workspace_bytes(dtype, rows, cin, cout)
+    size = lib.fpn_gated_workspace_bytes(dtype, rows, cin, cout, _whole(dtype, (cin, cout), (x, ldx), (w_gate, ldg), (w_up, ldu)))
     ws = _workspace(size, x)
     _call(x, lib.fpn_gated, dtype, rows, cin, cout, _p(x), ldx, _p(w_gate), ldg, _p(w_up), ldu, transposed, _p(bias_gate), _p(bias_up), act,
           _p(h), ldh, _p(gate), _p(up), cout, _p(ws), size)
@@ -346,7 +358,9 @@ def gated_grad(dh, x, w_gate, w_up, gate, up, activation="silu", bias=False, nee
         dx = torch.empty((rows, cin), dtype=x.dtype, device=x.device) if need_x else None
         dwg, dwu = (_like_weights(w_gate, transposed) for _ in range(2)) if need_w else (None, None)
         dbg, dbu = (torch.empty(cout, dtype=x.dtype, device=x.device) for _ in range(2)) if bias else (None, None)
-    size = lib.fpn_gated_grad_workspace_bytes(dtype, rows, cin, cout, cdown)
+    whole = _whole(dtype, (cin, cout, cdown), (x, ldx), (w_gate, ldg), (w_up, ldu), (dh, lddh)) and \
+        (not cdown or _whole(dtype, (), (w_down, ldd)))
+    size = lib.fpn_gated_grad_workspace_bytes(dtype, rows, cin, cout, cdown, int(whole))
     ws = _workspace(size, x)
     _call(x, lib.fpn_gated_grad, dtype, rows, cin, cout, cdown, _p(dh), lddh, _p(w_down), ldd, down_transposed, _p(x), ldx, _p(w_gate),
           ldg, _p(w_up), ldu, transposed, _p(gate), _p(up), ldp, act, _p(dx), cin, _p(dwg), _p(dwu), cin if transposed else cout,

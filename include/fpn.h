@@ -764,7 +764,10 @@ int fpn_detection_records(int b, int n, const float *mask_logits, const float *b
  *   - rows 0 is a valid call: forward writes nothing, weight and bias gradients become 0;
  *   - outputs may not share memory with inputs, except y with residual (same address and stride);
  *   - the workspace (16-byte aligned, at least what the _workspace_bytes function of the same arguments says) belongs
- *     to the call until its work is done: calls that may run at the same time need one each;
+ *     to the call until its work is done: calls that may run at the same time need one each.  `whole` there: nonzero
+ *     if every operand's address, row stride and width (cin, cout, cdown) is a multiple of 16 bytes.  With 0 the size has
+ *     room for copies of ragged operands, which a call makes where that is faster; a workspace of the size for
+ *     whole ones is enough for any call to run;
  *   - results do not depend on anything but the arguments: no atomics, a fixed order of every sum.
  */
 
@@ -772,7 +775,7 @@ int fpn_detection_records(int b, int n, const float *mask_logits, const float *b
  * y = act(x w + bias) + residual.   x (rows,cin), w (cin,cout), bias (cout) or NULL, residual (rows,cout) or NULL,
  * y (rows,cout); pre (rows,cout), always float, or NULL receives x w + bias for fpn_dense_grad.
  */
-size_t fpn_dense_workspace_bytes(int dtype, long rows, int cin, int cout);
+size_t fpn_dense_workspace_bytes(int dtype, long rows, int cin, int cout, int whole);
 int fpn_dense(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w, long ldw, int w_transposed,
               const void *bias, int activation, const void *residual, long ldr, void *y, long ldy, float *pre, long ldp,
               void *workspace, size_t workspace_bytes, void *stream);
@@ -782,7 +785,7 @@ int fpn_dense(int dtype, long rows, int cin, int cout, const void *x, long ldx, 
  * sums of d; the residual's gradient is dy itself.  dx, dw, dbias may each be NULL; pre is not read where the
  * activation is FPN_ACT_NONE, x only for dw, w only for dx.
  */
-size_t fpn_dense_grad_workspace_bytes(int dtype, long rows, int cin, int cout, int activation);
+size_t fpn_dense_grad_workspace_bytes(int dtype, long rows, int cin, int cout, int activation, int whole);
 int fpn_dense_grad(int dtype, long rows, int cin, int cout, const void *dy, long lddy, const void *x, long ldx, const void *w,
                    long ldw, int w_transposed, const float *pre, long ldp, int activation, void *dx, long lddx, void *dw, long lddw,
                    void *dbias, void *workspace, size_t workspace_bytes, void *stream);
@@ -792,7 +795,7 @@ int fpn_dense_grad(int dtype, long rows, int cin, int cout, const void *dy, long
  * row stride (halves of one matrix will do); gate and up (rows,cout), always float, row stride ldp, receive the
  * two sums for fpn_gated_grad, or are both NULL.
  */
-size_t fpn_gated_workspace_bytes(int dtype, long rows, int cin, int cout);
+size_t fpn_gated_workspace_bytes(int dtype, long rows, int cin, int cout, int whole);
 int fpn_gated(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w_gate, long ldg, const void *w_up,
               long ldu, int w_transposed, const void *bias_gate, const void *bias_up, int activation, void *h, long ldh, float *gate,
               float *up, long ldp, void *workspace, size_t workspace_bytes, void *stream);
@@ -805,7 +808,7 @@ int fpn_gated(int dtype, long rows, int cin, int cout, const void *x, long ldx, 
  * dh = dy w_down^T is formed here and never rounded (w_down (cout,cdown), or (cdown,cout) where down_transposed);
  * cdown 0: w_down is not read.
  */
-size_t fpn_gated_grad_workspace_bytes(int dtype, long rows, int cin, int cout, int cdown);
+size_t fpn_gated_grad_workspace_bytes(int dtype, long rows, int cin, int cout, int cdown, int whole);
 int fpn_gated_grad(int dtype, long rows, int cin, int cout, int cdown, const void *dh, long lddh, const void *w_down, long ldd,
                    int down_transposed, const void *x, long ldx, const void *w_gate, long ldg, const void *w_up, long ldu,
                    int w_transposed, const float *gate, const float *up, long ldp, int activation, void *dx, long lddx, void *dw_gate,

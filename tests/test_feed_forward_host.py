@@ -87,20 +87,24 @@ def test_no_rows_is_a_valid_call_without_a_launch():
 
 def test_workspace_sizes():
     L = lib()
-    assert L.fpn_dense_workspace_bytes(BF16, 8192, 4096, 4096) == 0            # enough tiles: k is not split
-    assert L.fpn_dense_workspace_bytes(BF16, 1, 64, 64) == 0                   # a short k is not split either
-    assert L.fpn_dense_workspace_bytes(7, 1, 64, 64) == 0 and L.fpn_dense_workspace_bytes(BF16, 1, 0, 64) == 0
+    assert L.fpn_dense_workspace_bytes(BF16, 8192, 4096, 4096, 1) == 0            # enough tiles: k is not split
+    assert L.fpn_dense_workspace_bytes(BF16, 1, 64, 64, 1) == 0                   # a short k is not split either
+    assert L.fpn_dense_workspace_bytes(7, 1, 64, 64, 1) == 0 and L.fpn_dense_workspace_bytes(BF16, 1, 0, 64, 1) == 0
     for t, size in ((F32, 4), (BF16, 2), (F16, 2)):
         d = 1000 * 512 * size
-        assert L.fpn_dense_grad_workspace_bytes(t, 1000, 64, 512, 2) >= d
-        assert L.fpn_gated_grad_workspace_bytes(t, 1000, 64, 512, 0) >= 2 * d
+        assert L.fpn_dense_grad_workspace_bytes(t, 1000, 64, 512, 2, 1) >= d
+        assert L.fpn_gated_grad_workspace_bytes(t, 1000, 64, 512, 0, 1) >= 2 * d
         # partial sums of a split product: whole copies of the result
-        need = L.fpn_dense_workspace_bytes(t, 16, 8192, 256)
+        need = L.fpn_dense_workspace_bytes(t, 16, 8192, 256, 1)
         assert need % (16 * 256 * 4) == 0
+        # ragged operands: room for their copies, rows padded to whole chunks, where there is enough to multiply
+        need = L.fpn_dense_workspace_bytes(t, 2000, 1091, 515, 0) - L.fpn_dense_workspace_bytes(t, 2000, 1091, 515, 1)
+        assert need >= (2000 * 1092 + 1091 * 516) * size
+        assert L.fpn_dense_workspace_bytes(t, 20, 1091, 515, 0) == L.fpn_dense_workspace_bytes(t, 20, 1091, 515, 1)
     # one row more never needs a workspace out of proportion (splits times result stays bounded)
     for rows in (1, 16, 17, 64, 65, 1000, 131072):
         for n in (2, 64, 4096, 8192):
-            assert L.fpn_dense_workspace_bytes(BF16, rows, 8192, n) <= 256 << 20
+            assert L.fpn_dense_workspace_bytes(BF16, rows, 8192, n, 1) <= 256 << 20
 
 
 def test_python_refusals_without_a_device():
