@@ -498,9 +498,8 @@ template <class T> __device__ inline floatx16 multiply(uintx4 b, uintx4 a, float
 
 // A wave's accumulators to memory through its own piece of LDS, 32 rows at a time: written as they lie (a lane has four
 // consecutive columns of one row), read back as runs of eight columns of consecutive rows - whole lines for the
-// loads and stores, bias loaded once, and one copy of the epilogue's arithmetic: unrolled over a wave's tiles it was 200 KB of
-// code, which small products spent their time fetching (a gated fp32 product of 777 x 259 x 515: 21 us against XX).  `lds` is
-// the wave's, epilogue_bytes(TN); nobody else uses it.
+// loads and stores, bias loaded once, and one copy of the epilogue's arithmetic (unrolled over a wave's tiles it was 200 KB
+// of code for an activation and spilled registers).  `lds` is the wave's, epilogue_bytes(TN); nobody else uses it.
 constexpr int epilogue_bytes(int tn) { return 32 * (32 * tn * 4 + 16); }
 
 // MODE: a plain product, a gated one, or the gated block's backward epilogue on a plain one

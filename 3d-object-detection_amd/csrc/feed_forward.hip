@@ -135,7 +135,7 @@ int launch_grad(GradArgs p, bool gated, bool dy_float, void *const (&sums_out)[2
 //
 // Such rows cannot be brought straight into LDS, and reading them at their own alignment costs the load path several
 // passes per instruction.  Where there is enough to multiply they are copied once, rows padded with zeros to whole chunks
-// (a dense product of 1999 x 1091 x 515 fp16: 28 us without, XX with).
+// (a dense product of 1999 x 1091 x 515 in 16 bits: 26 us without, 22 with; 4000 x 2001 x 1001: 55 and 39).
 struct CopyArgs {
     struct { const void *from; void *to; long rows, ld, ldto; int cols; } of[3];
 };
@@ -407,24 +407,24 @@ namespace {
 // The time of a launch of `tiles` workgroups of one shape, in us, from what these took on a 256-CU chip: a stage of k (32
 // sixteen-bit elements, 16 floats) with workgroups on few CUs, with one on every CU and with `per_cu` on every CU - the
 // sixteen-bit shapes share the L2's bandwidth, 50 bytes/ns and CU -, and what a round of workgroups costs besides (first loads,
-// epilogue).  Measured against predicted, bf16, us:   large  medium  small  tiny
-//   8192 x 4096 x 4096                                 239     276    311   502
-//   4096 x 2048 x 2048                                  53      44     45    64
-//   2048 x 2048 x 2048                                  48      36     26    35
-//   1024 x 1024 x 1024                                  29      21     14    11
-//   4096 x 8192 x 1024, k split by 1 / 2 / 4    146/108/85 104/92/99 80/96/106 124/150/152
+// epilogue).  Measured, bf16, us:   large  medium  small  tiny
+//   8192 x 4096 x 4096                                 244     282    330   500
+//   4096 x 2048 x 2048                                  53      45     46    68
+//   2048 x 2048 x 2048                                  48      37     27    37
+//   1024 x 1024 x 1024                                  29      21     14    10
+//   4096 x 8192 x 1024, k split by 1 / 2 / 4    145/106/90 109/94/105 87/103/117 144/157/158
 struct Pace { int bm, bn, per_cu; double few, one, full, round; };
 constexpr Pace kWide[] = {
     {256, 256, 1, 0.50, 0.88, 0.88, 8.0},
     {256, 128, 2, 0.36, 0.58, 1.00, 6.0},
     {128, 128, 2, 0.28, 0.31, 0.62, 5.0},
-    {64, 64, 4, 0.20, 0.22, 0.48, 3.0},
+    {64, 64, 4, 0.17, 0.20, 0.50, 3.0},
 };
-// fp32: bound by its matrix rate, so the smallest tiles that keep it fed (us: small 264, tiny 263 at 1024 x 4096 x 4096,
-// 71 and 42 at 1024 x 1024 x 1024, 104 and 130 at 131072 x 128 x 256)
+// fp32: bound by its matrix rate, so the smallest tiles that keep it fed (us, k not split: small 264, tiny 268 at
+// 1024 x 4096 x 4096, 71 and 27 at 1024 x 1024 x 1024)
 constexpr Pace kWideF32[] = {
     {128, 128, 2, 1.00, 1.08, 2.00, 6.0},
-    {64, 64, 4, 0.55, 0.60, 1.20, 3.0},
+    {64, 64, 4, 0.33, 0.38, 1.06, 4.5},
 };
 
 double launch_time(const Pace &p, long tiles, double stages, int cus)
@@ -438,10 +438,6 @@ double launch_time(const Pace &p, long tiles, double stages, int cus)
 
 // writing and reading the partial sums of a split, and the join's launch
 double join_time(double bytes) { return 4.0 + bytes / 4e6; }
-
-}  // namespace
-
-namespace {
 
 Plan make_plan(int dtype, long m, int n, long k, int segs, int batch, bool gated, bool aligned, int order_a, int order_b, int cus)
 {

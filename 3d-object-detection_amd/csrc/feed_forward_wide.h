@@ -1,13 +1,15 @@
-// The feed-forward products' kernel for large products of 16-bit operands: 256 x 256 output tiles, operands brought
-// into LDS by loads that write it directly.
+// The feed-forward products' pipelined kernel: operands are brought into LDS by loads that write it directly.
 //
-// Eight waves, each 128 x 64 of the tile: 8 MFMA tiles of 32 x 32, 128 accumulator registers, two waves per SIMD, so that
-// one wave's MFMAs run while the other's requests wait to be taken (four waves of 128 x 128 read less from LDS,
-// but every request that waited stopped the SIMD: 247 us against XXX at 8192 x 4096 x 4096).
+// A workgroup of the largest shape makes a 256 x 256 tile with eight waves, each 128 x 64 of it: 8 MFMA tiles of 32 x 32, 128
+// accumulator registers, two waves per SIMD, so that one wave's MFMAs run while the other's requests wait to be taken
+// (four waves of 128 x 128 read less from LDS, but every request that waited stopped the SIMD: 247 us against 235 for the product of
+// 8192 x 4096 x 4096 bf16, 1.17 PFLOP/s).  The smaller shapes are for fewer rows and columns, where 256 x 256 tiles leave CUs
+// without work, and two or four workgroups on a CU cover each other's waits; fp32 uses only the two smallest, whose matrix
+// rate (153 TFLOP/s at most) bounds it with any tile.
 //
-// LDS holds four stages of 32 k (32 KB each).  A wave requests its eighth of stage t + 4 as soon as everyone has read
-// stage t, so a request has three stages' time (3072 cycles of MFMA) to arrive, and reads the next 16 of k
-// while it multiplies the present ones: one barrier per 32 of k, nothing else waits.
+// LDS holds three or four stages of 64 bytes of k per row: 32 sixteen-bit elements, 16 floats.  A wave requests its share
+// of stage t + 4 as soon as everyone has read stage t, so a request has three stages' time to arrive, and reads the next
+// half stage while it multiplies the present one: one barrier per stage, nothing else waits.
 //
 // The requests are written in assembly because the compiler, which cannot tell the stages apart, would wait for all of
 // them before every LDS read.  They have no result registers; the counts in `arrive` are theirs alone, since the loop
@@ -19,7 +21,7 @@ namespace fpn {
 namespace ff {
 
 constexpr int kStretch = 64;                                // bytes of k per stage: 32 sixteen-bit elements, 16 floats
-// A shape of workgroup: BM x BN tile, WM x WN waves of TM x TN MFMA tiles, stages of 32 k in LDS, workgroups per CU.
+// A shape of workgroup: BM x BN tile, WM x WN waves of TM x TN MFMA tiles, stages in LDS, workgroups per CU.
 template <int BM_, int BN_, int WM_, int WN_, int STAGES, int PER_CU> struct Shape {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, kStages = STAGES;
     static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves, TM = BM / WM / 32, TN = BN / WN / 32;
@@ -31,7 +33,8 @@ template <int BM_, int BN_, int WM_, int WN_, int STAGES, int PER_CU> struct Sha
 using Large = Shape<256, 256, 2, 4, 4, 1>;
 using Medium = Shape<256, 128, 2, 2, 3, 2>;
 using Small = Shape<128, 128, 4, 2, 4, 2>;
-using Tiny = Shape<64, 64, 2, 1, 4, 4>;
+// (one MFMA tile per wave: a chain of 1024 x 1024 x 1024 fp32 27 us, with two tiles on half as many waves 42)
+using Tiny = Shape<64, 64, 2, 2, 4, 4>;
 
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"             // (m0 is reserved: nothing here indexes registers through it)
@@ -62,8 +65,8 @@ __device__ inline unsigned lds_address(const char *p)
     return (unsigned)(size_t)(const __attribute__((address_space(3))) char *)p;
 }
 
-// One operand's R rows (m or n) x 32 k of a stage.  A request fills 1 KB: kInner 16 rows of 64 bytes, the four 16-byte
-// chunks of row r permuted by r >> 2 & 3; kOuter 2 or 4 rows (k) of R elements, permuted as in Tile.  The permutation is on
+// One operand's R rows (m or n) x 64 bytes of k of a stage.  A request fills 1 KB: kInner 16 rows of 64 bytes, the four 16-byte
+// chunks of row r permuted by r >> 2 & 3; kOuter rows (k) of R elements, permuted as in Tile.  The permutation is on
 // the source side: the lane that fills a slot fetches the chunk that belongs there.
 template <class T, int ORDER, int R, int WAVES> struct Stream {
     static constexpr int E = Type<T>::kE, BK = kStretch / (int)sizeof(T);
@@ -130,7 +133,7 @@ template <class T, int ORDER, int R, int WAVES> struct Stream {
     }
 };
 
-// A lane's operands of TILES 32-row groups, 16 of k at a time
+// A lane's operands of TILES 32-row groups, half a stage of k at a time
 template <class T, int ORDER, int R, int TILES> struct StreamReader {
     static constexpr int kRowBytes = R * (int)sizeof(T);
     unsigned at[ORDER == kInner ? 2 : TILES];
@@ -188,9 +191,12 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void wide_product_kernel(
     int am[kTM], bn[kTN];
 #pragma unroll
     for (int i = 0; i < kTM; ++i) am[i] = (wm * kTM + i) * 32;
-    // GATED: the first half of a wave's column tiles are of the gate half, the second the same columns of the up half
+    // GATED: the first half of a wave's column tiles are of the gate half, the second the same columns of the up half; where a
+    // wave has one column tile, gate and up are two waves' (kApart)
+    constexpr bool kApart = GATED && kTN == 1;
+    static_assert(!kApart || (S::WN == 2 && kTM == 1 && S::WM * (epilogue_bytes(2) + 4096) <= S::kBytes), "two halves, joined in LDS");
 #pragma unroll
-    for (int j = 0; j < kTN; ++j) bn[j] = GATED ? (wn * (kTN / 2) + j % (kTN / 2)) * 32 : (wn * kTN + j) * 32;
+    for (int j = 0; j < kTN; ++j) bn[j] = kApart ? 0 : GATED ? (wn * (kTN / 2) + j % std::max(kTN / 2, 1)) * 32 : (wn * kTN + j) * 32;
     StreamReader<T, ORDER_A, BM, kTM> ra;
     StreamReader<T, ORDER_B, kCols, kTN> rb;
     ra.init(am, lane);
@@ -242,9 +248,9 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void wide_product_kernel(
     };
     auto read_a = [&](const char *stage, int i, int s) { return ra.frag(stage, am[i], i, s); };
     auto read_b = [&](const char *stage, int j, int s) {
-        return rb.frag(stage + kABytes + (GATED && j >= kTN / 2 ? kHalfBytes : 0), bn[j], j, s);
+        return rb.frag(stage + kABytes + (kApart ? wn * kHalfBytes : GATED && j >= kTN / 2 ? kHalfBytes : 0), bn[j], j, s);
     };
-    // 16 of k: multiplies ca, cb while na, nb come from `stage`, and issues half a stage's requests from Q on to stage `to`.  A wave
+    // Half a stage: multiplies ca, cb while na, nb come from `stage`, and issues half a stage's requests from Q on to stage `to`.  A wave
     // issues in order: an MFMA occupies its unit for 32 cycles, in which seven other instructions can go out, so the
     // reads and requests are dealt out among the MFMAs one by one (all in front of a group of four MFMAs cost 12 %);
     // no read is left for the last two, which cover their latency.
@@ -282,9 +288,9 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void wide_product_kernel(
         segment(s);
         if (t0 < t1) {
             const long n = t1 - t0;
-            // Stage t + 4 is requested in two halves: behind the barrier of t, and in the first half of t + 1 (behind the
+            // Stage t + kStages is requested in two halves: behind the barrier of t, and in the first half of t + 1 (behind the
             // segment's end its last stage again, which nobody reads: a loop without branches, and counts that hold).
-            // In flight at a barrier are the three stages ahead; the one read next must be there.
+            // In flight at a barrier are the stages ahead; the one read next must be there.
             most = n - 1;
             asked = 0;
             sa.next = sa.base + t0 * sa.step;
@@ -331,6 +337,21 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void wide_product_kernel(
             }
         }
         __syncthreads();
+    }
+    if constexpr (kApart) {
+        float *const meet = reinterpret_cast<float *>(lds + S::WM * epilogue_bytes(2) + wm * 4096) + lane;
+        if (wn) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) meet[r * 64] = acc[0][0][r];
+        }
+        __syncthreads();
+        if (wn) return;
+        floatx16 both[1][2];
+        both[0][0] = acc[0][0];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) both[0][1][r] = meet[r * 64];
+        store_piece<T, MODE, 1, 2>(p, both, lds + wave * epilogue_bytes(2), at.member, at.split, m0 + wm * 32, n0, lane);
+        return;
     }
     store_piece<T, MODE, kTM, kTN>(p, acc, lds + wave * S::kEpilogueBytes, at.member, at.split, m0 + wm * 32 * kTM,
                              n0 + wn * 32 * (GATED ? kTN / 2 : kTN), lane);
