@@ -123,6 +123,8 @@ def _output(out, x, rows, cols, inputs, may_be=None):
     if out is None:
         return torch.empty((rows, cols), dtype=x.dtype, device=x.device), cols
     _tensor("out", out, x, (rows, cols))
+    if out.requires_grad and torch.is_grad_enabled():
+        raise ValueError("out requires gradients: autograd would not see that it is overwritten")
     ld = _rows("out", out)
     for name, t in inputs:
         t2 = t if t is None or t.dim() == 2 else t.unsqueeze(0)
@@ -130,6 +132,8 @@ def _output(out, x, rows, cols, inputs, may_be=None):
             raise ValueError("out shares memory with %s" % name)
     if may_be is not None and not (out.data_ptr() == may_be.data_ptr() and out.stride() == may_be.stride()) and _overlap(out, may_be):
         raise ValueError("out shares memory with residual without being it")
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)         # (a backward pass that saved it has to notice)
     return out, ld
 
 

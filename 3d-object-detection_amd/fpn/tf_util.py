@@ -6,10 +6,14 @@ A layer is ONE call into libfpn_hip.so: the 1x1 convolution (or matmul), bias,
 inference batch norm and ReLU are fused (the reference issues them as separate TF
 ops, tf_util.py:170-184).  Variables come from the active VariableStore under the
 same scoped names TF would give them.
+
+Two layers go beyond the reference's, for per-point feature blocks in float32,
+bfloat16 or float16: dense (activation and residual in the product's epilogue) and
+gated_feed_forward (feed_forward.py's block).
 """
 import torch
 
-from . import ops, variables
+from . import feed_forward, ops, variables
 
 
 def relu(x):
@@ -98,3 +102,45 @@ def dropout(inputs, is_training, scope, keep_prob=0.5, noise_shape=None):
     """Reference: tf_util.dropout, models/tf_util.py:594-615: identity at inference."""
     _inference_only(is_training)
     return inputs
+
+
+def _projection(scope, cin, cout, use_bias, dtype):
+    """A layer's weights (cin, cout) and bias, in the type of its inputs."""
+    store = variables.get_default_store()
+    name = variables.scoped(scope)
+    kept = [(name + "/weights", (cin, cout), "xavier")]
+    if use_bias:
+        kept.append((name + "/biases", (cout,), "zeros"))
+    held = [(key, store.get_variable(key, shape, init)) for key, shape, init in kept]
+    cast = [v if dtype == torch.float32 else store.cached(("cast", key, dtype), lambda v=v: v.to(dtype)) for key, v in held]
+    return cast[0], cast[1] if use_bias else None
+
+
+def _as_rows(t):
+    """(rows, channels) of a tensor with the channels innermost."""
+    if t.dim() < 2:
+        raise ValueError("expected a tensor of rank 2 or more with the channels innermost, got shape %s" % (tuple(t.shape),))
+    return t if t.dim() == 2 else t.flatten(0, -2)
+
+
+def dense(inputs, num_outputs, scope, activation=None, residual=None, use_bias=True):
+    """act(inputs W + b) + residual over the last dimension (feed_forward.dense): inputs (..., C), residual and result
+    (..., num_outputs), all of one type; activation by name (feed_forward.ACTIVATIONS)."""
+    x = _as_rows(inputs)
+    w, b = _projection(scope, x.shape[1], num_outputs, use_bias, x.dtype)
+    y = feed_forward.dense(x, w, b, activation, None if residual is None else _as_rows(residual))
+    return y.reshape(inputs.shape[:-1] + (num_outputs,))
+
+
+def gated_feed_forward(inputs, num_hidden, scope, num_outputs=None, activation="silu", residual=None, use_bias=True):
+    """(act(inputs Wg + bg) * (inputs Wu + bu)) Wd + bd + residual over the last dimension (feed_forward.gated_feed_forward):
+    inputs (..., C), residual and result (..., num_outputs), num_outputs = C unless given.  The variables are those of three
+    layers, <scope>/gate, <scope>/up and <scope>/down."""
+    x = _as_rows(inputs)
+    if num_outputs is None:
+        num_outputs = x.shape[1]
+    wg, bg = _projection(scope + "/gate", x.shape[1], num_hidden, use_bias, x.dtype)
+    wu, bu = _projection(scope + "/up", x.shape[1], num_hidden, use_bias, x.dtype)
+    wd, bd = _projection(scope + "/down", num_hidden, num_outputs, use_bias, x.dtype)
+    y = feed_forward.gated_feed_forward(x, wg, wu, wd, bg, bu, bd, activation, None if residual is None else _as_rows(residual))
+    return y.reshape(inputs.shape[:-1] + (num_outputs,))

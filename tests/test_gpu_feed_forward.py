@@ -505,3 +505,59 @@ def test_larger_products(device, t):
         h = F.gated(d["x"], d["wg"], d["wu"])
         g, up = d["x"].double() @ d["wg"].double(), d["x"].double() @ d["wu"].double()
         near(h, torch.nn.functional.silu(g) * up, cin, 5)
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+def test_layers(device, t):
+    """tf_util's layers are the operators on the store's variables, in the inputs' type, over any leading dimensions."""
+    from fpn import feed_forward as F
+    from fpn import tf_util, variables
+    dtype = TYPES[t][0]
+    g = torch.Generator().manual_seed(3)
+    points = torch.randn((2, 37, 64), generator=g).to(dtype).to(device).requires_grad_()
+    skip = torch.randn((2, 37, 64), generator=g).to(dtype).to(device)
+    with variables.use_store(variables.VariableStore(device, seed=4)) as store:
+        def layers():
+            with variables.variable_scope("refine"):
+                h = tf_util.gated_feed_forward(points, 96, "block", residual=points)
+                return tf_util.dense(h, 64, "out", "gelu", skip), tf_util.dense(h, 10, "head", use_bias=False)
+        y, z = layers()
+        assert sorted(store.keys()) == sorted("refine/%s/%s" % (layer, kind) for layer, kinds in (
+            ("block/gate", 2), ("block/up", 2), ("block/down", 2), ("out", 2), ("head", 1)) for kind in ("weights", "biases")[:kinds])
+        for name in list(store.keys()):                     # biases that are seen, and the casts made again
+            store[name] = store[name] + 0.25
+        y, z = layers()
+        v = {name: value.to(dtype) for name, value in store.items()}
+    x = points.reshape(-1, 64)
+    h = F.gated_feed_forward(x, v["refine/block/gate/weights"], v["refine/block/up/weights"], v["refine/block/down/weights"],
+                             v["refine/block/gate/biases"], v["refine/block/up/biases"], v["refine/block/down/biases"], residual=x)
+    want_y = F.dense(h, v["refine/out/weights"], v["refine/out/biases"], "gelu", skip.reshape(-1, 64))
+    want_z = F.dense(h, v["refine/head/weights"])
+    assert y.shape == (2, 37, 64) and torch.equal(y.reshape(-1, 64), want_y)
+    assert z.shape == (2, 37, 10) and torch.equal(z.reshape(-1, 10), want_z)
+    (got,) = torch.autograd.grad([y, z], [points], [torch.ones_like(y), torch.ones_like(z)])
+    (want,) = torch.autograd.grad([want_y, want_z], [points], [torch.ones_like(want_y), torch.ones_like(want_z)])
+    assert torch.equal(got, want)
+    with variables.use_store(store):
+        with pytest.raises(ValueError, match="rank 2 or more"):
+            tf_util.dense(points.reshape(-1), 10, "head")
+        with pytest.raises(ValueError, match="residual has shape"):
+            tf_util.dense(points, 10, "head2", residual=skip)
+
+
+def test_overwritten_results_are_noticed(device):
+    """`out` counts as written in place: a backward pass that saved it refuses, and a leaf that requires gradients cannot
+    be given."""
+    from fpn import feed_forward as F
+    x, w = torch.ones((4, 8), device=device), torch.ones((8, 8), device=device)
+    leaf = torch.ones((4, 8), device=device, requires_grad=True)
+    with pytest.raises(ValueError, match="out requires gradients"):
+        F.dense(x, w, out=leaf)
+    held = torch.ones((4, 8), device=device)
+    y = (leaf * held).sum()
+    F.dense(x, w, out=held)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        inside = torch.ones((4, 8), device=device)
+        assert (F.dense(x, w, out=inside) == 8).all()
