@@ -850,10 +850,18 @@ extern template int launch_few<__bf16>(const Args &, int, bool, int, int, hipStr
 extern template int launch_few<_Float16>(const Args &, int, bool, int, int, hipStream_t);
 #endif
 
+// (a launch has fewer than 2^32 threads)
+inline int check_grid(long blocks, int threads)
+{
+    if (blocks > 0xffffffffl / threads) return fail(FPN_E_UNSUPPORTED, "a launch of %ld workgroups of %d threads", blocks, threads);
+    return FPN_OK;
+}
+
 #define FPN_FF_LAUNCH(A, B, BM_, BN_, WM_, WN_, G)                                                                            \
     do {                                                                                                                      \
         auto kern = product_kernel<T, A, B, BM_, BN_, WM_, WN_, G>;                                                           \
         constexpr int bytes = std::max(2 * (BM_ + BN_) * kTileBytes, WM_ * WN_ * epilogue_bytes(BN_ / WN_ / 32));             \
+        if (check_grid(blocks, kThreads) != FPN_OK) return FPN_E_UNSUPPORTED;                                                 \
         if (!allow_dynamic_lds(reinterpret_cast<const void *>(kern), bytes))                                                  \
             return fail(FPN_E_LAUNCH, "%d bytes of LDS refused", bytes);                                                      \
         hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(kThreads), bytes, stream, p);                                   \
@@ -878,8 +886,7 @@ int launch_tiles(const Args &p, int order_a, int order_b, bool gated, long block
 template <class T> int launch_join(const Args &p, bool gated, hipStream_t stream)
 {
     const long runs8 = p.m * ((p.n + 7) / 8);
-    const long join_blocks = (runs8 + 31) / 32;
-    if (join_blocks > 0x7fffffffl) return fail(FPN_E_UNSUPPORTED, "a join of %ld workgroups", join_blocks);
+    const long join_blocks = (runs8 + 31) / 32;             // (partial sums are at most 128 MB, or those of 64 rows)
     const dim3 grid((unsigned)join_blocks, p.batch);
     if (gated) hipLaunchKernelGGL((join_kernel<T, true>), grid, dim3(kThreads), 0, stream, p);
     else hipLaunchKernelGGL((join_kernel<T, false>), grid, dim3(kThreads), 0, stream, p);
@@ -899,7 +906,6 @@ template <class T> int launch_product(Args p, int order_a, int order_b, bool gat
     p.mt = (p.m + plan.bm - 1) / plan.bm;
     p.nt = (p.n + cols - 1) / cols;
     const long blocks = p.mt * p.nt * p.splits * p.batch;
-    if (blocks > 0x7fffffffl) return fail(FPN_E_UNSUPPORTED, "a product of %ld workgroups", blocks);
     int rc;
     if (plan.wide) rc = launch_wide<T>(p, order_a, order_b, gated, plan.bm, plan.bn, blocks, stream);
     else if (plan.bm == 128) rc = launch_tiles<T, 128, 128, 2, 2>(p, order_a, order_b, gated, blocks, stream);

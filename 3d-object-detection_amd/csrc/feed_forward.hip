@@ -200,11 +200,13 @@ int run_product(int dtype, const Args &p, int order_a, int order_b, bool gated, 
 
 constexpr int kStretchBytes = 64;             // of k per stage of the wide kernel
 constexpr long kMostLd = (1l << 21) - 1;      // a tile's byte offsets inside an operand are 32 bits
+constexpr long kMostRows = 1l << 40;          // (products of sizes stay inside 64 bits)
 
 int check_common(int dtype, long rows, int cin, int cout, int activation)
 {
     FPN_REQUIRE(dtype == FPN_F32 || dtype == FPN_BF16 || dtype == FPN_F16, "dtype %d is none of FPN_F32, FPN_BF16, FPN_F16", dtype);
     FPN_REQUIRE(rows >= 0 && cin >= 1 && cout >= 1, "rows %ld, cin %d, cout %d: rows >= 0 and widths >= 1 are needed", rows, cin, cout);
+    if (rows > kMostRows) return fail(FPN_E_UNSUPPORTED, "up to %ld rows are supported, got %ld", kMostRows, rows);
     FPN_REQUIRE(activation >= FPN_ACT_NONE && activation <= FPN_ACT_GELU_TANH, "unknown activation %d", activation);
     if (cin > kMostLd || cout > kMostLd) return fail(FPN_E_UNSUPPORTED, "widths up to %ld are supported, got %d and %d", kMostLd, cin, cout);
     return FPN_OK;

@@ -360,6 +360,7 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void wide_product_kernel(
 #define FPN_FF_WIDE(A, B, G)                                                                                                  \
     do {                                                                                                                      \
         auto kern = wide_product_kernel<T, A, B, G, S>;                                                                       \
+        if (check_grid(blocks, S::kThreads) != FPN_OK) return FPN_E_UNSUPPORTED;                                              \
         if (!allow_dynamic_lds(reinterpret_cast<const void *>(kern), S::kBytes))                                              \
             return fail(FPN_E_LAUNCH, "%d bytes of LDS refused", S::kBytes);                                                  \
         hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(S::kThreads), S::kBytes, stream, p);                            \

@@ -149,3 +149,12 @@ def test_row_strides_and_overlap():
     assert F._overlap(wide[:, :8], wide[:, 7:20]) and F._overlap(wide, wide) and F._overlap(wide[2:], wide[:3])
     assert not F._overlap(wide[:3], wide[3:]) and not F._overlap(wide, torch.zeros(4, 4))
     assert F._overlap(wide[:, 30:], wide[1:, :4].as_strided((3, 20), (40, 1), 35))
+
+
+@pytest.mark.parametrize("call,more", [(dense, {}), (gated, {}), (dense_grad, dict(act=0, dw=None, db=None))])
+def test_more_rows_than_one_launch_takes(call, more):
+    """Products of sizes would overflow, or a grid have 2^32 threads or more: refused before anything is launched."""
+    assert call(rows=(1 << 40) + 1, **more) == -3
+    assert "rows" in said()
+    assert call(rows=1 << 34, **more) == -3
+    assert "workgroups" in said()
