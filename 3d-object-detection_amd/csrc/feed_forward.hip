@@ -417,16 +417,16 @@ namespace {
 //   4096 x 8192 x 1024, k split by 1 / 2 / 4    145/106/90 109/94/105 87/103/117 144/157/158
 struct Pace { int bm, bn, per_cu; double few, one, full, round; };
 constexpr Pace kWide[] = {
-    {256, 256, 1, 0.50, 0.88, 0.88, 8.0},
-    {256, 128, 2, 0.36, 0.58, 1.00, 6.0},
-    {128, 128, 2, 0.28, 0.31, 0.62, 5.0},
-    {64, 64, 4, 0.17, 0.20, 0.50, 3.0},
+    {256, 256, 1, 0.54, 0.82, 0.82, 8.0},
+    {256, 128, 1, 0.40, 0.52, 0.52, 6.0},
+    {128, 128, 2, 0.25, 0.30, 0.53, 5.0},
+    {64, 64, 4, 0.19, 0.21, 0.42, 3.0},
 };
 // fp32: bound by its matrix rate, so the smallest tiles that keep it fed (us, k not split: small 264, tiny 268 at
 // 1024 x 4096 x 4096, 71 and 27 at 1024 x 1024 x 1024)
 constexpr Pace kWideF32[] = {
-    {128, 128, 2, 1.00, 1.08, 2.00, 6.0},
-    {64, 64, 4, 0.33, 0.38, 1.06, 4.5},
+    {128, 128, 2, 0.97, 1.02, 2.00, 6.0},
+    {64, 64, 4, 0.31, 0.34, 1.04, 4.5},
 };
 
 double launch_time(const Pace &p, long tiles, double stages, int cus)
@@ -799,7 +799,7 @@ int fpn_gated_grad(int dtype, long rows, int cin, int cout, int cdown, const voi
         }
         FPN_FF_TRY(run_product(dtype, p, kInner, order_down, false, partial, space.partial, st));
         if (done && g.sums) {
-            const int rows_each = plan.bm == 256 ? 128 : 32;       // (of a wave: 32 TM of feed_forward_wide.h)
+            const int rows_each = plan.bn == 256 ? 128 : plan.bm == 256 ? 64 : 32;       // (of a wave: 32 TM of feed_forward_wide.h)
             FPN_FF_TRY(run_column_join(dtype, cout, (int)((rows + plan.bm - 1) / plan.bm * (plan.bm / rows_each)), g.sums, sums_out, st));
         }
     }

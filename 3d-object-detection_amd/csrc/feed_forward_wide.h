@@ -2,14 +2,16 @@
 //
 // A workgroup of the largest shape makes a 256 x 256 tile with eight waves, each 128 x 64 of it: 8 MFMA tiles of 32 x 32, 128
 // accumulator registers, two waves per SIMD, so that one wave's MFMAs run while the other's requests wait to be taken
-// (four waves of 128 x 128 read less from LDS, but every request that waited stopped the SIMD: 247 us against 235 for the product of
-// 8192 x 4096 x 4096 bf16, 1.17 PFLOP/s).  The smaller shapes are for fewer rows and columns, where 256 x 256 tiles leave CUs
-// without work, and two or four workgroups on a CU cover each other's waits; fp32 uses only the two smallest, whose matrix
-// rate (153 TFLOP/s at most) bounds it with any tile.
+// (four waves of 128 x 128 read less from LDS, but every request that waited stopped the SIMD: 247 us against 235 for the product
+// of 8192 x 4096 x 4096 bf16).  The smaller shapes are for fewer rows and columns, where 256 x 256 tiles leave CUs without
+// work; fp32 uses only the two smallest, whose matrix rate (153 TFLOP/s at most) bounds it with any tile.
 //
-// LDS holds three or four stages of 64 bytes of k per row: 32 sixteen-bit elements, 16 floats.  A wave requests its share
-// of stage t + 4 as soon as everyone has read stage t, so a request has three stages' time to arrive, and reads the next
-// half stage while it multiplies the present one: one barrier per stage, nothing else waits.
+// LDS holds four to eight stages of 64 bytes of k per row: 32 sixteen-bit elements, 16 floats.  Stages are asked for in
+// pairs, each row's two 64-byte halves of a cache line one right after the other: what a CU receives from L2 comes by whole
+// lines, and the halves of a line asked for a stage apart were fetched twice (the product above: 241 us, in pairs 224; with
+// 64 x 64 tiles 532 and 403).  A pair is asked for as soon as everyone has read the one that had its place, half of it
+// behind the barrier and half in the next step; a wave reads the next half stage while it multiplies the present one:
+// one barrier per stage, nothing else waits.
 //
 // The requests are written in assembly because the compiler, which cannot tell the stages apart, would wait for all of
 // them before every LDS read.  They have no result registers; the counts in `arrive` are theirs alone, since the loop
@@ -31,9 +33,11 @@ template <int BM_, int BN_, int WM_, int WN_, int STAGES, int PER_CU> struct Sha
     static constexpr int kBytes = std::max(kStages * kStage, kWaves * kEpilogueBytes);
 };
 using Large = Shape<256, 256, 2, 4, 4, 1>;
-using Medium = Shape<256, 128, 2, 2, 3, 2>;
+using Medium = Shape<256, 128, 4, 2, 6, 1>;
 using Small = Shape<128, 128, 4, 2, 4, 2>;
-// (one MFMA tile per wave: a chain of 1024 x 1024 x 1024 fp32 27 us, with two tiles on half as many waves 42)
+// (Small where it is alone on its CU and k is long: 4096 x 8192 x 1024 bf16 77 us against 82)
+using Deep = Shape<128, 128, 4, 2, 8, 1>;
+// (one MFMA tile per wave: a product of 1024 x 1024 x 1024 fp32 27 us, with two tiles on half as many waves 42)
 using Tiny = Shape<64, 64, 2, 2, 4, 4>;
 
 #pragma clang diagnostic push
@@ -50,14 +54,7 @@ template <int AT> __device__ inline void request(unsigned lds, unsigned off, con
 // everyone's.
 template <int LEFT> __device__ inline void arrive()
 {
-    static_assert(LEFT == 0 || LEFT == 4 || LEFT == 5 || LEFT == 6 || LEFT == 8 || LEFT == 9 || LEFT == 10, "a count written out below");
-    if (LEFT == 4) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" : : : "memory");
-    else if (LEFT == 5) asm volatile("s_waitcnt vmcnt(5) lgkmcnt(0)\n\ts_barrier" : : : "memory");
-    else if (LEFT == 6) asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)\n\ts_barrier" : : : "memory");
-    else if (LEFT == 8) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" : : : "memory");
-    else if (LEFT == 9) asm volatile("s_waitcnt vmcnt(9) lgkmcnt(0)\n\ts_barrier" : : : "memory");
-    else if (LEFT == 10) asm volatile("s_waitcnt vmcnt(10) lgkmcnt(0)\n\ts_barrier" : : : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(LEFT) : "memory");
 }
 
 __device__ inline unsigned lds_address(const char *p)
@@ -73,7 +70,7 @@ template <class T, int ORDER, int R, int WAVES> struct Stream {
     static constexpr int kPer = R * kStretch / 1024 / WAVES;    // requests per wave
     static constexpr int kRowBytes = R * (int)sizeof(T);        // kOuter
     const char *base;                                       // uniform: k = 0 of the segment
-    const char *next;                                       // the stage to be requested next
+    const char *next[2];                                    // the two stages to be requested next
     long step;                                              // bytes between stages
     unsigned off[kPer];
 
@@ -106,8 +103,8 @@ template <class T, int ORDER, int R, int WAVES> struct Stream {
         }
     }
 
-    // request I of kPer; lds: the stage's piece for this operand and wave
-    template <int I> __device__ void issue(unsigned lds) const { request<I * 1024>(lds, off[I], next); }
+    // request I of kPer of one of the two; lds: the stage's piece for this operand and wave
+    template <int I> __device__ void issue(unsigned lds, int half) const { request<I * 1024>(lds, off[I], next[half]); }
 
     // the last, partial stage of a segment, through registers, zeros behind the last k
     __device__ void put_tail(char *lds, long kt, int left_k, int wave, int lane) const
@@ -171,6 +168,15 @@ template <class T, int ORDER, int R, int TILES> struct StreamReader {
     }
 };
 
+// f(0), f(1) .. f(COUNT - 1), each with its number as a type
+template <int COUNT, int FROM = 0, class F> __device__ inline void each(F &&f)
+{
+    if constexpr (FROM < COUNT) {
+        f(ActTag<FROM>());
+        each<COUNT, FROM + 1>(f);
+    }
+}
+
 template <class T, int ORDER_A, int ORDER_B, int MODE, class S>
 __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void wide_product_kernel(const Args p)
 {
@@ -228,36 +234,28 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void wide_product_kernel(
             sb[0].init(p.b[s + at.member], p.ldb[s + at.member], n0, left_n, wave, lane);
         }
     };
-    // request Q of a wave's kPer of a stage
     constexpr int kPerA = decltype(sa)::kPer, kPerB = Stream<T, ORDER_B, kCols, kWavesB>::kPer, kPer = kPerA + kStreams * kPerB;
-    static_assert(kPer % 2 == 0 && kPerA > 0 && kPerB > 0, "half a stage's requests per step");
+    static_assert(kPerA > 0 && kPerB > 0 && kStages % 2 == 0, "a wave has requests of both operands");
     const unsigned lds_a = lds0 + wave * (kPerA * 1024), lds_b = lds0 + kABytes + (kDealt ? dealt * kHalfBytes : 0) + wave_b * (kPerB * 1024);
+    // request Q of a wave's 2 kPer of a pair of stages, the first of which is `stage`: the two stages in turn
     auto issue = [&](auto q, int stage) {
-        constexpr int Q = decltype(q)::value;
+        constexpr int H = decltype(q)::value & 1, Q = decltype(q)::value >> 1;
         constexpr int G = (Q - kPerA) / kPerB * (Q >= kPerA);
-        if constexpr (Q < kPerA) sa.template issue<Q>(lds_a + stage * kStage);
-        else sb[G].template issue<(Q - kPerA) % kPerB>(lds_b + G * kHalfBytes + stage * kStage);
-    };
-    long asked = 0, most = 0;                               // stages whose requests are complete, and the last to ask for
-    auto advance = [&] {
-        const bool on = asked < most;
-        ++asked;
-        sa.next += on ? sa.step : 0;
-#pragma unroll
-        for (int g = 0; g < kStreams; ++g) sb[g].next += on ? sb[g].step : 0;
+        if constexpr (Q < kPerA) sa.template issue<Q>(lds_a + (stage + H) * kStage, H);
+        else sb[G].template issue<(Q - kPerA) % kPerB>(lds_b + G * kHalfBytes + (stage + H) * kStage, H);
     };
     auto read_a = [&](const char *stage, int i, int s) { return ra.frag(stage, am[i], i, s); };
     auto read_b = [&](const char *stage, int j, int s) {
         return rb.frag(stage + kABytes + (kApart ? wn * kHalfBytes : GATED && j >= kTN / 2 ? kHalfBytes : 0), bn[j], j, s);
     };
-    // Half a stage: multiplies ca, cb while na, nb come from `stage`, and issues half a stage's requests from Q on to stage `to`.  A wave
-    // issues in order: an MFMA occupies its unit for 32 cycles, in which seven other instructions can go out, so the
-    // reads and requests are dealt out among the MFMAs one by one (all in front of a group of four MFMAs cost 12 %);
-    // no read is left for the last two, which cover their latency.
+    // Half a stage: multiplies ca, cb while na, nb come from `stage`, and issues requests Q to Q + kPer (none: Q < 0) of the
+    // pair at `to`.  A wave issues in order: an MFMA occupies its unit for 32 cycles, in which seven other instructions can go
+    // out, so the reads and requests are dealt out among the MFMAs one by one (all in front of a group of four MFMAs cost
+    // 12 %); no read is left for the last two, which cover their latency.
     auto step = [&](const uintx4 (&ca)[kTM], const uintx4 (&cb)[kTN], uintx4 (&na)[kTM], uintx4 (&nb)[kTN], const char *stage, int s,
                     auto q, int to) {
         constexpr int Q = decltype(q)::value;
-        constexpr int kAll = kTM * kTN, kHalf = kPer / 2;
+        constexpr int kAll = kTM * kTN;
 #pragma unroll
         for (int i = 0; i < kAll; ++i) {
             acc[i % kTM][i / kTM] = multiply<T>(cb[i / kTM], ca[i % kTM], acc[i % kTM][i / kTM]);
@@ -267,10 +265,11 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void wide_product_kernel(
                     if (r < kTM) na[r] = read_a(stage, r, s);
                     else nb[r - kTM] = read_b(stage, r - kTM, s);
                 }
-            if (kAll / (2 * kHalf) == i) issue(ActTag<Q>(), to);
-            if (kHalf > 1 && 3 * kAll / (2 * kHalf) == i) issue(ActTag<Q + (kHalf > 1)>(), to);
-            if (kHalf > 2 && 5 * kAll / (2 * kHalf) == i) issue(ActTag<Q + 2 * (kHalf > 2)>(), to);
-            static_assert(kHalf <= 3, "a request written out above");
+            if constexpr (Q >= 0)
+                each<kPer>([&](auto j) {
+                    constexpr int J = decltype(j)::value;
+                    if ((2 * J + 1) * kAll / (2 * kPer) == i) issue(ActTag<Q + J>(), to);
+                });
             __builtin_amdgcn_sched_barrier(0);
         }
     };
@@ -288,35 +287,43 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void wide_product_kernel(
         segment(s);
         if (t0 < t1) {
             const long n = t1 - t0;
-            // Stage t + kStages is requested in two halves: behind the barrier of t, and in the first half of t + 1 (behind the
-            // segment's end its last stage again, which nobody reads: a loop without branches, and counts that hold).
-            // In flight at a barrier are the stages ahead; the one read next must be there.
-            most = n - 1;
-            asked = 0;
-            sa.next = sa.base + t0 * sa.step;
+            // Behind the segment's end its last stage is asked for again, which nobody reads: a loop without branches, and
+            // counts that hold.  On their way at a barrier are the pairs behind the one read next.
+            long asked = 0;
+            auto aim = [&] {
+                const long first_at = t0 + min(asked, n - 1), second_at = t0 + min(asked + 1, n - 1);
+                auto point = [&](auto &stream) {
+                    stream.next[0] = stream.base + first_at * stream.step;
+                    stream.next[1] = stream.base + second_at * stream.step;
+                };
+                point(sa);
 #pragma unroll
-            for (int g = 0; g < kStreams; ++g) sb[g].next = sb[g].base + t0 * sb[g].step;
+                for (int g = 0; g < kStreams; ++g) point(sb[g]);
+                asked += 2;
+            };
 #pragma unroll
-            for (int i = 0; i < kStages; ++i) {
-                issue(ActTag<0>(), i);
-                if constexpr (kPer > 2) issue(ActTag<1>(), i);
-                if constexpr (kPer > 4) issue(ActTag<2>(), i);
-                if (i == kStages - 1) break;
-                issue(ActTag<kPer / 2>(), i);
-                if constexpr (kPer > 2) issue(ActTag<kPer / 2 + (kPer > 2)>(), i);
-                if constexpr (kPer > 4) issue(ActTag<kPer - 1>(), i);
-                advance();
+            for (int i = 0; i < kStages; i += 2) {
+                aim();
+                each<kPer>([&](auto j) { issue(ActTag<decltype(j)::value>(), i); });
+                if (i < kStages - 2) each<kPer>([&](auto j) { issue(ActTag<kPer + decltype(j)::value>(), i); });
             }
-            arrive<(kStages - 2) * kPer + kPer / 2>();
+            arrive<(kStages - 4) * kPer + kPer>();
             read(fa[0], fb[0], 0);
-            int stage = 0;
-            for (long t = 0; t < n; ++t) {
-                step(fa[0], fb[0], fa[1], fb[1], lds + stage * kStage, 1, ActTag<kPer / 2>(), stage ? stage - 1 : kStages - 1);
-                advance();
+            int pair = 0;                                   // its first stage
+            for (long t = 1; t < n; t += 2) {
+                step(fa[0], fb[0], fa[1], fb[1], lds + pair * kStage, 1, ActTag<kPer>(), pair ? pair - 2 : kStages - 2);
                 arrive<(kStages - 2) * kPer>();
-                const int freed = stage;
-                stage = stage == kStages - 1 ? 0 : stage + 1;
-                step(fa[1], fb[1], fa[0], fb[0], lds + stage * kStage, 0, ActTag<0>(), freed);
+                step(fa[1], fb[1], fa[0], fb[0], lds + (pair + 1) * kStage, 0, ActTag<-1>(), 0);
+                step(fa[0], fb[0], fa[1], fb[1], lds + (pair + 1) * kStage, 1, ActTag<-1>(), 0);
+                aim();
+                arrive<(kStages - 4) * kPer>();
+                const int freed = pair;
+                pair = pair == kStages - 2 ? 0 : pair + 2;
+                step(fa[1], fb[1], fa[0], fb[0], lds + pair * kStage, 0, ActTag<0>(), freed);
+            }
+            if (n & 1) {                                    // (the second step reads what is not used)
+                step(fa[0], fb[0], fa[1], fb[1], lds + pair * kStage, 1, ActTag<-1>(), 0);
+                step(fa[1], fb[1], fa[0], fb[0], lds + pair * kStage, 0, ActTag<-1>(), 0);
             }
             arrive<0>();
         }
@@ -389,6 +396,7 @@ template <class T> int launch_wide(const Args &p, int order_a, int order_b, bool
     if constexpr (sizeof(T) == 2) {                         // (fp32 is bound by its matrix rate with any tile)
         if (bn == 256) return launch_shape<T, Large>(p, order_a, order_b, gated, blocks, stream);
         if (bm == 256) return launch_shape<T, Medium>(p, order_a, order_b, gated, blocks, stream);
+        if (bm == 128 && blocks <= current_device_cus() && p.tiles_per_split >= 40) return launch_shape<T, Deep>(p, order_a, order_b, gated, blocks, stream);
     }
     if (bm == 128) return launch_shape<T, Small>(p, order_a, order_b, gated, blocks, stream);
     return launch_shape<T, Tiny>(p, order_a, order_b, gated, blocks, stream);
