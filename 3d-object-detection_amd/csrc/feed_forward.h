@@ -200,6 +200,42 @@ template <class T> __device__ inline void load8(const T *p, long count, float (&
     }
 }
 
+// load8 in two steps: the bytes, and what they are
+template <class T> struct Raw8 {
+    uintx4 v[sizeof(T) / 2];
+
+    __device__ void load(const T *p, long count)
+    {
+        if (count >= 8) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = *reinterpret_cast<const uintx4_u *>(p + i * (16 / sizeof(T)));
+        } else {
+            typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+            constexpr int E = 16 / (int)sizeof(T);
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+                vec e;
+#pragma unroll
+                for (int j = 0; j < E; ++j) e[j] = i * E + j < count ? p[i * E + j] : (T)0.f;
+                v[i] = __builtin_bit_cast(uintx4, e);
+            }
+        }
+    }
+
+    __device__ void add_to(float (&sum)[8]) const
+    {
+        typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+        constexpr int E = 16 / (int)sizeof(T);
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+            const uintx4 raw = v[i];
+            const vec e = __builtin_bit_cast(vec, raw);
+#pragma unroll
+            for (int j = 0; j < E; ++j) sum[i * E + j] += (float)e[j];
+        }
+    }
+};
+
 template <class T> __device__ inline void store8(T *p, long count, const float (&v)[8])
 {
     if (count >= 8) {
@@ -529,6 +565,16 @@ __device__ inline void store_piece(const Args &p, const floatx16 (&acc)[TM][TN],
     float bias[8] = {}, bias2[8] = {};
     if (MODE != kGateGradMode && left > 0 && p.bias[GATED ? 0 : member]) load8(reinterpret_cast<const T *>(p.bias[GATED ? 0 : member]) + n, left, bias);
     if (GATED && left > 0 && p.bias[1]) load8(reinterpret_cast<const T *>(p.bias[1]) + n, left, bias2);
+    // the residual of the next rows is on its way while the present ones are finished (8192 x 4096 x 4096 bf16 with gelu and
+    // residual: 251 us without, 244 with)
+    constexpr bool RESIDUAL = MODE == kPlainMode;
+    Raw8<T> res[RESIDUAL ? kBatch : 1];
+    auto fetch = [&](long row) {
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) res[RESIDUAL ? b : 0].load(reinterpret_cast<const T *>(p.residual) + min(row + b * kRowsAtOnce, p.m - 1) * p.ldr + n, left);
+    };
+    const bool adds = RESIDUAL && p.residual && !p.partial && left > 0;
+    if (adds) fetch(m0 + row0);
 #pragma unroll 1
     for (int i = 0; i < TM; ++i) {
         if (i == 0) put(acc[0]);
@@ -541,11 +587,7 @@ __device__ inline void store_piece(const Args &p, const floatx16 (&acc)[TM][TN],
 #pragma unroll 1
         for (int r = row0; r < 32; r += kRowsAtOnce * kBatch) {
             const long m = m0 + 32 * i + r;
-            float v[kBatch][8], v2[GATED ? kBatch : 1][8], res[kBatch][8];
-            if (MODE != kGateGradMode && p.residual)
-#pragma unroll
-                for (int b = 0; b < kBatch; ++b)
-                    load8(reinterpret_cast<const T *>(p.residual) + min(m + b * kRowsAtOnce, p.m - 1) * p.ldr + n, left, res[b]);
+            float v[kBatch][8], v2[GATED ? kBatch : 1][8];
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
                 const float *from = reinterpret_cast<const float *>(lds + (r + b * kRowsAtOnce) * kEpilogueRow) + run * 8;
@@ -620,13 +662,17 @@ __device__ inline void store_piece(const Args &p, const floatx16 (&acc)[TM][TN],
 #pragma unroll
                         for (int e = 0; e < 8; ++e) v[b][e] = activate<decltype(tag)::value, EXACT>(v[b][e]);
                 });
+            if (adds) {
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b) res[RESIDUAL ? b : 0].add_to(v[b]);
+                // (behind a piece's last rows come the next piece's first)
+                fetch(r + kRowsAtOnce * kBatch < 32 ? m + kRowsAtOnce * kBatch : m0 + 32 * (i + 1) + row0);
+            }
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
+                for (int e = 0; e < 8; ++e)
                     if (GATED) v[b][e] *= v2[b][e];
-                    if (p.residual) v[b][e] += res[b][e];
-                }
                 if (m + b * kRowsAtOnce < p.m) {
                     if (p.c_float) store8(reinterpret_cast<float *>(p.c[member]) + (m + b * kRowsAtOnce) * p.ldc + n, left, v[b]);
                     else store8(reinterpret_cast<T *>(p.c[member]) + (m + b * kRowsAtOnce) * p.ldc + n, left, v[b]);
