@@ -254,8 +254,13 @@ long padded(int dtype, long cols)
 }
 
 // whether operands with ragged rows are copied: a copy's launch and traffic (4 us and more) against what the pipelined
-// kernel saves, which takes half the time from about 10^8 operations on
-bool worth_copies(long rows, int cin, int cout) { return rows > 64 && cin >= 64 && cout >= 64 && 2.0 * rows * cin * cout >= 1e8; }
+// kernel saves, which takes half the time from about 10^8 operations on (an output narrower than its tile counts as 64
+// columns: 40189 x 1280 x 3 bf16 90 us without copies of the weights, 23 with; 40189 x 1281 x 3, where x is copied too, 96 and
+// 56; but 70000 x 131 x 37 24 either way and its weights' gradient 29 and 38, so that a narrow one wants a longer sum)
+bool worth_copies(long rows, int cin, int cout)
+{
+    return rows > 64 && cin >= (cout >= 64 ? 64 : 192) && 2.0 * rows * cin * std::max(cout, 64) >= 1e8;
+}
 
 // the bytes of copies of a matrix in either storage order
 size_t copy_bytes(int dtype, long rows, long cols) { return align256((size_t)rows * padded(dtype, cols) * element_size(dtype)); }

@@ -492,7 +492,7 @@ def test_larger_products(device, t):
 
     def near(got, want, k, factor=1):
         assert float((got.double() - want).norm() / want.norm()) <= u + factor * 2.0 ** -24 * k ** 0.5
-    for rows, cin, cout in [(2048, 1024, 2048), (4099, 515, 1027), (1024, 2000, 4096), (16, 4096, 4096), (70000, 64, 96)]:
+    for rows, cin, cout in [(2048, 1024, 2048), (4099, 515, 1027), (1024, 2000, 4096), (16, 4096, 4096), (70000, 64, 96), (9001, 640, 3), (4100, 515, 13)]:
         d = make(device, dtype, rows, cin, cout, seed=6)
         want = d["x"].double() @ d["w"].double()
         y = F.dense(d["x"], d["w"])
