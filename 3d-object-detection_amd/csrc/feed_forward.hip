@@ -414,24 +414,24 @@ namespace {
 // The time of a launch of `tiles` workgroups of one shape, in us, from what these took on a 256-CU chip: a stage of k (32
 // sixteen-bit elements, 16 floats) with workgroups on few CUs, with one on every CU and with `per_cu` on every CU - the
 // sixteen-bit shapes share the L2's bandwidth, 50 bytes/ns and CU -, and what a round of workgroups costs besides (first loads,
-// epilogue).  Measured, bf16, us:   large  medium  small  tiny
-//   8192 x 4096 x 4096                                 244     282    330   500
-//   4096 x 2048 x 2048                                  53      45     46    68
-//   2048 x 2048 x 2048                                  48      37     27    37
-//   1024 x 1024 x 1024                                  29      21     14    10
-//   4096 x 8192 x 1024, k split by 1 / 2 / 4    145/106/90 109/94/105 87/103/117 144/157/158
+// epilogue).  Measured, bf16, k not split, us:   large  medium  small  tiny
+//   8192 x 4096 x 4096                             230     272    287   414
+//   4096 x 2048 x 2048                              51      41     42    58
+//   2048 x 2048 x 2048                              49      36     27    32
+//   1024 x 1024 x 1024                              28      18     14    10
+//   4096 x 8192 x 1024                             148     110     79   102
 struct Pace { int bm, bn, per_cu; double few, one, full, round; };
 constexpr Pace kWide[] = {
-    {256, 256, 1, 0.54, 0.82, 0.82, 8.0},
+    {256, 256, 1, 0.54, 0.82, 0.82, 10.0},
     {256, 128, 1, 0.40, 0.52, 0.52, 6.0},
-    {128, 128, 2, 0.25, 0.30, 0.53, 5.0},
-    {64, 64, 4, 0.19, 0.21, 0.42, 3.0},
+    {128, 128, 2, 0.25, 0.30, 0.53, 6.2},
+    {64, 64, 4, 0.18, 0.19, 0.41, 4.5},
 };
-// fp32: bound by its matrix rate, so the smallest tiles that keep it fed (us, k not split: small 264, tiny 268 at
-// 1024 x 4096 x 4096, 71 and 27 at 1024 x 1024 x 1024)
+// fp32: bound by its matrix rate, so the smallest tiles that keep it fed (us, k not split: small 265, tiny 270 at
+// 1024 x 4096 x 4096, 68 and 25 at 1024 x 1024 x 1024)
 constexpr Pace kWideF32[] = {
     {128, 128, 2, 0.97, 1.02, 2.00, 6.0},
-    {64, 64, 4, 0.31, 0.34, 1.04, 4.5},
+    {64, 64, 4, 0.29, 0.31, 1.02, 5.5},
 };
 
 double launch_time(const Pace &p, long tiles, double stages, int cus)
@@ -444,7 +444,7 @@ double launch_time(const Pace &p, long tiles, double stages, int cus)
 }
 
 // writing and reading the partial sums of a split, and the join's launch
-double join_time(double bytes) { return 4.0 + bytes / 4e6; }
+double join_time(double bytes) { return 5.0 + bytes / 4e6; }
 
 Plan make_plan(int dtype, long m, int n, long k, int segs, int batch, bool gated, bool aligned, int order_a, int order_b, int cus)
 {

@@ -35,10 +35,12 @@ template <int BM_, int BN_, int WM_, int WN_, int STAGES, int PER_CU> struct Sha
 using Large = Shape<256, 256, 2, 4, 4, 1>;
 using Medium = Shape<256, 128, 4, 2, 6, 1>;
 using Small = Shape<128, 128, 4, 2, 4, 2>;
-// (Small where it is alone on its CU and k is long: 4096 x 8192 x 1024 bf16 77 us against 82)
-using Deep = Shape<128, 128, 4, 2, 8, 1>;
 // (one MFMA tile per wave: a product of 1024 x 1024 x 1024 fp32 27 us, with two tiles on half as many waves 42)
 using Tiny = Shape<64, 64, 2, 2, 4, 4>;
+// Where few workgroups share a CU and k is long, twice the stages cover the latency that the neighbours would have covered
+// (16 bits, k from 40 stages on: 4096 x 8192 x 1024 77 us against 82, 1088 x 2000 x 512 15.6 against 20.4; at 34 stages as fast)
+using SmallDeep = Shape<128, 128, 4, 2, 8, 1>;
+using TinyDeep = Shape<64, 64, 2, 2, 8, 2>;
 
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"             // (m0 is reserved: nothing here indexes registers through it)
@@ -396,7 +398,10 @@ template <class T> int launch_wide(const Args &p, int order_a, int order_b, bool
     if constexpr (sizeof(T) == 2) {                         // (fp32 is bound by its matrix rate with any tile)
         if (bn == 256) return launch_shape<T, Large>(p, order_a, order_b, gated, blocks, stream);
         if (bm == 256) return launch_shape<T, Medium>(p, order_a, order_b, gated, blocks, stream);
-        if (bm == 128 && blocks <= current_device_cus() && p.tiles_per_split >= 40) return launch_shape<T, Deep>(p, order_a, order_b, gated, blocks, stream);
+        if (p.tiles_per_split >= 40 && blocks <= (bm == 128 ? 1 : 2) * (long)current_device_cus()) {
+            if (bm == 128) return launch_shape<T, SmallDeep>(p, order_a, order_b, gated, blocks, stream);
+            return launch_shape<T, TinyDeep>(p, order_a, order_b, gated, blocks, stream);
+        }
     }
     if (bm == 128) return launch_shape<T, Small>(p, order_a, order_b, gated, blocks, stream);
     return launch_shape<T, Tiny>(p, order_a, order_b, gated, blocks, stream);
