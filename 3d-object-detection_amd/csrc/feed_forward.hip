@@ -413,7 +413,7 @@ namespace {
 
 // The time of a launch of `tiles` workgroups of one shape, in us, from what these took on a 256-CU chip: a stage of k (32
 // sixteen-bit elements, 16 floats) with workgroups on few CUs, with one on every CU and with `per_cu` on every CU - the
-// sixteen-bit shapes share the L2's bandwidth, 50 bytes/ns and CU -, and what a round of workgroups costs besides (first loads,
+// sixteen-bit shapes are bound by what a CU receives from L2, 60 to 80 bytes/ns -, and what a round of workgroups costs besides (first loads,
 // epilogue).  Measured, bf16, k not split, us:   large  medium  small  tiny
 //   8192 x 4096 x 4096                             230     272    287   414
 //   4096 x 2048 x 2048                              51      41     42    58
