@@ -561,3 +561,46 @@ def test_overwritten_results_are_noticed(device):
     with torch.inference_mode():
         inside = torch.ones((4, 8), device=device)
         assert (F.dense(x, w, out=inside) == 8).all()
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("cols", [False, True])
+@pytest.mark.parametrize("rows,cin,n", [(4096, 544, 4096), (4096, 2048, 2048), (2048, 1312, 1408), (640, 1312, 640), (1088, 1999, 520), (512, 96, 512)])
+def test_every_tile_shape(device, t, cols, rows, cin, n):
+    """Sizes from which the choice of tile takes each shape, with even and odd numbers of stages and what is left of k: every
+    product of a step (with and without gates, and the one that ends in dg and du) relative to its norm.  A result has its
+    own rounding, u; dpre (dg, du) were rounded once, independent errors of at most u of each, which a product with independent
+    factors passes on as at most u of its norm: 2 u; sums as in test_larger_products."""
+    from fpn import feed_forward as F
+    dtype, u = TYPES[t]
+    g = torch.Generator(device=device).manual_seed(rows + cin)
+
+    def r(*shape, s=1.0):
+        return (torch.randn(shape, generator=g, device=device) * s).to(dtype)
+
+    def w(k, m):
+        return r(m, k, s=k ** -0.5).t() if cols else r(k, m, s=k ** -0.5)
+
+    def near(got, want, k, halves=1, factor=1, what=""):
+        off = float((got.double() - want).norm() / want.norm())
+        assert off <= halves * u + factor * 2.0 ** -24 * k ** 0.5, (what, off)
+    x, wg, wu, wd, dy, dh = r(rows, cin), w(cin, n), w(cin, n), w(n, cin), r(rows, cin), r(rows, n)
+    x6, wg6, wu6, wd6, dy6, dh6 = (v.double() for v in (x, wg, wu, wd, dy, dh))
+    gate6, up6 = x6 @ wg6, x6 @ wu6
+    sig = torch.sigmoid(gate6)
+    value, slope = gate6 * sig, sig * (1 + gate6 * (1 - sig))
+    near(F.dense(x, wg), gate6, cin, what="y")
+    dx, dw, _ = F.dense_grad(dh, x, wg)
+    near(dx, dh6 @ wg6.t(), n, what="dx")
+    near(dw, x6.t() @ dh6, rows, what="dw")
+    h, gate, up = F.gated(x, wg, wu, keep=True)
+    near(h, value * up6, cin, 1, 5, "h")
+    assert torch.equal(h, F.gated(x, wg, wu))
+    dh6 = dy6 @ wd6.t()
+    dg6, du6 = dh6 * up6 * slope, dh6 * value
+    dx, dwg, dwu, dbg, dbu = F.gated_grad(dy, x, wg, wu, gate, up, bias=True, w_down=wd)
+    near(dx, dg6 @ wg6.t() + du6 @ wu6.t(), 2 * n, 2, 10, "gated dx")
+    near(dwg, x6.t() @ dg6, rows, 2, 10, "dw_gate")
+    near(dwu, x6.t() @ du6, rows, 2, 10, "dw_up")
+    near(dbg, dg6.sum(0), rows, 1, 10, "dbias_gate")
+    near(dbu, du6.sum(0), rows, 1, 10, "dbias_up")
