@@ -604,3 +604,28 @@ def test_every_tile_shape(device, t, cols, rows, cin, n):
     near(dwu, x6.t() @ du6, rows, 2, 10, "dw_up")
     near(dbg, dg6.sum(0), rows, 1, 10, "dbias_gate")
     near(dbu, du6.sum(0), rows, 1, 10, "dbias_up")
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("cols", [False, True])
+@pytest.mark.parametrize("rows,cin,n", [(1, 2080, 4104), (3, 2048, 4096), (16, 2048, 2048), (20, 1040, 4096), (31, 96, 512), (50, 1024, 4128),
+                                        (5, 64, 8200), (27, 72, 8208), (64, 200, 8192), (512, 1024, 4096)])
+def test_few_rows_of_wide_weights(device, t, cols, rows, cin, n):
+    """Sizes that take the few-row kernel with each of its shapes (k split over workgroups among them), relative to the
+    results' norm as above; the residual may be the output."""
+    from fpn import feed_forward as F
+    dtype, u = TYPES[t]
+    g = torch.Generator(device=device).manual_seed(rows + cin)
+
+    def r(*shape, s=1.0):
+        return (torch.randn(shape, generator=g, device=device) * s).to(dtype)
+    x, bias, res = r(rows, cin), r(n), r(rows, n)
+    wg, wu = (r(n, cin, s=cin ** -0.5).t() if cols else r(cin, n, s=cin ** -0.5) for _ in range(2))
+    x6, wg6, wu6, bias6, res6 = (v.double() for v in (x, wg, wu, bias, res))
+
+    def near(got, want, factor):
+        assert float((got.double() - want).norm() / want.norm()) <= u + factor * 2.0 ** -24 * cin ** 0.5
+    gate = x6 @ wg6 + bias6
+    near(F.dense(x, wg, bias), gate, 1)
+    near(F.gated(x, wg, wu, bias), gate * torch.sigmoid(gate) * (x6 @ wu6), 5)
+    near(F.dense(x, wg, bias, "relu", res, out=res), torch.relu(gate) + res6, 1)
