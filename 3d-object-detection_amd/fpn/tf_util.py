@@ -105,15 +105,15 @@ def dropout(inputs, is_training, scope, keep_prob=0.5, noise_shape=None):
 
 
 def _projection(scope, cin, cout, use_bias, dtype):
-    """A layer's weights (cin, cout) and bias, in the type of its inputs."""
+    """A layer's weights (cin, cout) and bias, in the type of its inputs.
+
+    The store holds float32, so 16-bit inputs cost a cast of each variable per call.  It is not kept: a variable may be
+    trained, written in place or read in a capture or on another stream between two calls, and only a cast of the call's own is
+    right in all of these.  A program that keeps 16-bit weights calls feed_forward with them."""
     store = variables.get_default_store()
     name = variables.scoped(scope)
-    kept = [(name + "/weights", (cin, cout), "xavier")]
-    if use_bias:
-        kept.append((name + "/biases", (cout,), "zeros"))
-    held = [(key, store.get_variable(key, shape, init)) for key, shape, init in kept]
-    cast = [v if dtype == torch.float32 else store.cached(("cast", key, dtype), lambda v=v: v.to(dtype)) for key, v in held]
-    return cast[0], cast[1] if use_bias else None
+    w = store.get_variable(name + "/weights", (cin, cout), "xavier").to(dtype)
+    return w, store.get_variable(name + "/biases", (cout,), "zeros").to(dtype) if use_bias else None
 
 
 def _as_rows(t):

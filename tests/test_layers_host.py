@@ -1,0 +1,64 @@
+"""tf_util's dense layers: what they take from the variable store and which arguments they refuse, decided on the host."""
+import pytest
+import torch
+
+from fpn import tf_util, variables
+
+
+def store_with(weights, biases):
+    store = variables.VariableStore("cpu")
+    store["layer/weights"], store["layer/biases"] = weights, biases
+    return store
+
+
+def hold(store, name, parameter):
+    """A trained parameter in the store itself, as a program that trains the layer holds it."""
+    store._vars[name] = parameter
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_a_layer_sees_its_variables_as_they_are_now(dtype):
+    """Updated in place (an optimiser's step, .data, the store's own tensor), by assignment, or replaced."""
+    store = store_with(torch.ones(4, 3), torch.zeros(3))
+    with variables.use_store(store):
+        w, b = tf_util._projection("layer", 4, 3, True, dtype)
+        assert w.dtype is dtype and b.dtype is dtype and (w == 1).all() and not b.any()
+        with torch.no_grad():
+            store["layer/weights"].add_(1)
+            store["layer/biases"].fill_(5)
+        w, b = tf_util._projection("layer", 4, 3, True, dtype)
+        assert (w == 2).all() and (b == 5).all()
+        store["layer/weights"].data.fill_(7)                # (leaves the version counter as it was)
+        assert (tf_util._projection("layer", 4, 3, True, dtype)[0] == 7).all()
+        hold(store, "layer/weights", torch.nn.Parameter(torch.full((4, 3), 3.0)))
+        assert (tf_util._projection("layer", 4, 3, True, dtype)[0] == 3).all()
+        step = torch.optim.SGD([store["layer/weights"]], lr=1.0)
+        store["layer/weights"].grad = torch.ones(4, 3)
+        step.step()
+        assert (tf_util._projection("layer", 4, 3, True, dtype)[0] == 2).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+def test_a_first_call_without_gradients_does_not_cost_later_ones_theirs(dtype, mode):
+    store = store_with(torch.ones(4, 3), torch.zeros(3))
+    for name in ("layer/weights", "layer/biases"):
+        hold(store, name, torch.nn.Parameter(store[name].clone()))
+    with variables.use_store(store):
+        with mode():
+            tf_util._projection("layer", 4, 3, True, dtype)
+        for _ in range(2):                                  # (a second step has a graph of its own)
+            w, b = tf_util._projection("layer", 4, 3, True, dtype)
+            assert w.requires_grad and b.requires_grad and not w.is_inference()
+            (w.float().sum() + b.float().sum()).backward()
+        assert (store["layer/weights"].grad == 2).all() and (store["layer/biases"].grad == 2).all()
+
+
+def test_frozen_variables_after_inference_mode():
+    """A cast that inference mode made could not be saved for a backward pass of the points."""
+    store = store_with(torch.ones(4, 3), torch.zeros(3))
+    with variables.use_store(store):
+        with torch.inference_mode():
+            tf_util._projection("layer", 4, 3, True, torch.bfloat16)
+        w, _ = tf_util._projection("layer", 4, 3, True, torch.bfloat16)
+    assert not w.is_inference()
