@@ -38,7 +38,12 @@ class VariableStore:
         t = torch.as_tensor(value, dtype=torch.float32)
         if t.dim() == 4 and t.shape[0] == 1 and t.shape[1] == 1:   # TF conv kernel (1,1,Cin,Cout)
             t = t.reshape(t.shape[2], t.shape[3])
-        self._vars[name] = t.to(self.device).contiguous()
+        t = t.to(self.device).contiguous()
+        if t.is_inference():
+            # (a variable outlives the mode it was made in; as an inference tensor it could not be saved for a backward pass)
+            with torch.inference_mode(False), torch.no_grad():
+                t = t.clone()
+        self._vars[name] = t
         self.version += 1
         self._cache.clear()
 

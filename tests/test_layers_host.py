@@ -62,3 +62,16 @@ def test_frozen_variables_after_inference_mode():
             tf_util._projection("layer", 4, 3, True, torch.bfloat16)
         w, _ = tf_util._projection("layer", 4, 3, True, torch.bfloat16)
     assert not w.is_inference()
+
+
+def test_variables_made_inside_inference_mode_are_ordinary_tensors():
+    """A layer's first call makes its variables: made in inference mode they could never be saved for a backward pass."""
+    store = variables.VariableStore("cpu")
+    with variables.use_store(store):
+        with torch.inference_mode():
+            tf_util._projection("layer", 4, 3, True, torch.float32)
+            store["given"] = torch.ones(2)
+        for name in ("layer/weights", "layer/biases", "given"):
+            assert not store[name].is_inference(), name
+        w, _ = tf_util._projection("layer", 4, 3, True, torch.float32)
+        (torch.ones(2, 4, requires_grad=True) @ w).sum().backward()
