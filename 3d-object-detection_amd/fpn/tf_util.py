@@ -123,12 +123,21 @@ def _as_rows(t):
     return t if t.dim() == 2 else t.flatten(0, -2)
 
 
+def _residual_rows(residual, inputs, num_outputs):
+    """A residual's rows: (..., num_outputs) with the inputs' leading dimensions, or the matrix of all rows."""
+    if residual is None:
+        return None
+    if residual.shape[-1:] != (num_outputs,) or residual.dim() != 2 and residual.shape[:-1] != inputs.shape[:-1]:
+        raise ValueError("residual has shape %s, expected %s" % (tuple(residual.shape), tuple(inputs.shape[:-1]) + (num_outputs,)))
+    return _as_rows(residual)
+
+
 def dense(inputs, num_outputs, scope, activation=None, residual=None, use_bias=True):
     """act(inputs W + b) + residual over the last dimension (feed_forward.dense): inputs (..., C), residual and result
     (..., num_outputs), all of one type; activation by name (feed_forward.ACTIVATIONS)."""
     x = _as_rows(inputs)
     w, b = _projection(scope, x.shape[1], num_outputs, use_bias, x.dtype)
-    y = feed_forward.dense(x, w, b, activation, None if residual is None else _as_rows(residual))
+    y = feed_forward.dense(x, w, b, activation, _residual_rows(residual, inputs, num_outputs))
     return y.reshape(inputs.shape[:-1] + (num_outputs,))
 
 
@@ -142,5 +151,5 @@ def gated_feed_forward(inputs, num_hidden, scope, num_outputs=None, activation="
     wg, bg = _projection(scope + "/gate", x.shape[1], num_hidden, use_bias, x.dtype)
     wu, bu = _projection(scope + "/up", x.shape[1], num_hidden, use_bias, x.dtype)
     wd, bd = _projection(scope + "/down", num_hidden, num_outputs, use_bias, x.dtype)
-    y = feed_forward.gated_feed_forward(x, wg, wu, wd, bg, bu, bd, activation, None if residual is None else _as_rows(residual))
+    y = feed_forward.gated_feed_forward(x, wg, wu, wd, bg, bu, bd, activation, _residual_rows(residual, inputs, num_outputs))
     return y.reshape(inputs.shape[:-1] + (num_outputs,))

@@ -75,3 +75,22 @@ def test_variables_made_inside_inference_mode_are_ordinary_tensors():
             assert not store[name].is_inference(), name
         w, _ = tf_util._projection("layer", 4, 3, True, torch.float32)
         (torch.ones(2, 4, requires_grad=True) @ w).sum().backward()
+
+
+@pytest.mark.parametrize("points,residual", [((4, 8, 5), (8, 4, 3)), ((4, 8, 5), (2, 16, 3)), ((4, 8, 5), (1, 4, 8, 3)), ((32, 5), (4, 8, 3)),
+                                             ((4, 8, 5), (4, 8, 2))])
+def test_a_residual_of_other_rows_is_refused(points, residual):
+    """As many rows, but not the inputs' own: adding them row by row would pair the wrong ones."""
+    with variables.use_store(variables.VariableStore("cpu")):
+        with pytest.raises(ValueError, match="residual has shape"):
+            tf_util.dense(torch.zeros(points), 3, "layer", residual=torch.zeros(residual))
+        with pytest.raises(ValueError, match="residual has shape"):
+            tf_util.gated_feed_forward(torch.zeros(points), 6, "block", num_outputs=3, residual=torch.zeros(residual))
+
+
+@pytest.mark.parametrize("points,residual", [((4, 8, 5), (4, 8, 3)), ((4, 8, 5), (32, 3)), ((32, 5), (32, 3))])
+def test_a_residual_of_the_same_rows_passes_the_check(points, residual):
+    """(a matrix of all rows is the same rows; behind the check comes the refusal of host tensors)"""
+    with variables.use_store(variables.VariableStore("cpu")):
+        with pytest.raises(ValueError, match="ROCm device"):
+            tf_util.dense(torch.zeros(points), 3, "layer", residual=torch.zeros(residual))
