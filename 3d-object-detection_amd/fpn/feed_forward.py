@@ -14,8 +14,10 @@ Gradients, either way:
   * `keep=True` returns what the backward pass needs beside the result, and `dense_grad` / `gated_grad` are that pass.
     This is the form for HIP graphs: recording through autograd while a graph is being captured is refused, since
     autograd would join streams that the capture does not know.
+There are no forward-mode derivatives: a tensor that carries a tangent is refused.
 """
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -30,10 +32,17 @@ def _activation(name):
         raise ValueError("activation must be one of %s, got %r" % (", ".join(repr(a) for a in ACTIVATIONS), name)) from None
 
 
+def _no_tangent(name, t):
+    """Refuses a tensor of forward-mode differentiation: it has a value like any other, and the result would lack a tangent."""
+    if forward_ad._current_level >= 0 and isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+        raise NotImplementedError("%s carries a tangent: the feed-forward operators have no forward-mode derivatives" % name)
+
+
 def _tensor(name, t, like, shape):
     """The checks that every argument gets: a tensor of the call's type, on its device, of this shape."""
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s must be a torch.Tensor, got %s" % (name, type(t).__name__))
+    _no_tangent(name, t)
     if t.dtype is not like.dtype:
         raise ValueError("%s must be %s like x, got %s" % (name, like.dtype, t.dtype))
     if not t.is_cuda:
@@ -47,6 +56,7 @@ def _tensor(name, t, like, shape):
 def _first(name, x):
     if not isinstance(x, torch.Tensor):
         raise TypeError("%s must be a torch.Tensor, got %s" % (name, type(x).__name__))
+    _no_tangent(name, x)
     if x.dim() != 2:
         raise ValueError("%s must have rank 2, got shape %s" % (name, tuple(x.shape)))
     if x.dtype not in _DTYPES:
@@ -258,6 +268,7 @@ def dense_grad(dy, x, w, pre=None, activation=None, bias=False, need_x=True, nee
 
 def _kept(name, t, x, shape):
     """The row stride of a pre-activation that a forward pass kept."""
+    _no_tangent(name, t)
     if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or not t.is_cuda or t.get_device() != x.get_device() or t.shape != shape:
         raise ValueError("%s must be the float32 %s tensor on %s that keep=True returned" % (name, tuple(shape), x.device))
     return _rows(name, t)
@@ -396,6 +407,10 @@ class _Gated(torch.autograd.Function):
 def gated_feed_forward(x, w_gate, w_up, w_down, bias_gate=None, bias_up=None, bias_down=None, activation="silu", residual=None,
                        out=None):
     """y = gated(x) w_down + bias_down + residual: `gated` and then `dense` with the residual in its epilogue."""
+    if forward_ad._current_level >= 0:                       # (before anything is recorded or launched)
+        for name, t in (("x", x), ("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down), ("bias_gate", bias_gate),
+                        ("bias_up", bias_up), ("bias_down", bias_down), ("residual", residual), ("out", out)):
+            _no_tangent(name, t)
     if isinstance(x, torch.Tensor) and isinstance(w_down, torch.Tensor) and \
             _recorded(x, w_gate, w_up, w_down, bias_gate, bias_up, bias_down, residual):
         if out is not None:
