@@ -159,6 +159,8 @@ def _whole(dtype, widths, *operands):
     for n in widths:
         bits |= n
     for t, ld in operands:
+        if t is None:
+            continue
         bits |= ld
         if t.data_ptr() & 15:
             return 0
@@ -255,14 +257,23 @@ def dense_grad(dy, x, w, pre=None, activation=None, bias=False, need_x=True, nee
         if pre is None:
             raise ValueError("pre (from dense(..., keep=True)) is needed where there is an activation")
         ldp = _kept("pre", pre, x, (rows, cout))
+    return _dense_backward(dtype, (rows, cin, cout), dy, lddy, x if need_w else None, ldx, w if need_x else None, ldw, transposed,
+                           pre if act else None, ldp, act, bias, need_x, need_w)
+
+
+def _dense_backward(dtype, sizes, dy, lddy, x, ldx, w, ldw, transposed, pre, ldp, act, bias, need_x, need_w):
+    """The call of dense_grad: x is there for dw only, w for dx only."""
+    lib = _lib.load()
+    rows, cin, cout = sizes
     with torch.no_grad():
-        dx = torch.empty((rows, cin), dtype=x.dtype, device=x.device) if need_x else None
-        dw = _like_weights(w, transposed) if need_w else None
-        db = torch.empty(cout, dtype=x.dtype, device=x.device) if bias else None
-    size = lib.fpn_dense_grad_workspace_bytes(dtype, rows, cin, cout, act, _whole(dtype, (cin, cout), (x, ldx), (w, ldw), (dy, lddy)))
-    ws = _workspace(size, x)
-    _call(x, lib.fpn_dense_grad, dtype, rows, cin, cout, _p(dy), lddy, _p(x), ldx, _p(w), ldw, transposed, _p(pre) if act else None, ldp,
-          act, _p(dx), cin, _p(dw), cin if transposed else cout, _p(db), _p(ws), size)
+        dx = torch.empty((rows, cin), dtype=dy.dtype, device=dy.device) if need_x else None
+        dw = _weight_gradient(dy, cin, cout, transposed) if need_w else None
+        db = torch.empty(cout, dtype=dy.dtype, device=dy.device) if bias else None
+    whole = _whole(dtype, (cin, cout), (x, ldx), (w, ldw), (dy, lddy))
+    size = lib.fpn_dense_grad_workspace_bytes(dtype, rows, cin, cout, act, whole)
+    ws = _workspace(size, dy)
+    _call(dy, lib.fpn_dense_grad, dtype, rows, cin, cout, _p(dy), lddy, _p(x), ldx, _p(w), ldw, transposed, _p(pre), ldp, act, _p(dx), cin,
+          _p(dw), cin if transposed else cout, _p(db), _p(ws), size)
     return dx, dw, db
 
 
@@ -274,11 +285,11 @@ def _kept(name, t, x, shape):
     return _rows(name, t)
 
 
-def _like_weights(w, transposed):
-    cin, cout = w.shape
+def _weight_gradient(like, cin, cout, transposed):
+    """A (cin, cout) matrix in the weights' storage order."""
     if transposed:
-        return torch.empty((cout, cin), dtype=w.dtype, device=w.device).t()
-    return torch.empty((cin, cout), dtype=w.dtype, device=w.device)
+        return torch.empty((cout, cin), dtype=like.dtype, device=like.device).t()
+    return torch.empty((cin, cout), dtype=like.dtype, device=like.device)
 
 
 def _dense_rows(t):
@@ -289,11 +300,19 @@ def _dense_rows(t):
 
 
 class _Dense(torch.autograd.Function):
+    """Keeps what the gradients that will be asked for are formed from, and nothing else."""
+
     @staticmethod
     def forward(ctx, x, w, bias, activation, residual):
-        y, pre = dense(x, w, bias, activation, residual, keep=True)
-        ctx.save_for_backward(x, w, pre)
-        ctx.activation = activation
+        need_x, need_w, need_b, _, _ = ctx.needs_input_grad
+        act = ACTIVATIONS[activation]
+        pre = None
+        if act and (need_x or need_w or need_b):
+            y, pre = dense(x, w, bias, activation, residual, keep=True)
+        else:
+            y = dense(x, w, bias, activation, residual)
+        ctx.save_for_backward(x if need_w else None, w if need_x else None, pre)
+        ctx.layout = _DTYPES[x.dtype], (x.shape[0], x.shape[1], w.shape[1]), _weights(("w",), (w,))[0], act
         return y
 
     @staticmethod
@@ -304,8 +323,25 @@ class _Dense(torch.autograd.Function):
         need_x, need_w, need_b, _, need_r = ctx.needs_input_grad
         dx = dw = db = None
         if need_x or need_w or need_b:
-            dx, dw, db = dense_grad(_dense_rows(dy), x, w, pre, ctx.activation, need_b, need_x, need_w)
+            dx, dw, db = _dense_gradients(ctx.layout, _dense_rows(dy), x if need_w else None, w if need_x else None, pre, need_b)
         return dx, dw, db, None, dy if need_r else None
+
+
+def _dense_gradients(layout, dy, x, w, pre, bias):
+    """dense_grad on what an autograd function kept: dw where x is given, dx where w is.  (Hooks on saved tensors may have
+    brought back copies laid out otherwise.)"""
+    dtype, (rows, cin, cout), transposed, act = layout
+    _tensor("dy", dy, dy, (rows, cout))
+    ldx = ldw = 0
+    if x is not None:
+        _tensor("x", x, dy, (rows, cin))
+        ldx = _rows("x", x, broadcast=True)
+    if w is not None:
+        _tensor("w", w, dy, (cin, cout))
+        transposed, (ldw,) = _weights(("w",), (w,))
+    ldp = _kept("pre", pre, dy, (rows, cout)) if act else cout
+    return _dense_backward(dtype, (rows, cin, cout), dy, _rows("dy", dy), x, ldx, w, ldw, transposed, pre if act else None, ldp, act, bias,
+                           w is not None, x is not None)
 
 
 # ---- gated ---------------------------------------------------------------------------------------------------------
@@ -369,37 +405,79 @@ def gated_grad(dh, x, w_gate, w_up, gate, up, activation="silu", bias=False, nee
         raise ValueError("gate and up must have the same row stride")
     lddh, ldx = _rows("dh", dh), _rows("x", x, broadcast=True)
     transposed, (ldg, ldu) = _weights(("w_gate", "w_up"), (w_gate, w_up))
+    return _gated_backward(dtype, (rows, cin, cout, cdown), dh, lddh, w_down, ldd, down_transposed, x if need_w else None, ldx,
+                           (w_gate, w_up) if need_x else (None, None), (ldg, ldu), transposed, gate, up, ldp, act, bias, need_x, need_w)
+
+
+def _gated_backward(dtype, sizes, dh, lddh, w_down, ldd, down_transposed, x, ldx, ws, lds, transposed, gate, up, ldp, act, bias, need_x,
+                    need_w):
+    """The call of gated_grad: x is there for the weights' gradients only, the weights `ws` for dx only."""
+    lib = _lib.load()
+    rows, cin, cout, cdown = sizes
     with torch.no_grad():
-        dx = torch.empty((rows, cin), dtype=x.dtype, device=x.device) if need_x else None
-        dwg, dwu = (_like_weights(w_gate, transposed) for _ in range(2)) if need_w else (None, None)
-        dbg, dbu = (torch.empty(cout, dtype=x.dtype, device=x.device) for _ in range(2)) if bias else (None, None)
-    whole = _whole(dtype, (cin, cout, cdown), (x, ldx), (w_gate, ldg), (w_up, ldu), (dh, lddh)) and \
-        (not cdown or _whole(dtype, (), (w_down, ldd)))
-    size = lib.fpn_gated_grad_workspace_bytes(dtype, rows, cin, cout, cdown, int(whole))
-    ws = _workspace(size, x)
-    _call(x, lib.fpn_gated_grad, dtype, rows, cin, cout, cdown, _p(dh), lddh, _p(w_down), ldd, down_transposed, _p(x), ldx, _p(w_gate),
-          ldg, _p(w_up), ldu, transposed, _p(gate), _p(up), ldp, act, _p(dx), cin, _p(dwg), _p(dwu), cin if transposed else cout,
-          _p(dbg), _p(dbu), _p(ws), size)
+        dx = torch.empty((rows, cin), dtype=dh.dtype, device=dh.device) if need_x else None
+        dwg, dwu = (_weight_gradient(dh, cin, cout, transposed) for _ in range(2)) if need_w else (None, None)
+        dbg, dbu = (torch.empty(cout, dtype=dh.dtype, device=dh.device) for _ in range(2)) if bias else (None, None)
+    whole = _whole(dtype, (cin, cout, cdown), (x, ldx), (ws[0], lds[0]), (ws[1], lds[1]), (dh, lddh), (w_down, ldd))
+    size = lib.fpn_gated_grad_workspace_bytes(dtype, rows, cin, cout, cdown, whole)
+    space = _workspace(size, dh)
+    _call(dh, lib.fpn_gated_grad, dtype, rows, cin, cout, cdown, _p(dh), lddh, _p(w_down), ldd, down_transposed, _p(x), ldx, _p(ws[0]),
+          lds[0], _p(ws[1]), lds[1], transposed, _p(gate), _p(up), ldp, act, _p(dx), cin, _p(dwg), _p(dwu), cin if transposed else cout,
+          _p(dbg), _p(dbu), _p(space), size)
     return dx, dwg, dwu, dbg, dbu
 
 
 class _Gated(torch.autograd.Function):
+    """Keeps what the gradients that will be asked for are formed from, and nothing else."""
+
     @staticmethod
     def forward(ctx, x, w_gate, w_up, bias_gate, bias_up, activation):
+        need_x, need_g, need_u = ctx.needs_input_grad[:3]
         h, gate, up = gated(x, w_gate, w_up, bias_gate, bias_up, activation, keep=True)
-        ctx.save_for_backward(x, w_gate, w_up, gate, up)
-        ctx.activation = activation
+        ctx.save_for_backward(x if need_g or need_u else None, w_gate if need_x else None, w_up if need_x else None, None, gate, up)
+        ctx.layout = _gated_layout(x, w_gate, w_up, 0, activation)
         return h
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
         _no_capture()
-        x, w_gate, w_up, gate, up = ctx.saved_tensors
-        need_x, need_g, need_u, need_bg, need_bu, _ = ctx.needs_input_grad
-        dx, dwg, dwu, dbg, dbu = gated_grad(_dense_rows(dh), x, w_gate, w_up, gate, up, ctx.activation, need_bg or need_bu, need_x,
-                                            need_g or need_u)
-        return dx, dwg if need_g else None, dwu if need_u else None, dbg if need_bg else None, dbu if need_bu else None, None
+        return _gated_gradients(ctx.layout, _dense_rows(dh), ctx.saved_tensors, ctx.needs_input_grad[:5]) + (None,)
+
+
+def _gated_layout(x, w_gate, w_up, cdown, activation):
+    """(dtype, sizes, storage order of the gated weights, activation) of a recorded call."""
+    return (_DTYPES[x.dtype], (x.shape[0], x.shape[1], w_gate.shape[1], cdown), _weights(("w_gate", "w_up"), (w_gate, w_up))[0],
+            ACTIVATIONS[activation])
+
+
+def _gated_gradients(layout, dh, saved, needs):
+    """gated_grad on what an autograd function kept: the gradients of x, w_gate, w_up, bias_gate and bias_up that are asked
+    for."""
+    dtype, sizes, transposed, act = layout
+    rows, cin, cout, cdown = sizes
+    x, w_gate, w_up, w_down, gate, up = saved
+    need_x, need_g, need_u, need_bg, need_bu = needs
+    need_w = need_g or need_u
+    _tensor("dh", dh, dh, (rows, cdown or cout))
+    ldx, lds, ldd, down_transposed = 0, (0, 0), 0, 0
+    if need_w:
+        _tensor("x", x, dh, (rows, cin))
+        ldx = _rows("x", x, broadcast=True)
+    if need_x:
+        _tensor("w_gate", w_gate, dh, (cin, cout))
+        _tensor("w_up", w_up, dh, (cin, cout))
+        transposed, lds = _weights(("w_gate", "w_up"), (w_gate, w_up))
+    if cdown:
+        _tensor("w_down", w_down, dh, (cout, cdown))
+        down_transposed, (ldd,) = _weights(("w_down",), (w_down,))
+    ldp = _kept("gate", gate, dh, (rows, cout))
+    if _kept("up", up, dh, (rows, cout)) != ldp:
+        raise ValueError("gate and up must have the same row stride")
+    dx, dwg, dwu, dbg, dbu = _gated_backward(dtype, sizes, dh, _rows("dh", dh), w_down, ldd, down_transposed, x if need_w else None, ldx,
+                                             (w_gate, w_up) if need_x else (None, None), lds, transposed, gate, up, ldp, act,
+                                             need_bg or need_bu, need_x, need_w)
+    return dx, dwg if need_g else None, dwu if need_u else None, dbg if need_bg else None, dbu if need_bu else None
 
 
 # ---- the block -----------------------------------------------------------------------------------------------------
@@ -421,26 +499,36 @@ def gated_feed_forward(x, w_gate, w_up, w_down, bias_gate=None, bias_up=None, bi
 
 
 class _GatedFeedForward(torch.autograd.Function):
+    """Keeps what the gradients that will be asked for are formed from, and nothing else."""
+
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, bias_gate, bias_up, bias_down, activation, residual):
-        h, gate, up = gated(x, w_gate, w_up, bias_gate, bias_up, activation, keep=True)
-        y, _ = dense(h, w_down, bias_down, None, residual, keep=True)
-        ctx.save_for_backward(x, w_gate, w_up, w_down, h, gate, up)
-        ctx.activation = activation
+        need_x, need_g, need_u, need_d, need_bg, need_bu = ctx.needs_input_grad[:6]
+        gate = up = None
+        through = need_x or need_g or need_u or need_bg or need_bu       # (a gradient goes back through h)
+        if through:
+            h, gate, up = gated(x, w_gate, w_up, bias_gate, bias_up, activation, keep=True)
+        else:
+            h = gated(x, w_gate, w_up, bias_gate, bias_up, activation)
+        y = dense(h, w_down, bias_down, None, residual)
+        ctx.save_for_backward(x if need_g or need_u else None, w_gate if need_x else None, w_up if need_x else None,
+                              w_down if through else None, gate, up, h if need_d else None)
+        ctx.layout = _gated_layout(x, w_gate, w_up, w_down.shape[1], activation)
+        ctx.down_transposed = _weights(("w_down",), (w_down,))[0]
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         _no_capture()
-        x, w_gate, w_up, w_down, h, gate, up = ctx.saved_tensors
+        *saved, h = ctx.saved_tensors
         need_x, need_g, need_u, need_d, need_bg, need_bu, need_bd, _, need_r = ctx.needs_input_grad
+        dtype, (rows, _, hidden, cout), _, _ = ctx.layout
         dx = dwg = dwu = dwd = dbg = dbu = dbd = None
         d = _dense_rows(dy)
         if need_d or need_bd:
-            _, dwd, dbd = dense_grad(d, h, w_down, None, None, need_bd, False, need_d)
+            layout = dtype, (rows, hidden, cout), ctx.down_transposed, 0
+            _, dwd, dbd = _dense_gradients(layout, d, h if need_d else None, None, None, need_bd)
         if need_x or need_g or need_u or need_bg or need_bu:
-            dx, dwg, dwu, dbg, dbu = gated_grad(d, x, w_gate, w_up, gate, up, ctx.activation, need_bg or need_bu, need_x,
-                                                need_g or need_u, w_down)
-        return (dx, dwg if need_g else None, dwu if need_u else None, dwd, dbg if need_bg else None, dbu if need_bu else None, dbd, None,
-                dy if need_r else None)
+            dx, dwg, dwu, dbg, dbu = _gated_gradients(ctx.layout, d, saved, (need_x, need_g, need_u, need_bg, need_bu))
+        return dx, dwg, dwu, dwd, dbg, dbu, dbd, None, dy if need_r else None
