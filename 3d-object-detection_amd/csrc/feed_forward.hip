@@ -200,7 +200,9 @@ int run_product(int dtype, const Args &p, int order_a, int order_b, bool gated, 
 
 constexpr int kStretchBytes = 64;             // of k per stage of the wide kernel
 constexpr long kMostLd = (1l << 21) - 1;      // a tile's byte offsets inside an operand are 32 bits
-constexpr long kMostRows = 1l << 40;          // (products of sizes stay inside 64 bits)
+// Rows times the widest row of floats are 2^61 bytes, and the largest workspace (dg, du, dh and the copies of x and dy: five
+// such matrices) and every byte offset stay inside 64 bits.  No gradient of more rows would fit a card.
+constexpr long kMostRows = 1l << 38;
 
 int check_common(int dtype, long rows, int cin, int cout, int activation)
 {
