@@ -869,6 +869,8 @@ struct Plan {
     long tiles_per_split;
     size_t partial_bytes;
 };
+// threads of a workgroup of the pipelined kernel's shapes, which have BM output rows
+constexpr int wide_threads(int bm) { return bm == 64 ? 256 : 512; }
 // (aligned: every operand consists of whole 16-byte chunks at 16-byte addresses)
 Plan plan_product(int dtype, long m, int n, long k, int segs, int batch, bool gated, bool aligned, int order_a, int order_b);
 
@@ -880,6 +882,13 @@ inline bool whole_chunks(const void *p, long ld, int order, long extent, int ele
 
 template <class T> int launch_few(const Args &p, int order_b, bool gated, int mt, int nt, hipStream_t stream);
 template <class T> int launch_wide(const Args &p, int order_a, int order_b, bool gated, int bm, int bn, long blocks, hipStream_t stream);
+
+// workgroups of a planned product (of the tiled kernels)
+inline long plan_blocks(const Args &p, bool gated, const Plan &plan)
+{
+    const int cols = gated ? plan.bn / 2 : plan.bn;
+    return (p.m + plan.bm - 1) / plan.bm * ((p.n + cols - 1) / cols) * plan.splits * p.batch;
+}
 
 // Launches a planned product (p.partial and the plan's fields are filled in here)
 template <class T> int launch_product(Args p, int order_a, int order_b, bool gated, const Plan &plan, float *partial, hipStream_t stream);
@@ -951,7 +960,7 @@ template <class T> int launch_product(Args p, int order_a, int order_b, bool gat
     const int cols = gated ? plan.bn / 2 : plan.bn;
     p.mt = (p.m + plan.bm - 1) / plan.bm;
     p.nt = (p.n + cols - 1) / cols;
-    const long blocks = p.mt * p.nt * p.splits * p.batch;
+    const long blocks = plan_blocks(p, gated, plan);
     int rc;
     if (plan.wide) rc = launch_wide<T>(p, order_a, order_b, gated, plan.bm, plan.bn, blocks, stream);
     else if (plan.bm == 128) rc = launch_tiles<T, 128, 128, 2, 2>(p, order_a, order_b, gated, blocks, stream);

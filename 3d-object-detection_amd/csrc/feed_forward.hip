@@ -198,6 +198,14 @@ int run_product(int dtype, const Args &p, int order_a, int order_b, bool gated, 
     return launch_product<_Float16>(p, order_a, order_b, gated, plan, partial, stream);
 }
 
+// Whether a product's grid fits one launch.  An entry point asks this of all its products before it launches anything.
+int check_product(int dtype, const Args &p, int order_a, int order_b, bool gated)
+{
+    const Plan plan = plan_of(dtype, p, order_a, order_b, gated);
+    if (plan.few) return FPN_OK;                  // (widths below 2^21: at most 2^29 threads)
+    return check_grid(plan_blocks(p, gated, plan), plan.wide ? wide_threads(plan.bm) : kThreads);
+}
+
 constexpr int kStretchBytes = 64;             // of k per stage of the wide kernel
 constexpr long kMostLd = (1l << 21) - 1;      // a tile's byte offsets inside an operand are 32 bits
 // Rows times the widest row of floats are 2^61 bytes, and the largest workspace (dg, du, dh and the copies of x and dy: five
@@ -353,12 +361,11 @@ Args product(long m, int n, long k)
     return p;
 }
 
-// dw = x^T d for one or two d, in the weights' own storage order
-int weight_gradients(int dtype, const Matrix &x, const Matrix (&d)[2], int members, void *const (&dw)[2], long lddw, int transposed,
-                     float *partial, size_t partial_bytes, hipStream_t stream)
+// dw = x^T d for one or two d, in the weights' own storage order: one product or two
+int weight_products(const Matrix &x, const Matrix (&d)[2], int members, void *const (&dw)[2], long lddw, int transposed, Args (&out)[2])
 {
     if (!transposed) {
-        Args p = product(x.cols, d[0].cols, x.rows);
+        Args &p = out[0] = product(x.cols, d[0].cols, x.rows);
         p.load_m = x.wide;
         p.load_n = (int)d[0].wide;
         p.a[0] = x.p;
@@ -366,11 +373,11 @@ int weight_gradients(int dtype, const Matrix &x, const Matrix (&d)[2], int membe
         p.batch = members;
         for (int i = 0; i < members; ++i) { p.b[i] = d[i].p; p.ldb[i] = d[i].ld; p.c[i] = dw[i]; }
         p.ldc = lddw;
-        return run_product(dtype, p, kOuter, kOuter, false, partial, partial_bytes, stream);
+        return 1;
     }
     // held (out,in): the operands change places (one product each, x is the b side of both)
     for (int i = 0; i < members; ++i) {
-        Args p = product(d[i].cols, x.cols, x.rows);
+        Args &p = out[i] = product(d[i].cols, x.cols, x.rows);
         p.load_m = d[i].wide;
         p.load_n = (int)x.wide;
         p.a[0] = d[i].p;
@@ -379,9 +386,8 @@ int weight_gradients(int dtype, const Matrix &x, const Matrix (&d)[2], int membe
         p.ldb[0] = x.ld;
         p.c[0] = dw[i];
         p.ldc = lddw;
-        FPN_FF_TRY(run_product(dtype, p, kOuter, kOuter, false, partial, partial_bytes, stream));
     }
-    return FPN_OK;
+    return members;
 }
 
 // the operands of a forward product (or two, gated)
@@ -561,13 +567,13 @@ int fpn_dense(int dtype, long rows, int cin, int cout, const void *x, long ldx, 
     const hipStream_t st = as_stream(stream);
     Matrix mx = {x, ldx, rows, cin, cin}, mw = weights(w, ldw, cin, cout, w_transposed);
     size_t partial_space = workspace_bytes;
+    Copies copies(dtype, nullptr, 0);
     if (worth_copies(rows, cin, cout)) {
         const size_t partial = align256(partial_bytes(dtype, rows, cout, cin, 1, 1, false, kInner));
         if (workspace && workspace_bytes > partial) {
-            Copies copies(dtype, reinterpret_cast<char *>(workspace) + partial, workspace_bytes - partial);
+            copies = Copies(dtype, reinterpret_cast<char *>(workspace) + partial, workspace_bytes - partial);
             copies.take(mx, false);
             copies.take(mw, order_b == kOuter);
-            FPN_FF_TRY(copies.make(st));
             partial_space = partial;
         }
     }
@@ -582,6 +588,8 @@ int fpn_dense(int dtype, long rows, int cin, int cout, const void *x, long ldx, 
     p.ldc = ldy;
     p.pre[0] = pre;
     p.ldp = ldp;
+    FPN_FF_TRY(check_product(dtype, p, kInner, order_b, false));
+    FPN_FF_TRY(copies.make(st));
     return run_product(dtype, p, kInner, order_b, false, reinterpret_cast<float *>(workspace), partial_space, st);
 }
 
@@ -614,44 +622,50 @@ int fpn_dense_grad(int dtype, long rows, int cin, int cout, const void *dy, long
     const hipStream_t st = as_stream(stream);
 
     Matrix mx = {x, ldx, rows, cin, cin}, mw = weights(w, ldw, cin, cout, w_transposed), md[2] = {{dy, lddy, rows, cout, cout}, {}};
+    Copies copies(dtype, ws + space.total, workspace_bytes - space.total);
     if (worth_copies(rows, cin, cout)) {
-        Copies copies(dtype, ws + space.total, workspace_bytes - space.total);
         if (dw) copies.take(mx, true);
         if (dx) copies.take(mw, w_transposed);
         if (!act) copies.take(md[0], dw);
-        FPN_FF_TRY(copies.make(st));
     }
+    GradArgs g = {};
+    g.rows = rows;
+    g.n = cout;
+    g.dy = dy;
+    g.lddy = lddy;
+    g.pre[0] = pre;
+    g.ldp = ldp;
+    g.act = activation;
+    if (act) {
+        const long ldd = padded(dtype, cout);
+        g.d[0] = ws;
+        g.ldd = ldd;
+        md[0] = {ws, ldd, rows, cout, ldd};
+    }
+    g.sums = dbias ? reinterpret_cast<float *>(ws + space.d) : nullptr;
+    Args px = product(rows, cin, cout), pw[2];
+    const int order_x = w_transposed ? kOuter : kInner;
+    const bool want_x = dx && rows > 0;
+    if (want_x) {
+        set_operands(px, md[0], &mw, 1);
+        if (w_transposed) px.load_n = (int)mw.wide;
+        px.c[0] = dx;
+        px.ldc = lddx;
+        FPN_FF_TRY(check_product(dtype, px, kInner, order_x, false));
+    }
+    void *const dw_out[2] = {dw, nullptr};
+    if (dw) {
+        weight_products(mx, md, 1, dw_out, lddw, w_transposed, pw);
+        FPN_FF_TRY(check_product(dtype, pw[0], kOuter, kOuter, false));
+    }
+
+    FPN_FF_TRY(copies.make(st));
     if (act || dbias) {
-        GradArgs g = {};
-        g.rows = rows;
-        g.n = cout;
-        g.dy = dy;
-        g.lddy = lddy;
-        g.pre[0] = pre;
-        g.ldp = ldp;
-        g.act = activation;
-        if (act) {
-            const long ldd = padded(dtype, cout);
-            g.d[0] = ws;
-            g.ldd = ldd;
-            md[0] = {ws, ldd, rows, cout, ldd};
-        }
-        g.sums = dbias ? reinterpret_cast<float *>(ws + space.d) : nullptr;
         void *const out[2] = {dbias, nullptr};
         FPN_FF_TRY(run_grad(dtype, g, false, false, out, st));
     }
-    if (dx && rows > 0) {
-        Args p = product(rows, cin, cout);
-        set_operands(p, md[0], &mw, 1);
-        if (w_transposed) p.load_n = (int)mw.wide;
-        p.c[0] = dx;
-        p.ldc = lddx;
-        FPN_FF_TRY(run_product(dtype, p, kInner, w_transposed ? kOuter : kInner, false, partial, space.partial, st));
-    }
-    if (dw) {
-        void *const out[2] = {dw, nullptr};
-        FPN_FF_TRY(weight_gradients(dtype, mx, md, 1, out, lddw, w_transposed, partial, space.partial, st));
-    }
+    if (want_x) FPN_FF_TRY(run_product(dtype, px, kInner, order_x, false, partial, space.partial, st));
+    if (dw) FPN_FF_TRY(run_product(dtype, pw[0], kOuter, kOuter, false, partial, space.partial, st));
     return FPN_OK;
 }
 
@@ -683,14 +697,14 @@ int fpn_gated(int dtype, long rows, int cin, int cout, const void *x, long ldx, 
     const hipStream_t st = as_stream(stream);
     Matrix mx = {x, ldx, rows, cin, cin}, mw[2] = {weights(w_gate, ldg, cin, cout, w_transposed), weights(w_up, ldu, cin, cout, w_transposed)};
     size_t partial_space = workspace_bytes;
+    Copies copies(dtype, nullptr, 0);
     if (worth_copies(rows, cin, cout)) {
         const size_t partial = align256(partial_bytes(dtype, rows, cout, cin, 1, 1, true, kInner));
         if (workspace && workspace_bytes > partial) {
-            Copies copies(dtype, reinterpret_cast<char *>(workspace) + partial, workspace_bytes - partial);
+            copies = Copies(dtype, reinterpret_cast<char *>(workspace) + partial, workspace_bytes - partial);
             copies.take(mx, false);
             copies.take(mw[0], order_b == kOuter);
             copies.take(mw[1], order_b == kOuter);
-            FPN_FF_TRY(copies.make(st));
             partial_space = partial;
         }
     }
@@ -705,6 +719,8 @@ int fpn_gated(int dtype, long rows, int cin, int cout, const void *x, long ldx, 
     p.pre[0] = gate;
     p.pre[1] = up;
     p.ldp = ldp;
+    FPN_FF_TRY(check_product(dtype, p, kInner, order_b, true));
+    FPN_FF_TRY(copies.make(st));
     return run_product(dtype, p, kInner, order_b, true, reinterpret_cast<float *>(workspace), partial_space, st);
 }
 
@@ -756,13 +772,12 @@ int fpn_gated_grad(int dtype, long rows, int cin, int cout, int cdown, const voi
         if (dw_gate) copies.take(mx, true);
         if (dx) copies.take(mw[0], w_transposed);
         if (dx) copies.take(mw[1], w_transposed);
-        FPN_FF_TRY(copies.make(st));
     }
-    if (cdown && rows > 0 && worth_copies(rows, cdown, cout)) {
-        Copies more(dtype, copies.at, copies.left);
+    const bool down = cdown && rows > 0;
+    Copies more(dtype, copies.at, copies.left);
+    if (down && worth_copies(rows, cdown, cout)) {
         more.take(mdy, false);
         more.take(mdown, order_down == kOuter);
-        FPN_FF_TRY(more.make(st));
     }
 
     const long ldd_own = padded(dtype, cout);
@@ -781,51 +796,60 @@ int fpn_gated_grad(int dtype, long rows, int cin, int cout, int cdown, const voi
     const Matrix md[2] = {{g.d[0], ldd_own, rows, cout, ldd_own}, {g.d[1], ldd_own, rows, cout, ldd_own}};
     g.sums = dbias_gate ? reinterpret_cast<float *>(ws + space.d) : nullptr;
     void *const sums_out[2] = {dbias_gate, dbias_up};
-    bool done = false;
-    if (cdown && rows > 0) {                      // dh = dy w_down^T, never rounded to 16 bits
-        Args p = product(rows, cout, cdown);
-        set_operands(p, mdy, &mdown, 1);
-        if (order_down == kOuter) p.load_n = (int)mdown.wide;
-        const Plan plan = plan_of(dtype, p, kInner, order_down, false);
-        done = plan.wide && plan.splits == 1;
-        if (done) {                               // dg and du straight from the product's epilogue
-            p.c[0] = g.d[0];
-            p.c[1] = g.d[1];
-            p.ldc = ldd_own;
-            p.act = activation;
-            p.gate = gate;
-            p.up = up;
-            p.ldp = ldp;
-            p.sums = g.sums;
+    Args ph = product(rows, cout, cdown), px = product(rows, cin, cout), pw[2];
+    Plan plan_h = {};
+    bool fused = false;                           // dg and du straight from the product that forms dh
+    if (down) {                                   // dh = dy w_down^T, never rounded to 16 bits
+        set_operands(ph, mdy, &mdown, 1);
+        if (order_down == kOuter) ph.load_n = (int)mdown.wide;
+        plan_h = plan_of(dtype, ph, kInner, order_down, false);
+        fused = plan_h.wide && plan_h.splits == 1;
+        if (fused) {
+            ph.c[0] = g.d[0];
+            ph.c[1] = g.d[1];
+            ph.ldc = ldd_own;
+            ph.act = activation;
+            ph.gate = gate;
+            ph.up = up;
+            ph.ldp = ldp;
+            ph.sums = g.sums;
         } else {
-            p.c[0] = ws + space.d + space.sums;
-            p.ldc = cout;
-            p.c_float = true;
-            g.dy = p.c[0];
+            ph.c[0] = ws + space.d + space.sums;
+            ph.ldc = cout;
+            ph.c_float = true;
+            g.dy = ph.c[0];
             g.lddy = cout;
         }
-        FPN_FF_TRY(run_product(dtype, p, kInner, order_down, false, partial, space.partial, st));
-        if (done && g.sums) {
-            const int rows_each = plan.bn == 256 ? 128 : plan.bm == 256 ? 64 : 32;       // (of a wave: 32 TM of feed_forward_wide.h)
-            FPN_FF_TRY(run_column_join(dtype, cout, (int)((rows + plan.bm - 1) / plan.bm * (plan.bm / rows_each)), g.sums, sums_out, st));
+        FPN_FF_TRY(check_product(dtype, ph, kInner, order_down, false));
+    }
+    const int order_x = w_transposed ? kOuter : kInner;
+    const bool want_x = dx && rows > 0;
+    if (want_x) {                                 // dg Wg^T + du Wu^T: one sum over both
+        px.segs = 2;
+        set_operands(px, md[0], mw, 2);
+        px.a[1] = md[1].p;
+        px.lda[1] = md[1].ld;
+        if (w_transposed) px.load_n = (int)std::min(mw[0].wide, mw[1].wide);
+        px.c[0] = dx;
+        px.ldc = lddx;
+        FPN_FF_TRY(check_product(dtype, px, kInner, order_x, false));
+    }
+    void *const dw_out[2] = {dw_gate, dw_up};
+    const int dws = dw_gate ? weight_products(mx, md, 2, dw_out, lddw, w_transposed, pw) : 0;
+    for (int i = 0; i < dws; ++i) FPN_FF_TRY(check_product(dtype, pw[i], kOuter, kOuter, false));
+
+    FPN_FF_TRY(copies.make(st));
+    FPN_FF_TRY(more.make(st));
+    if (down) {
+        FPN_FF_TRY(run_product(dtype, ph, kInner, order_down, false, partial, space.partial, st));
+        if (fused && g.sums) {
+            const int rows_each = plan_h.bn == 256 ? 128 : plan_h.bm == 256 ? 64 : 32;       // (of a wave: 32 TM of feed_forward_wide.h)
+            FPN_FF_TRY(run_column_join(dtype, cout, (int)((rows + plan_h.bm - 1) / plan_h.bm * (plan_h.bm / rows_each)), g.sums, sums_out, st));
         }
     }
-    if (!done) FPN_FF_TRY(run_grad(dtype, g, true, cdown && rows > 0, sums_out, st));
-    if (dx && rows > 0) {                         // dg Wg^T + du Wu^T: one sum over both
-        Args p = product(rows, cin, cout);
-        p.segs = 2;
-        set_operands(p, md[0], mw, 2);
-        p.a[1] = md[1].p;
-        p.lda[1] = md[1].ld;
-        if (w_transposed) p.load_n = (int)std::min(mw[0].wide, mw[1].wide);
-        p.c[0] = dx;
-        p.ldc = lddx;
-        FPN_FF_TRY(run_product(dtype, p, kInner, w_transposed ? kOuter : kInner, false, partial, space.partial, st));
-    }
-    if (dw_gate) {
-        void *const out[2] = {dw_gate, dw_up};
-        FPN_FF_TRY(weight_gradients(dtype, mx, md, 2, out, lddw, w_transposed, partial, space.partial, st));
-    }
+    if (!fused) FPN_FF_TRY(run_grad(dtype, g, true, down, sums_out, st));
+    if (want_x) FPN_FF_TRY(run_product(dtype, px, kInner, order_x, false, partial, space.partial, st));
+    for (int i = 0; i < dws; ++i) FPN_FF_TRY(run_product(dtype, pw[i], kOuter, kOuter, false, partial, space.partial, st));
     return FPN_OK;
 }
 

@@ -28,6 +28,7 @@ template <int BM_, int BN_, int WM_, int WN_, int STAGES, int PER_CU> struct Sha
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, kStages = STAGES;
     static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves, TM = BM / WM / 32, TN = BN / WN / 32;
     static constexpr int kStage = (BM + BN) * kStretch;            // bytes: BM rows of a, BN of b
+    static_assert(kThreads == wide_threads(BM), "what the host checks a grid with");
     static constexpr int kPerSimd = kWaves * PER_CU / 4;               // waves
     static constexpr int kEpilogueBytes = epilogue_bytes(TN);
     static constexpr int kBytes = std::max(kStages * kStage, kWaves * kEpilogueBytes);

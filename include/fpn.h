@@ -759,8 +759,8 @@ int fpn_detection_records(int b, int n, const float *mask_logits, const float *b
  *
  *   - every matrix of a call has the call's element type (FPN_F32, FPN_BF16, FPN_F16); sums are fp32;
  *   - "ld" arguments are row strides in elements, at least the matrix' width (x and residual: or 0, one row for all)
- *     and below 2^21; widths below 2^21; any alignment of an element; up to 2^38 rows, and what a launch of fewer than
- *     2^32 threads takes (at least 2^24 tiles of 64 x 64);
+ *     and below 2^21; widths below 2^21; any alignment of an element; up to 2^38 rows, and results of what a
+ *     launch of fewer than 2^32 threads takes (fewer than 2^23 tiles of 64 x 64 always fit; refused before anything is launched);
  *   - w_transposed 0: weights (cin,cout); 1: held (cout,cin), row stride >= cin;
  *   - rows 0 is a valid call: forward writes nothing, weight and bias gradients become 0;
  *   - outputs may not share memory with inputs, except y with residual (same address and stride);

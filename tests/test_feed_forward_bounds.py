@@ -50,3 +50,30 @@ def test_workspaces_of_the_largest_sizes_are_whole(t, size):
         code = L.fpn_gated_grad(t, rows, WIDE, WIDE, WIDE, P, WIDE, P, WIDE, 0, P, WIDE, P, WIDE, P, WIDE, 0, P, P, WIDE, 2, P, WIDE, P, P,
                                 WIDE, P, P, P, need - 1, None)
         assert code == -1 and "workspace" in said()
+
+
+ROWS = 1 << 34
+CALLS = {
+    # ragged rows, so that copies would be made first; activations and biases, so that dpre and its sums would
+    "dense": lambda L, t: L.fpn_dense(t, ROWS, 515, 259, P, 515, P, 259, 0, P, 2, None, 0, P, 259, P, 259, P, 1 << 60, None),
+    "dense_grad": lambda L, t: L.fpn_dense_grad(t, ROWS, 515, 259, P, 259, P, 515, P, 259, 0, P, 259, 2, P, 515, P, 259, P, P, 1 << 60, None),
+    "dense_grad, no activation": lambda L, t: L.fpn_dense_grad(t, ROWS, 515, 259, P, 259, P, 515, P, 259, 0, None, 0, 0, P, 515, P, 259, P, P,
+                                                               1 << 60, None),
+    "dense_grad, held (out,in)": lambda L, t: L.fpn_dense_grad(t, ROWS, 512, 256, P, 256, P, 512, P, 512, 1, P, 256, 2, P, 512, P, 512, P, P,
+                                                               1 << 60, None),
+    "gated": lambda L, t: L.fpn_gated(t, ROWS, 515, 259, P, 515, P, 259, P, 259, 0, P, P, 2, P, 259, P, P, 259, P, 1 << 60, None),
+    "gated_grad": lambda L, t: L.fpn_gated_grad(t, ROWS, 515, 259, 0, P, 259, None, 0, 0, P, 515, P, 259, P, 259, 0, P, P, 259, 2, P, 515, P, P,
+                                                259, P, P, P, 1 << 60, None),
+    "gated_grad, down projection only": lambda L, t: L.fpn_gated_grad(t, ROWS, 515, 259, 131, P, 131, P, 131, 0, P, 515, P, 259, P, 259, 0, P, P,
+                                                                      259, 2, None, 0, None, None, 0, P, P, P, 1 << 60, None),
+    "gated_grad, whole rows": lambda L, t: L.fpn_gated_grad(t, ROWS, 512, 256, 128, P, 128, P, 128, 0, P, 512, P, 256, P, 256, 0, P, P, 256, 2, P,
+                                                            512, P, P, 256, P, P, P, 1 << 60, None),
+}
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("call", list(CALLS))
+def test_a_product_beyond_one_launch_is_refused_before_any_launch(call, t):
+    """Also where copies, dpre or another product come before it.  (Without a device a launch fails with another code.)"""
+    assert CALLS[call](lib(), t) == -3, said()
+    assert "workgroups" in said()
