@@ -406,17 +406,20 @@ int launch_fps_wave(int b, int n, int m, const float *inp, int *out, hipStream_t
     return check_launch("fpn_farthest_point_sample");
 }
 
-// Which kernel a call takes: the wave-per-frustum form from kFpsWaveMinBatch frustums on
-// (at least one wave for every SIMD of the chip) for 257..2048 points; FPN_FPS=block /
-// FPN_FPS=wave force one form where it exists (the two are bit-identical: tests use both).
-constexpr int kFpsWaveMinBatch = 1024;
+// Which kernel a call takes: for 257..2048 points the wave-per-frustum form from so many frustums on; FPN_FPS=block /
+// FPN_FPS=wave force one form where it exists (the two are bit-identical: tests use both).  Both forms' instructions are
+// scalar fp32 ones; block : wave, us, 128 points picked of
+//   2048   1024 frustums 117 : 131   1536 156 : 171   1792 181 : 175   2048 196 : 179   4096 400 : 302
+//   1024                  82 :  76        109 : 103        120 : 103        134 : 105        263 : 177   (1152: 95 : 103)
+//   512                   54 :  58         72 :  65         72 :  65         73 :  65        136 : 102
+constexpr int fps_wave_min_batch(int n) { return n > 1024 ? 1792 : 1536; }
 inline bool fps_use_wave(int b, int n)
 {
     if (n <= 256 || n > 2048) return false;
     const char *e = std::getenv("FPN_FPS");
     if (e && e[0] == 'b') return false;
     if (e && e[0] == 'w') return true;
-    return b >= kFpsWaveMinBatch;
+    return b >= fps_wave_min_batch(n);
 }
 
 // ---------------------------------------------------------------------------
