@@ -445,8 +445,8 @@ struct StagedConsts {
     }
 };
 
-// relu(acc + shift) as the next layer's operand, three instructions per register pair:
-// packed add, packed conversion, and the clamp as a packed 16-bit INTEGER max with 0 on
+// relu(acc + shift) as the next layer's operand, four instructions per register pair:
+// two adds, a packed conversion, and the clamp as a packed 16-bit INTEGER max with 0 on
 // the bf16 bit patterns (negative floats, -0 included, are the negative integers).
 __device__ __forceinline__ void finish(Act &o, const floatx16 &a, const TileConst &sh)
 {
@@ -1477,8 +1477,7 @@ __device__ __forceinline__ void tail_round(const Act (&pf)[NP][2], const float *
         }
     }
     // conv10 (128 -> 2) in fp32 on the vector ALU, as in seg_tail_bf16_kernel: per point group the same fused
-    // multiply-adds in the same order.  Both logits of a channel in one packed instruction (no MFMA runs beside
-    // these, where a packed instruction would cost more than its two halves), the point groups side by side - one
+    // multiply-adds in the same order.  Both logits of a channel and the point groups side by side - one
     // LDS read of a weight pair serves both, and their sums are independent chains - and the bias from LDS: read
     // from memory here, it was a whole trip to memory with nothing else to do.
     floatx2 s01[NP];

@@ -112,9 +112,8 @@ __device__ __forceinline__ void load_const(TileConst &c, const float *__restrict
 
 typedef float floatx2 __attribute__((ext_vector_type(2)));
 
-// a = relu(a * sc + sh) in place.  The multiply-add is written on register pairs so that
-// it becomes v_pk_fma_f32 (two results per instruction): vector-ALU instructions issued
-// next to the MFMA stream are not free, each costs it a few cycles.
+// a = relu(a * sc + sh) in place, a multiply-add and a maximum per value (no packed fp32: the library is built
+// without).  Vector-ALU instructions issued next to the MFMA stream are not free, each costs it a few cycles.
 __device__ __forceinline__ void bn_relu(floatx16 &a, const TileConst &sc, const TileConst &sh)
 {
 #pragma unroll
@@ -488,7 +487,7 @@ __device__ __forceinline__ void max_points(const floatx16 &acc, float sc, float 
     float m = 0.f;
     const floatx2 s2 = {sc, sc}, b2 = {sh, sh};
 #pragma unroll
-    for (int r = 0; r < 16; r += 2) {     // v_pk_fma_f32 + v_max3_f32 per register pair
+    for (int r = 0; r < 16; r += 2) {     // two multiply-adds + v_max3_f32 per register pair
         const floatx2 v = {acc[r], acc[r + 1]};
         const floatx2 y = v * s2 + b2;
         m = fmaxf(m, fmaxf(y[0], y[1]));

@@ -82,10 +82,9 @@ __global__ __launch_bounds__(THREADS) void fps_kernel(int n, int m, const float 
     for (int i = tid; i < n * 3; i += THREADS) sxyz[i] = pts[i];
     __syncthreads();
 
-    // The thread's points are kept as PAIRS: the subtract / multiply / add chain of the
-    // squared distance then runs on the packed fp32 instructions (v_pk_add_f32,
-    // v_pk_mul_f32: two IEEE-rounded results per instruction, same values as the scalar
-    // forms), which is what bounds this kernel once several frustums share a CU.
+    // The thread's points are kept as PAIRS: two independent subtract / multiply / add chains of
+    // the squared distance side by side (scalar fp32 instructions: the library is built without
+    // the packed ones), which bound this kernel once several frustums share a CU.
     constexpr int NP = (PPT + 1) / 2;   // with an odd PPT the last pair's second half is unused
     float2v px[NP], py[NP], pz[NP];
 #pragma unroll
@@ -239,10 +238,9 @@ int launch_fps(int b, int n, int m, const float *inp, int *out, hipStream_t st)
 // whole run, PPL = 32 for 2048 points: 128 registers, three waves per SIMD - and the waves
 // of a SIMD belong to different frustums, so one wave's dependent steps (the cross-lane
 // maximum, the picked point's coordinates coming back from memory) are covered by the
-// others' distance updates.  Per point and iteration: the packed subtract / multiply / add
-// chain (4 instructions for the exactly rounded squared distance), one minimum and half a
-// maximum - 5.5 against 8, and a per-iteration overhead (reduction, search) that is spread
-// over 32 points per lane instead of 8.
+// others' distance updates.  Per point and iteration: the subtract / multiply / add chain (8
+// instructions for the exactly rounded squared distance), one minimum and half a maximum, and a
+// per-iteration overhead (reduction, search) that is spread over 32 points per lane instead of 8.
 //
 // Lowest index among equal maxima (the tie rule of the workgroup kernel): the lane maximum
 // is a maximum of VALUES only, formed over groups of four positions; after the wave maximum
@@ -500,9 +498,8 @@ __global__ __launch_bounds__(kQbThreads) void query_ball_kernel(
     const int q0 = blk.x * qpb, q1 = min(m, q0 + qpb);
 
     // the tile as three arrays (x | y | z, tile_pts even): a lane tests the points 2 lane and
-    // 2 lane + 1 of a 128-point step, read as 8-byte pairs, on the packed fp32 instructions
-    // (v_pk_add_f32 / v_pk_mul_f32: two IEEE-rounded results per instruction, the values of the
-    // scalar forms) - this kernel is bound by its vector instructions.  (Four points per lane
+    // 2 lane + 1 of a 128-point step, read as 8-byte pairs: half the LDS instructions and steps of
+    // one point per lane - this kernel is bound by its vector instructions.  (Four points per lane
     // and step were measured too: 3 % faster on 2048-point sets, 30 % slower on 128-point ones.)
     float *tx = smem, *ty = smem + tile_pts, *tz = smem + 2 * tile_pts;
     int *s_cnt = reinterpret_cast<int *>(smem + tile_pts * 3); // qpb
