@@ -11,7 +11,9 @@
 // lines, and the halves of a line asked for a stage apart were fetched twice (the product above: 241 us, in pairs 224; with
 // 64 x 64 tiles 532 and 403).  A pair is asked for as soon as everyone has read the one that had its place, half of it
 // behind the barrier and half in the next step; a wave reads the next half stage while it multiplies the present one:
-// one barrier per pair (two in the largest shape), nothing else waits.
+// one barrier per pair, nothing else waits.  (A second one between a pair's two stages makes no difference in the largest shape,
+// twelve alternating runs each: gated 8192 x 2048 x 2 x 8192 455 - 461 us with it and 456 - 466 without, the product above
+// 220.4 - 221.0 and 220.6 - 221.5, weights held (out,in) 219.7 - 221.0 and 218.8 - 219.8; the smaller are up to 2 % slower with it.)
 //
 // The requests are written in assembly because the compiler, which cannot tell the stages apart, would wait for all of
 // them before every LDS read.  They have no result registers; the counts in `arrive` are theirs alone, since the loop
@@ -315,9 +317,6 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void wide_product_kernel(
             int pair = 0;                                   // its first stage
             for (long t = 1; t < n; t += 2) {
                 step(fa[0], fb[0], fa[1], fb[1], lds + pair * kStage, 1, ActTag<kPer>(), pair ? pair - 2 : kStages - 2);
-                // (needless, but it keeps the waves of a large tile at the same lines: gated 8192 x 2048 x 2 x 8192 482 us, without 494;
-                // the smaller tiles are up to 2 % faster without)
-                if constexpr (S::BN == 256) arrive<(kStages - 2) * kPer>();
                 step(fa[1], fb[1], fa[0], fb[0], lds + (pair + 1) * kStage, 0, ActTag<-1>(), 0);
                 step(fa[0], fb[0], fa[1], fb[1], lds + (pair + 1) * kStage, 1, ActTag<-1>(), 0);
                 aim();
