@@ -38,11 +38,18 @@ def _no_tangent(name, t):
         raise NotImplementedError("%s carries a tangent: the feed-forward operators have no forward-mode derivatives" % name)
 
 
+def _as_it_is(name, t):
+    """Refuses a tensor whose memory does not say all of it."""
+    _no_tangent(name, t)
+    if t.is_neg():
+        raise ValueError("%s has a pending negation: call its resolve_neg() first" % name)
+
+
 def _tensor(name, t, like, shape):
     """The checks that every argument gets: a tensor of the call's type, on its device, of this shape."""
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s must be a torch.Tensor, got %s" % (name, type(t).__name__))
-    _no_tangent(name, t)
+    _as_it_is(name, t)
     if t.dtype is not like.dtype:
         raise ValueError("%s must be %s like x, got %s" % (name, like.dtype, t.dtype))
     if not t.is_cuda:
@@ -56,7 +63,7 @@ def _tensor(name, t, like, shape):
 def _first(name, x):
     if not isinstance(x, torch.Tensor):
         raise TypeError("%s must be a torch.Tensor, got %s" % (name, type(x).__name__))
-    _no_tangent(name, x)
+    _as_it_is(name, x)
     if x.dim() != 2:
         raise ValueError("%s must have rank 2, got shape %s" % (name, tuple(x.shape)))
     if x.dtype not in _DTYPES:
@@ -279,7 +286,8 @@ def _dense_backward(dtype, sizes, dy, lddy, x, ldx, w, ldw, transposed, pre, ldp
 
 def _kept(name, t, x, shape):
     """The row stride of a pre-activation that a forward pass kept."""
-    _no_tangent(name, t)
+    if isinstance(t, torch.Tensor):
+        _as_it_is(name, t)
     if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or not t.is_cuda or t.get_device() != x.get_device() or t.shape != shape:
         raise ValueError("%s must be the float32 %s tensor on %s that keep=True returned" % (name, tuple(shape), x.device))
     return _rows(name, t)
@@ -293,7 +301,8 @@ def _weight_gradient(like, cin, cout, transposed):
 
 
 def _dense_rows(t):
-    """A gradient as autograd hands it over (it may be an expanded or transposed view), with dense rows."""
+    """A gradient as autograd hands it over (it may be an expanded, transposed or negated view), with dense rows."""
+    t = t.resolve_neg()
     if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
         return t.contiguous()
     return t
