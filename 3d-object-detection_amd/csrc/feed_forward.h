@@ -122,8 +122,9 @@ template <int ACT, bool EXACT> __device__ inline float activate(float v)
     return v;
 }
 
-// act(v) and act'(v).  1 - sigmoid(z) is taken as sigmoid(-z) (no cancellation); products that would be 0 * infinity
-// in the far tails are cut off where the derivative is 0 or 1 to all bits.
+// act(v) and act'(v).  1 - sigmoid(z) is taken as sigmoid(-z) (no cancellation); GELU's products that would be
+// 0 * infinity in the far tails are cut off where the derivative is 0 or 1 to all bits.  (SiLU is finite wherever v is; at an
+// infinity it is NaN, as its formula.)
 template <int ACT, bool EXACT> __device__ inline float activate_grad(float v, float &value)
 {
     if (ACT == FPN_ACT_RELU) {
@@ -598,8 +599,8 @@ __device__ inline void store_piece(const Args &p, const floatx16 (&acc)[TM][TN],
                 }
             }
             if constexpr (MODE == kGateGradMode) {
-                // the gated block's backward pass: dh in, dg and du out (no bias in such a product: its registers
-                // take the column sums)
+                // the gated block's backward pass: dh in, dg and du out, rounded to T as the next products' operands like
+                // grad_kernel's (no bias in such a product: its registers take the column sums)
                 float g[kBatch][8], u[kBatch][8];
 #pragma unroll
                 for (int b = 0; b < kBatch; ++b) {

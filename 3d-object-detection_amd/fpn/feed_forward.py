@@ -5,6 +5,18 @@ backward, through libfpn_hip.so (fpn_dense, fpn_dense_grad, fpn_gated, fpn_gated
     gated               h = act(x w_gate + bias_gate) * (x w_up + bias_up)
     gated_feed_forward  y = gated(x) w_down + bias_down + residual
 
+In 16-bit types every result is rounded once, and so are the operands that one product hands to the next, which the matrix
+units take in 16 bits: h between gated and the down projection, and dpre (dg, du) before dx and the weights' gradients.  Against
+float64 the error of those results is up to about sqrt 2 of one rounding's: relative to the norm 2.3e-3 for the weights'
+gradients of a bf16 block of 4096 x 1024 x 4096 (one rounding 1.7e-3), 1.9e-3 for its y; 2.9e-4 for dx and dw of an fp16 step of
+1999 x 1091 x 515 (one rounding 2.1e-4).  Kept pre-activations, dh of the block, sums and column sums are fp32.
+
+Which to use in fp32 with bias and ReLU, where both exist: `dense` is the faster for single rows and for many rows of whole
+16-byte chunks (us, dense : shared_mlp: 1 x 1027 x 512 6 : 13, 131072 x 128 x 256 89 : 133, 8192 x 512 x 512 40 : 63,
+131072 x 512 x 1024 1013 : 1346), `ops.shared_mlp` for widths that are not (1024 x 1027 x 512 26 : 18) and where it pools or
+scales.  From two to 64 rows at such widths `dense` takes 15 us where whole ones take 6 to 9 (2 to 64 x 1027 x 512 against 1024):
+the kernel for few rows reads whole chunks only.
+
 They stand beside `ops.shared_mlp` (fp32, scale / shift / ReLU, pooling): every tensor of a call is float32, bfloat16
 or float16, sums are fp32, weights are (in, out) - or the `.t()` view of weights held (out, in) -, rows may lie apart
 (column slices of wider buffers).  Work is enqueued on the current stream of the tensors' device; nothing synchronises.
@@ -34,13 +46,14 @@ def _activation(name):
 
 def _no_tangent(name, t):
     """Refuses a tensor of forward-mode differentiation: it has a value like any other, and the result would lack a tangent."""
-    if forward_ad._current_level >= 0 and isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+    if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
         raise NotImplementedError("%s carries a tangent: the feed-forward operators have no forward-mode derivatives" % name)
 
 
 def _as_it_is(name, t):
     """Refuses a tensor whose memory does not say all of it."""
-    _no_tangent(name, t)
+    if forward_ad._current_level >= 0:
+        _no_tangent(name, t)
     if t.is_neg():
         raise ValueError("%s has a pending negation: call its resolve_neg() first" % name)
 
@@ -49,7 +62,8 @@ def _tensor(name, t, like, shape):
     """The checks that every argument gets: a tensor of the call's type, on its device, of this shape."""
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s must be a torch.Tensor, got %s" % (name, type(t).__name__))
-    _as_it_is(name, t)
+    if forward_ad._current_level >= 0 or t.is_neg():
+        _as_it_is(name, t)
     if t.dtype is not like.dtype:
         raise ValueError("%s must be %s like x, got %s" % (name, like.dtype, t.dtype))
     if not t.is_cuda:
@@ -321,7 +335,9 @@ class _Dense(torch.autograd.Function):
         else:
             y = dense(x, w, bias, activation, residual)
         ctx.save_for_backward(x if need_w else None, w if need_x else None, pre)
-        ctx.layout = _DTYPES[x.dtype], (x.shape[0], x.shape[1], w.shape[1]), _weights(("w",), (w,))[0], act
+        # (dw is stored as w is: a kept w says how)
+        order = _weights(("w",), (w,))[0] if need_w and not need_x else 0
+        ctx.layout = _DTYPES[x.dtype], (x.shape[0], x.shape[1], w.shape[1]), order, act
         return y
 
     @staticmethod
@@ -444,7 +460,7 @@ class _Gated(torch.autograd.Function):
         need_x, need_g, need_u = ctx.needs_input_grad[:3]
         h, gate, up = gated(x, w_gate, w_up, bias_gate, bias_up, activation, keep=True)
         ctx.save_for_backward(x if need_g or need_u else None, w_gate if need_x else None, w_up if need_x else None, None, gate, up)
-        ctx.layout = _gated_layout(x, w_gate, w_up, 0, activation)
+        ctx.layout = _gated_layout(x, w_gate, w_up, 0, activation, need_x)
         return h
 
     @staticmethod
@@ -454,10 +470,10 @@ class _Gated(torch.autograd.Function):
         return _gated_gradients(ctx.layout, _dense_rows(dh), ctx.saved_tensors, ctx.needs_input_grad[:5]) + (None,)
 
 
-def _gated_layout(x, w_gate, w_up, cdown, activation):
+def _gated_layout(x, w_gate, w_up, cdown, activation, need_x):
     """(dtype, sizes, storage order of the gated weights, activation) of a recorded call."""
-    return (_DTYPES[x.dtype], (x.shape[0], x.shape[1], w_gate.shape[1], cdown), _weights(("w_gate", "w_up"), (w_gate, w_up))[0],
-            ACTIVATIONS[activation])
+    order = 0 if need_x else _weights(("w_gate", "w_up"), (w_gate, w_up))[0]             # (with need_x they are kept and say it)
+    return _DTYPES[x.dtype], (x.shape[0], x.shape[1], w_gate.shape[1], cdown), order, ACTIVATIONS[activation]
 
 
 def _gated_gradients(layout, dh, saved, needs):
@@ -522,7 +538,7 @@ class _GatedFeedForward(torch.autograd.Function):
         y = dense(h, w_down, bias_down, None, residual)
         ctx.save_for_backward(x if need_g or need_u else None, w_gate if need_x else None, w_up if need_x else None,
                               w_down if through else None, gate, up, h if need_d else None)
-        ctx.layout = _gated_layout(x, w_gate, w_up, w_down.shape[1], activation)
+        ctx.layout = _gated_layout(x, w_gate, w_up, w_down.shape[1], activation, need_x)
         ctx.down_transposed = _weights(("w_down",), (w_down,))[0]
         return y
 

@@ -107,7 +107,8 @@ def dropout(inputs, is_training, scope, keep_prob=0.5, noise_shape=None):
 def _projection(scope, cin, cout, use_bias, dtype):
     """A layer's weights (cin, cout) and bias, in the type of its inputs.
 
-    The store holds float32, so 16-bit inputs cost a cast of each variable per call.  It is not kept: a variable may be
+    The store holds float32, so 16-bit inputs cost a cast of each variable per call (bf16 layers of 64 x 256 x 256 9.5 us, the operator
+    alone 5.7; 4096 x 1024 x 1024 24 and 16; 64 x 4096 x 4096 33 and 16).  It is not kept: a variable may be
     trained, written in place or read in a capture or on another stream between two calls, and only a cast of the call's own is
     right in all of these.  A program that keeps 16-bit weights calls feed_forward with them."""
     store = variables.get_default_store()

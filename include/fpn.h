@@ -757,7 +757,8 @@ int fpn_detection_records(int b, int n, const float *mask_logits, const float *b
  * MLP layer (fpn_shared_mlp_f32: fp32, scale / shift / ReLU, pooling) and have what it lacks: bf16 and fp16 storage,
  * residuals, smooth activations, gates and gradients.  No counterpart in the reference.
  *
- *   - every matrix of a call has the call's element type (FPN_F32, FPN_BF16, FPN_F16); sums are fp32;
+ *   - every matrix of a call has the call's element type (FPN_F32, FPN_BF16, FPN_F16); sums are fp32; results are rounded
+ *     once, and in 16-bit types d, dg and du below once before the products that form dx and dw from them;
  *   - "ld" arguments are row strides in elements, at least the matrix' width (x and residual: or 0, one row for all)
  *     and below 2^21; widths below 2^21; any alignment of an element; up to 2^38 rows, and results of what a
  *     launch of fewer than 2^32 threads takes (fewer than 2^23 tiles of 64 x 64 always fit; refused before anything is launched);
