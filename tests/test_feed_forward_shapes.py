@@ -170,3 +170,36 @@ def test_gated_epilogues_of_every_shape(device, t, cols, rows, cin, n):
         near(dwu, x6.t() @ du, max(rows, cin), 2, "dwu")
         near(dbg, dg.sum(0), max(rows, cin), 1, "dbg")
         near(dbu, du.sum(0), max(rows, cin), 1, "dbu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("cols", [False, True])
+@pytest.mark.parametrize("rows,cin,n", SIZES)
+def test_a_block_rounds_no_more_than_twice(device, t, cols, rows, cin, n):
+    """gated_feed_forward and its gradients through autograd, relative to their norms: every result is rounded once, and of the
+    operands that one product hands to the next h (to y and dw_down) and dg, du (to dx and the gated weights' gradients) once
+    more, each time by at most u of every value - at most u of the norm.  The biases' gradients come from the unrounded
+    values.  fp32 sums add 10 2^-24 sqrt k as above."""
+    from fpn import feed_forward as F
+    dtype, u = TYPES[t]
+    a = inputs(device, dtype, rows, cin, n, cols)
+    g = torch.Generator(device=device).manual_seed(5)
+    a["bd"], a["res"] = ((torch.randn(s, generator=g, device=device) * 0.3).to(dtype) for s in ((cin,), (rows, cin)))
+    names = ("x", "wg", "wu", "wd", "bg", "bu", "bd", "res")
+    leaves = [a[k].detach().requires_grad_() for k in names]
+    y = F.gated_feed_forward(*leaves[:7], "silu", leaves[7])
+    got = dict(zip(names, torch.autograd.grad(y, leaves, a["dy"])), y=y.detach())
+    x, wg, wu, wd, bg, bu, bd, res = (a[k].double() for k in names)
+    dy = a["dy"].double()
+    pg, pu = x @ wg + bg, x @ wu + bu
+    v, slope = act64(pg, "silu")
+    h, dh = v * pu, dy @ wd.t()
+    dg, du = dh * pu * slope, dh * v
+    want = {"y": h @ wd + bd + res, "wd": h.t() @ dy, "bd": dy.sum(0), "x": dg @ wg.t() + du @ wu.t(), "wg": x.t() @ dg, "wu": x.t() @ du,
+            "bg": dg.sum(0), "bu": du.sum(0)}
+    assert torch.equal(got["res"], a["dy"])
+    for k, w in want.items():
+        halves = 1 if k in ("bd", "bg", "bu") else 2
+        off = float((got[k].double() - w).norm() / w.norm())
+        assert off <= halves * u + 10 * 2.0 ** -24 * max(rows, cin, n) ** 0.5, (k, off)
